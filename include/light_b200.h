@@ -365,6 +365,93 @@ typedef struct lb200_decode_attn_args {
  * caller composes the op as it does today, ops/decode_attn.go:116-170). */
 LB200_API int light_b200_decode_attn(const lb200_decode_attn_args *args, int device, void *stream);
 
+/* ---- many sequences over one paged key-value cache
+ *
+ * The reference holds one contiguous cache per sequence and decodes one sequence (models/llama.go:438-640); a server of many, each of its
+ * own age, keeps keys and values in a pool of pages of page_size rows.  Row `slot` of the pool is row slot % page_size of page
+ * slot / page_size; sequence b's token j is on page block_table[b][j / page_size], row j % page_size.  Keys and values are two arrays
+ * addressed by three strides each (page, head, row; in ELEMENTS), the D elements of a head's row being consecutive: any order of page,
+ * head and row is a cache.  One step:
+ *
+ *   light_b200_paged_advance       pages for the step's new tokens out of a stack of free ones; slot and position of each
+ *   light_b200_qk_norm_rope        per layer: q and k normed per head, rotated, k and v into their rows
+ *   light_b200_paged_decode_attn   per layer: one query token of each sequence over its rows
+ *   light_b200_paged_release       when sequences end: their pages back on the stack
+ *
+ * All of it reads lengths, tables and positions on the device: a step is the same launches whatever they are (graph-capturable). */
+
+/* 0, or of the calls so far on this device (synchronises): bit 0: a length outside [0, W page_size] reached the attention (it used the
+ * nearest inside); bit 1: a page outside [0, pages) did (its keys counted as absent); bit 2: a slot at or beyond pages * page_size
+ * reached qk_norm_rope (nothing was written for it); bit 3: paged_advance left a request without its tokens, or it or
+ * paged_release met a negative length or a count outside [0, capacity]. */
+LB200_API int light_b200_paged_status(int device);
+
+#define LB200_PAGED_MAX_REQUESTS 8192
+typedef struct lb200_paged_pages {
+  int32_t *block_table;       /* (B, W) page ids, rows table_stride apart                                                  */
+  const int32_t *lens;        /* (B) tokens of each request in the cache                                                   */
+  const int32_t *new_lens;    /* advance: (B) tokens of each request in this step                                          */
+  const uint8_t *done;        /* release: (B) nonzero: the request has ended                                               */
+  int32_t *free_pages;        /* (capacity) a stack: entries [0, free_count) are the free pages' ids                       */
+  const int32_t *free_count;  /* one element                                                                               */
+  int32_t *lens_out;          /* (B) lengths afterwards; may be lens                                                       */
+  int32_t *granted;           /* advance: (B) new_lens, or 0 for a request that got nothing                                */
+  int32_t *starts;            /* advance: (B + 1) token rows of request b: [starts[b], starts[b + 1])                      */
+  int32_t *free_count_out;    /* one element; may be free_count                                                            */
+  int64_t *positions, *slots; /* advance: (tokens) place in the sequence, row of the pool; 0 and -1 behind the last token  */
+  int64_t table_stride, tokens;
+  int32_t B, W, page_size, capacity;
+} lb200_paged_pages;
+
+/* Request b's tokens lens[b] .. lens[b] + new_lens[b] get pages where the held ones do not reach: the stack's top entries, request after
+ * request.  A request gets all of its pages or none: none when the stack ends before (then no later one that needs a page gets any),
+ * when its tokens do not fit W pages, or when its rows pass `tokens`; its rows then have slot -1 and its length stays.  (Negative lengths
+ * count as 0.)  The stack's entries are left as they are, so a call with the same inputs gives the same pages. */
+LB200_API int light_b200_paged_advance(const lb200_paged_pages *args, int device, void *stream);
+/* Pushes the ceil(lens[b] / page_size) pages of every request marked done, in order, and sets its length to 0.  The table keeps its
+ * entries.  Pages that the stack has no room for are dropped and reported. */
+LB200_API int light_b200_paged_release(const lb200_paged_pages *args, int device, void *stream);
+
+/* Queries and keys of T tokens: y = x * rsqrt(mean(x^2) + eps) * weight over each head's D elements (no weight: y = x), the first `rotary`
+ * of them then rotated in pairs by positions[t] * inv_freq[i] and multiplied by factor; pair i is (i, i + rotary / 2), or (2 i, 2 i + 1)
+ * with interleaved.  Angles in f64, the rest in f32, rounded once.  (Reference ops.RMSNorm over a head and ops.RoPE, ops/norm.go:69-111,
+ * ops/rope.go:30-77, as launches of their own.)
+ * With slots: key and value (copied) of token t go to row slots[t] of the cache instead of k_out; a negative slot writes nothing. */
+typedef struct lb200_qk_norm_rope_args {
+  const void *q, *k, *v;      /* (T, NH, D), (T, KH, D), (T, KH, D): token and head strides below; v with slots only       */
+  const void *q_weight, *k_weight; /* (D) at dtype, or NULL each                                                           */
+  const int64_t *positions;   /* (T)                                                                                       */
+  const int64_t *slots;       /* (T) or NULL                                                                               */
+  const double *inv_freq;     /* (rotary / 2)                                                                              */
+  void *q_out;                /* (T, NH, D) contiguous                                                                     */
+  void *k_out, *v_out;        /* k_out (T, KH, D) contiguous; with slots the cache's keys and values                       */
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  int64_t k_cache_stride[3], v_cache_stride[3], pages;
+  int64_t T;
+  int32_t dtype, NH, KH, D, rotary, interleaved, page_size;  /* dtype LB200_F32 / BF16 / F16; D <= 256                     */
+  float eps, factor;
+} lb200_qk_norm_rope_args;
+LB200_API int light_b200_qk_norm_rope(const lb200_qk_norm_rope_args *args, int device, void *stream);
+
+/* out (B, NH, D) = softmax(s) V over the keys [max(0, lens[b] - window), lens[b]) of sequence b (window 0: all), s = scale q.k, with
+ * softcap > 0 softcap * tanh(scale q.k / softcap).  lens[b] counts the new token, whose key and value are in the cache already.  A
+ * sequence without keys, or whose keys all score -inf, gives zeros.  scratch: device memory of light_b200_paged_attn_scratch_bytes or more, 256-byte aligned,
+ * uninitialised, which nothing else uses until the call has run; 0 bytes where the call has no use for any. */
+typedef struct lb200_paged_attn_args {
+  const void *q;              /* (B, NH, D): token and head strides below                                                  */
+  const void *k, *v;          /* the cache                                                                                 */
+  const int32_t *block_table; /* (B, W), rows table_stride apart                                                           */
+  const int32_t *lens;        /* (B)                                                                                       */
+  void *out;                  /* (B, NH, D) contiguous                                                                     */
+  void *scratch;
+  unsigned long long scratch_bytes;
+  int64_t q_stride[2], k_stride[3], v_stride[3], table_stride, pages;
+  int32_t dtype, B, NH, KH, D, page_size, W, window;  /* dtype of q, k, v, out: LB200_F32 / BF16 / F16; NH % KH == 0; D <= 256 */
+  float scale, softcap;
+} lb200_paged_attn_args;
+LB200_API unsigned long long light_b200_paged_attn_scratch_bytes(const lb200_paged_attn_args *args, int device);
+LB200_API int light_b200_paged_decode_attn(const lb200_paged_attn_args *args, int device, void *stream);
+
 /* Quantized embedding lookup (reference nn.Embedding over a quantized table: ops.IndexSelect of the byte
  * rows + quant.Dequantize of the gathered rows, nn/embedding.go; nn/embedding_test.go:127): out row i =
  * dequantized row ids[i] of the (V, K) table, bit-identical to light_b200_dequant of that row.  ids are

@@ -62,6 +62,29 @@ class DecodeAttnArgs(C.Structure):
     ]
 
 
+class PagedPages(C.Structure):
+    """lb200_paged_pages"""
+    _fields_ = [(n, C.c_void_p) for n in ("block_table", "lens", "new_lens", "done", "free_pages", "free_count", "lens_out", "granted", "starts", "free_count_out",
+                                          "positions", "slots")] + \
+               [("table_stride", C.c_int64), ("tokens", C.c_int64)] + [(n, C.c_int32) for n in ("B", "W", "page_size", "capacity")]
+
+
+class QKNormRopeArgs(C.Structure):
+    """lb200_qk_norm_rope_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_weight", "k_weight", "positions", "slots", "inv_freq", "q_out", "k_out", "v_out")] + \
+               [(n, C.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + [(n, C.c_int64 * 3) for n in ("k_cache_stride", "v_cache_stride")] + \
+               [("pages", C.c_int64), ("T", C.c_int64)] + [(n, C.c_int32) for n in ("dtype", "NH", "KH", "D", "rotary", "interleaved", "page_size")] + \
+               [("eps", C.c_float), ("factor", C.c_float)]
+
+
+class PagedAttnArgs(C.Structure):
+    """lb200_paged_attn_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "block_table", "lens", "out", "scratch")] + \
+               [("scratch_bytes", C.c_ulonglong), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("table_stride", C.c_int64),
+                ("pages", C.c_int64)] + [(n, C.c_int32) for n in ("dtype", "B", "NH", "KH", "D", "page_size", "W", "window")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
 # name -> (restype, argtypes): every symbol include/light_b200.h declares
 SYMBOLS = {
     "light_b200_init": (C.c_int, [C.c_int]),
@@ -129,6 +152,12 @@ SYMBOLS = {
     "light_b200_kv_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                        C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "light_b200_decode_attn": (C.c_int, [C.POINTER(DecodeAttnArgs), C.c_int, C.c_void_p]),
+    "light_b200_paged_advance": (C.c_int, [C.POINTER(PagedPages), C.c_int, C.c_void_p]),
+    "light_b200_paged_release": (C.c_int, [C.POINTER(PagedPages), C.c_int, C.c_void_p]),
+    "light_b200_qk_norm_rope": (C.c_int, [C.POINTER(QKNormRopeArgs), C.c_int, C.c_void_p]),
+    "light_b200_paged_attn_scratch_bytes": (C.c_ulonglong, [C.POINTER(PagedAttnArgs), C.c_int]),
+    "light_b200_paged_decode_attn": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_int, C.c_void_p]),
+    "light_b200_paged_status": (C.c_int, [C.c_int]),
     "light_b200_inc_i64": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "light_b200_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_float,
                                      C.c_int, C.c_void_p]),

@@ -63,6 +63,18 @@ static int bind(int device) {
   return 0;
 }
 
+// A device bound for one call: what was current before is again afterwards.
+struct OnDevice {
+  int before = -1, rc;
+  explicit OnDevice(int device) {
+    if (cudaGetDevice(&before) != cudaSuccess || before == device) before = -1;
+    rc = bind(device);
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
 static bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 }  // namespace lb
@@ -508,6 +520,47 @@ int light_b200_kv_append(const void *k, const void *v, void *kbuf, void *vbuf, c
 int light_b200_decode_attn(const lb200_decode_attn_args *a, int device, void *stream) {
   if (int rc = bind(device)) return rc;
   return decode_attn(a, (cudaStream_t)stream);
+}
+
+int light_b200_paged_advance(const lb200_paged_pages *a, int device, void *stream) {
+  if (int rc = paged_pages_check(a, "paged_advance", false)) return rc;
+  OnDevice on(device);
+  return on.rc ? on.rc : paged_advance(a, (cudaStream_t)stream);
+}
+
+int light_b200_paged_release(const lb200_paged_pages *a, int device, void *stream) {
+  if (int rc = paged_pages_check(a, "paged_release", true)) return rc;
+  OnDevice on(device);
+  return on.rc ? on.rc : paged_release(a, (cudaStream_t)stream);
+}
+
+int light_b200_qk_norm_rope(const lb200_qk_norm_rope_args *a, int device, void *stream) {
+  if (int rc = qk_norm_rope_check(a)) return rc;
+  OnDevice on(device);
+  return on.rc ? on.rc : qk_norm_rope(a, (cudaStream_t)stream);
+}
+
+unsigned long long light_b200_paged_attn_scratch_bytes(const lb200_paged_attn_args *a, int device) {
+  if (paged_attn_check(a)) return 0;
+  OnDevice on(device);
+  return on.rc ? 0 : paged_attn_scratch_bytes(a);
+}
+
+int light_b200_paged_decode_attn(const lb200_paged_attn_args *a, int device, void *stream) {
+  if (int rc = paged_attn_check(a)) return rc;
+  OnDevice on(device);
+  return on.rc ? on.rc : paged_decode_attn(a, (cudaStream_t)stream);
+}
+
+int light_b200_paged_status(int device) {
+  OnDevice on(device);
+  if (on.rc) return on.rc;
+  unsigned int x = 0, y = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_status: %s", cudaGetErrorString(e));
+  if (int rc = paged_attn_status(&x)) return fail(rc, "light_b200: paged_status: %s", cudaGetErrorString((cudaError_t)rc));
+  if (int rc = paged_step_status(&y)) return fail(rc, "light_b200: paged_status: %s", cudaGetErrorString((cudaError_t)rc));
+  return (int)(x | y);
 }
 
 int light_b200_embedding_q(int t, const void *table, const int64_t *ids, float *out, int64_t n_ids, int64_t V, int K, int device,

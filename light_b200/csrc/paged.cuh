@@ -1,0 +1,39 @@
+// What the kernels over a paged key-value cache share: element access at three types, division by a page size, bits of the status word.
+#pragma once
+#include "common.cuh"
+#include "mma_sync.cuh"
+#include "umma.cuh"
+
+namespace lb {
+
+enum { PAGED_LENGTH = 1, PAGED_PAGE = 2, PAGED_SLOT = 4, PAGED_REFUSED = 8 };  // light_b200_paged_status
+
+namespace {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// n / d for 0 <= n < 2^31: n m >> (31 + s) with 2^s >= d and m = ceil(2^(31 + s) / d).  m d exceeds 2^(31 + s) by less than d <= 2^s, so the
+// product's excess stays under 2^(31 + s).
+struct FastDiv {
+  uint32_t m = 0;
+  int s = 0, d = 1;
+  FastDiv() = default;
+  explicit FastDiv(int d_) : d(d_) {
+    while ((1ll << s) < d) s++;
+    m = (uint32_t)(((1ull << (31 + s)) + (unsigned)d - 1) / (unsigned)d);
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(((unsigned long long)(unsigned)n * m) >> (31 + s)); }
+};
+
+}  // namespace
+}  // namespace lb

@@ -1,0 +1,387 @@
+// What a step of a serving loop does around its attention over a paged key-value cache: pages for the new tokens, their return, and the
+// queries and keys of the new tokens normed, rotated and put in their rows.  The reference keeps one contiguous cache per sequence
+// (models/llama.go:438-640) and runs norm and rotation as launches of their own (ops/norm.go:69-111, ops/rope.go:30-77).
+#include "paged.cuh"
+
+namespace lb {
+namespace {
+
+__device__ unsigned int g_step_status = 0;
+
+// ------------------------------------------------------------------------------------ pages
+// Request b holds n_b tokens in held_b = ceil(n_b / P) pages and gets m_b more, which take more_b = ceil((n_b + m_b) / P) - held_b pages:
+// those at first_b, first_b + 1, .. from the top of the stack of free ones, first_b = sum of more_a over a < b.  A request whose pages
+// the stack does not hold gets none, and as first_b never falls, none after it that needs any.  Token i of the batch belongs to the
+// request with starts_b <= i < starts_{b + 1}: a binary search in shared memory.
+//
+// Two dependent reads (the lengths; then the stack or the table) and the stores bound it; the work is one cluster's: every CTA of it scans
+// the lengths for itself, and the barrier between the scan and the stores lets lengths and counter be updated in place.
+constexpr int PG_THREADS = 1024, PG_MAX_B = 8192;
+
+struct PagesArgs {
+  int *table;
+  long long table_stride;
+  const int *lens, *new_lens;
+  const unsigned char *done;
+  int *free_pages;
+  const int *free_count;
+  int *lens_out, *granted, *starts, *count_out;
+  long long *positions, *slots;
+  int B, W, capacity;  // capacity: entries of free_pages
+  FastDiv page;
+  long long tokens;
+};
+
+struct Two {
+  long long a, b;
+};
+// exclusive prefix of v over the CTA's threads, and the total
+__device__ __forceinline__ Two block_scan(Two v, Two &total) {
+  __shared__ Two part[PG_THREADS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Two x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, x.a, o), b = __shfl_up_sync(0xffffffffu, x.b, o);
+    if (lane >= o) x.a += a, x.b += b;
+  }
+  __syncthreads();  // (part may still be read from the call before)
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  Two before = {0, 0}, all = {0, 0};
+  for (int w = 0; w < (int)blockDim.x / 32; w++) {
+    if (w < warp) before.a += part[w].a, before.b += part[w].b;
+    all.a += part[w].a, all.b += part[w].b;
+  }
+  total = all;
+  return {before.a + x.a - v.a, before.b + x.b - v.b};
+}
+
+// the b with at[b] <= i < at[b + 1], for at[0] = 0 <= i < at[n]
+__device__ __forceinline__ int owner_of(const int *at, int n, int i) {
+  int lo = 0, hi = n;  // at[lo] <= i < at[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int saturated(long long v) { return (int)(v < 0x7fffffffll ? v : 0x7fffffffll); }
+
+__global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, int ctas) {
+  extern __shared__ int sm[];
+  int *starts = sm, *first = sm + a.B + 1, *len = first + a.B + 1;  // len: -1 - n for a request that gets nothing
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rank = blockIdx.x, tid = threadIdx.x;
+  const int free_now = a.free_count[0], avail = min(max(free_now, 0), a.capacity);
+  bool odd = free_now != avail;
+  Two carry = {0, 0};
+  long long taken = 0;
+  for (int base = 0; base < a.B; base += blockDim.x) {
+    const int b = base + tid;
+    long long n = 0, m = 0, more = 0;
+    if (b < a.B) {
+      const int n0 = a.lens[b], m0 = a.new_lens[b];
+      odd |= n0 < 0 || m0 < 0;
+      n = max(n0, 0), m = max(m0, 0);
+    }
+    Two total, at = block_scan({m, 0}, total);
+    const long long from = carry.a + at.a;
+    const bool fits = n + m <= (long long)a.W * a.page.d && from + m <= a.tokens;
+    if (b < a.B && fits) {
+      const int held = a.page.div((int)n + 0) + (a.page.div((int)n) * a.page.d < (int)n), want = a.page.div((int)(n + m)) + (a.page.div((int)(n + m)) * a.page.d < (int)(n + m));
+      more = want - held;
+    }
+    Two total2, at2 = block_scan({more, 0}, total2);
+    const long long f = carry.b + at2.a;
+    const bool given = fits && (more == 0 || f + more <= avail);
+    if (b < a.B) {
+      starts[b] = saturated(from), first[b] = saturated(f), len[b] = given ? (int)n : -1 - (int)n;
+      odd |= !given;
+    }
+    carry.a += total.a, carry.b += total2.a;
+  }
+  if (tid == 0) starts[a.B] = saturated(carry.a), first[a.B] = saturated(carry.b);
+  __syncthreads();
+  // pages taken: those of the requests before the first that does not get its own
+  int cut = saturated(carry.b);
+  for (int b = tid; b < a.B; b += blockDim.x)
+    if (len[b] < 0 && first[b + 1] > first[b]) cut = min(cut, first[b]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) cut = min(cut, __shfl_xor_sync(0xffffffffu, cut, o));
+  __shared__ int least;
+  if (tid == 0) least = 0x7fffffff;
+  __syncthreads();
+  if ((tid & 31) == 0) atomicMin(&least, cut);
+  if (ctas > 1) umma::cluster_sync();  // every CTA has read the lengths and the counter
+  else __syncthreads();
+  taken = least;
+  if (odd && rank == 0) atomicOr(&g_step_status, (unsigned)PAGED_REFUSED);
+
+  const int gid = rank * blockDim.x + tid, threads = ctas * blockDim.x;
+  for (int b = gid; b < a.B; b += threads) {
+    const int l = len[b], m = starts[b + 1] - starts[b];
+    a.lens_out[b] = l < 0 ? -1 - l : l + m;
+    a.granted[b] = l < 0 ? 0 : m;
+    a.starts[b] = starts[b];
+  }
+  if (gid == 0) a.starts[a.B] = starts[a.B], a.count_out[0] = avail - (int)taken;
+  auto held_of = [&](int b) {
+    const int n = len[b] < 0 ? -1 - len[b] : len[b], q = a.page.div(n);
+    return q + (q * a.page.d < n);
+  };
+  for (int p = gid; p < (int)taken; p += threads) {
+    const int b = owner_of(first, a.B, p);
+    a.table[(long long)b * a.table_stride + held_of(b) + (p - first[b])] = a.free_pages[avail - 1 - p];
+  }
+  const int given_rows = starts[a.B];
+  for (long long i = gid; i < a.tokens; i += threads) {
+    long long pos = 0, slot = -1;
+    if (i < given_rows) {
+      const int b = owner_of(starts, a.B, (int)i), l = len[b];
+      pos = (long long)(l < 0 ? -1 - l : l) + (int)i - starts[b];
+      if (l >= 0) {
+        const int w = a.page.div((int)pos), x = w - held_of(b);
+        const int pg = x >= 0 ? a.free_pages[avail - 1 - first[b] - x] : a.table[(long long)b * a.table_stride + w];
+        if (pg >= 0) slot = (long long)pg * a.page.d + ((int)pos - w * a.page.d);
+      }
+    }
+    a.positions[i] = pos, a.slots[i] = slot;
+  }
+}
+
+// The pages of the requests marked done, in order, on top of the stack.
+__global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, int ctas) {
+  extern __shared__ int sm[];
+  int *first = sm;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rank = blockIdx.x, tid = threadIdx.x;
+  const int free_now = a.free_count[0], avail = min(max(free_now, 0), a.capacity);
+  bool odd = free_now != avail;
+  long long carry = 0;
+  // a request's length and mark are read and written by the same threads: position b % threads of every CTA reads, one of them writes after the barrier
+  for (int base = 0; base < a.B; base += blockDim.x) {
+    const int b = base + tid;
+    long long held = 0;
+    if (b < a.B && a.done[b]) {
+      const int n = a.lens[b], q = a.page.div(max(n, 0));
+      odd |= n < 0;
+      held = min(q + (q * a.page.d < n), a.W);
+    }
+    Two total, at = block_scan({held, 0}, total);
+    if (b < a.B) first[b] = saturated(carry + at.a);
+    carry += total.a;
+  }
+  if (tid == 0) first[a.B] = saturated(carry);
+  const int total = (int)min(carry, (long long)(a.capacity - avail));
+  odd |= total < carry;
+  constexpr int OWN = (PG_MAX_B + PG_THREADS - 1) / PG_THREADS;
+  int keep[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; i++) {
+    const int b = (i * ctas + rank) * (int)blockDim.x + tid;
+    keep[i] = b < a.B ? (a.done[b] ? 0 : a.lens[b]) : 0;
+  }
+  if (ctas > 1) umma::cluster_sync();
+  else __syncthreads();
+  if (odd && rank == 0) atomicOr(&g_step_status, (unsigned)PAGED_REFUSED);
+  const int gid = rank * blockDim.x + tid, threads = ctas * blockDim.x;
+#pragma unroll
+  for (int i = 0; i < OWN; i++) {
+    const int b = (i * ctas + rank) * (int)blockDim.x + tid;
+    if (b < a.B) a.lens_out[b] = keep[i];
+  }
+  if (gid == 0) a.count_out[0] = avail + total;
+  for (int p = gid; p < total; p += threads) {
+    const int b = owner_of(first, a.B, p);
+    a.free_pages[avail + p] = a.table[(long long)b * a.table_stride + (p - first[b])];
+  }
+}
+
+int launch_pages(void (*kern)(PagesArgs, int), const PagesArgs &a, size_t smem, bool many, cudaStream_t st, DeviceOnce &once, const char *what) {
+  cudaError_t e = once.ensure([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (PG_MAX_B * 3 + 2) * 4); });
+  if (e != cudaSuccess) return fail((int)e, "light_b200: %s: %s", what, cudaGetErrorString(e));
+  const int ctas = many ? 8 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3(PG_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)ctas, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = many ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, a, ctas);
+  if (e != cudaSuccess) return fail((int)e, "light_b200: %s: %s", what, cudaGetErrorString(e));
+  return launched(what);
+}
+
+// ------------------------------------------------------------------------------------ norm, rotation, cache rows
+// y = x rsqrt(mean x^2 + eps) w over the D elements of a head (no weight: y = x), then the first R of them in pairs (a, b):
+//   (a cos t - b sin t, a sin t + b cos t) factor,   t = position * inv_freq[i],   pair i = (i, i + R / 2) or (2 i, 2 i + 1).
+// f32 from the operand to the one rounding at the end; t in f64 (200000 positions far, an f32 angle is off by 0.01), reduced there to
+// [-pi, pi] for the f32 functions.  The angles are the same for every head of a token, so a CTA takes a token and computes each once.
+struct RotateArgs {
+  const void *q, *k, *v, *qw, *kw;
+  void *q_out, *k_out, *v_out;            // k_out: dense, or the cache's keys with slots
+  long long q_s[2], k_s[2], v_s[2];       // token and head strides, elements
+  long long ks[3], vs[3];                 // cache strides: page, head, row, elements
+  const long long *positions, *slots;
+  const double *inv_freq;
+  long long T, rows;                      // rows of the cache
+  int NH, KH, D, R, interleaved;
+  float eps, factor;
+  FastDiv page;
+};
+
+__device__ __forceinline__ float2 cos_sin(long long pos, double freq) {
+  const double t = (double)pos * freq;
+  const double r = fma(-6.283185307179586476925, rint(t * 0.15915494309189533577), t);
+  float s, c;
+  sincosf((float)r, &s, &c);
+  return make_float2(c, s);
+}
+
+constexpr int RT_THREADS = 256, RT_MAX_D = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) {
+  __shared__ float trig[RT_MAX_D];  // cos, sin of R / 2 angles
+  __shared__ float rowbuf[RT_THREADS / 32][RT_MAX_D];
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.R >> 1;
+  const long long pos = a.positions[t];
+  for (int i = threadIdx.x; i < half; i += RT_THREADS) {
+    const float2 cs = cos_sin(pos, a.inv_freq[i]);
+    trig[i] = cs.x * a.factor, trig[half + i] = cs.y * a.factor;
+  }
+  __syncthreads();
+  long long slot = -1;
+  int page = 0, row = 0;
+  if (a.slots) {
+    slot = a.slots[t];
+    if (slot >= a.rows) {
+      if (threadIdx.x == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
+      slot = -1;
+    }
+    if (slot >= 0) page = (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
+  }
+  const int heads = a.NH + a.KH + (a.slots ? a.KH : 0);
+  float *buf = rowbuf[warp];
+  for (int h = warp; h < heads; h += RT_THREADS / 32) {
+    if (h >= a.NH && a.slots && slot < 0) break;  // a row without a place: its query alone
+    if (h >= a.NH + a.KH) {
+      const int kh = h - a.NH - a.KH;
+      const T *x = static_cast<const T *>(a.v) + t * a.v_s[0] + kh * a.v_s[1];
+      T *y = static_cast<T *>(a.v_out) + page * a.vs[0] + kh * a.vs[1] + row * a.vs[2];
+      for (int d = lane; d < a.D; d += 32) y[d] = x[d];
+      continue;
+    }
+    const bool is_q = h < a.NH;
+    const int kh = h - a.NH;
+    const T *x = is_q ? static_cast<const T *>(a.q) + t * a.q_s[0] + h * a.q_s[1] : static_cast<const T *>(a.k) + t * a.k_s[0] + kh * a.k_s[1];
+    const T *w = static_cast<const T *>(is_q ? a.qw : a.kw);
+    T *y = is_q ? static_cast<T *>(a.q_out) + (t * a.NH + h) * a.D
+                : static_cast<T *>(a.k_out) + (a.slots ? page * a.ks[0] + kh * a.ks[1] + row * a.ks[2] : (t * a.KH + kh) * a.D);
+    float ss = 0.f;
+    for (int d = lane; d < a.D; d += 32) {
+      const float v = to_f32(x[d]);
+      buf[d] = v, ss = fmaf(v, v, ss);
+    }
+    const float inv = w ? rsqrtf(warp_sum(ss) / (float)a.D + a.eps) : 1.f;
+    if (w)
+      for (int d = lane; d < a.D; d += 32) buf[d] = buf[d] * inv * to_f32(w[d]);
+    __syncwarp();  // a lane's pair is another lane's element
+    for (int d = lane; d < a.D; d += 32) {
+      float r = buf[d];
+      if (d < a.R) {
+        const int i = a.interleaved ? d >> 1 : (d < half ? d : d - half);
+        const bool second = a.interleaved ? d & 1 : d >= half;
+        const float o = buf[a.interleaved ? d ^ 1 : (second ? d - half : d + half)];
+        r = second ? o * trig[half + i] + r * trig[i] : r * trig[i] - o * trig[half + i];
+      }
+      y[d] = from_f32<T>(r);
+    }
+    __syncwarp();
+  }
+}
+
+}  // namespace
+
+int paged_pages_check(const lb200_paged_pages *p, const char *what, bool release) {
+  if (!p) return fail(LB200_E_NULL, "light_b200: %s: null argument block", what);
+  if (!p->block_table || !p->lens || !p->free_pages || !p->free_count || !p->lens_out || !p->free_count_out)
+    return fail(LB200_E_NULL, "light_b200: %s: null pointer", what);
+  if (release ? !p->done : !p->new_lens || !p->granted || !p->starts || (p->tokens > 0 && (!p->positions || !p->slots)))
+    return fail(LB200_E_NULL, "light_b200: %s: null pointer", what);
+  if (p->B <= 0 || p->W <= 0 || p->page_size <= 0 || p->capacity <= 0 || p->tokens < 0 || p->table_stride < p->W)
+    return fail(LB200_E_SHAPE, "light_b200: %s: %d requests, table of %d pages (stride %lld), page size %d, %d free entries, %lld tokens", what, p->B, p->W,
+                (long long)p->table_stride, p->page_size, p->capacity, (long long)p->tokens);
+  if (p->B > LB200_PAGED_MAX_REQUESTS) return fail(LB200_E_TOO_LARGE, "light_b200: %s: %d requests, at most %d", what, p->B, LB200_PAGED_MAX_REQUESTS);
+  if ((long long)p->W * p->page_size > 0x7fffffffll || p->tokens > 0x7fffffffll)
+    return fail(LB200_E_TOO_LARGE, "light_b200: %s: %d pages of %d rows, %lld tokens: want fewer than 2^31", what, p->W, p->page_size, (long long)p->tokens);
+  return 0;
+}
+
+static PagesArgs pages_args(const lb200_paged_pages *p) {
+  PagesArgs a{};
+  a.table = p->block_table, a.table_stride = p->table_stride, a.lens = p->lens, a.new_lens = p->new_lens, a.done = p->done;
+  a.free_pages = p->free_pages, a.free_count = p->free_count, a.lens_out = p->lens_out, a.granted = p->granted, a.starts = p->starts;
+  a.count_out = p->free_count_out, a.positions = (long long *)p->positions, a.slots = (long long *)p->slots;
+  a.B = p->B, a.W = p->W, a.capacity = p->capacity, a.page = FastDiv(p->page_size), a.tokens = p->tokens;
+  return a;
+}
+
+int paged_advance(const lb200_paged_pages *p, cudaStream_t st) {
+  static DeviceOnce once;
+  return launch_pages(paged_advance_kernel, pages_args(p), (size_t)(3 * p->B + 2) * 4, p->tokens > 4096, st, once, "paged_advance");
+}
+
+int paged_release(const lb200_paged_pages *p, cudaStream_t st) {
+  static DeviceOnce once;
+  return launch_pages(paged_release_kernel, pages_args(p), (size_t)(p->B + 1) * 4, true, st, once, "paged_release");
+}
+
+int qk_norm_rope_check(const lb200_qk_norm_rope_args *p) {
+  if (!p) return fail(LB200_E_NULL, "light_b200: qk_norm_rope: null argument block");
+  if (p->T < 0 || p->NH <= 0 || p->KH <= 0 || p->D <= 0 || p->D > RT_MAX_D || p->rotary < 0 || p->rotary % 2 || p->rotary > p->D)
+    return fail(LB200_E_SHAPE, "light_b200: qk_norm_rope: T %lld NH %d KH %d D %d (at most %d) rotary %d (even, at most D)", (long long)p->T, p->NH, p->KH, p->D, RT_MAX_D,
+                p->rotary);
+  if (p->dtype != LB200_F32 && p->dtype != LB200_BF16 && p->dtype != LB200_F16) return fail(LB200_E_DTYPE, "light_b200: qk_norm_rope: element type %d", p->dtype);
+  if (p->T > 0x7fffffffll) return fail(LB200_E_TOO_LARGE, "light_b200: qk_norm_rope: %lld tokens", (long long)p->T);
+  if (!(p->eps >= 0.f)) return fail(LB200_E_SHAPE, "light_b200: qk_norm_rope: eps %g", (double)p->eps);
+  if (p->slots && (p->pages <= 0 || p->page_size <= 0))
+    return fail(LB200_E_SHAPE, "light_b200: qk_norm_rope: cache of %lld pages of %d rows", (long long)p->pages, p->page_size);
+  if (p->slots && p->pages > 0x7fffffffll) return fail(LB200_E_TOO_LARGE, "light_b200: qk_norm_rope: %lld pages", (long long)p->pages);
+  if (p->T > 0 && (!p->q || !p->k || !p->q_out || !p->k_out || !p->positions || (p->rotary && !p->inv_freq) || (p->slots && (!p->v || !p->v_out))))
+    return fail(LB200_E_NULL, "light_b200: qk_norm_rope: null pointer (slots come with v and the cache)");
+  return 0;
+}
+
+int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
+  if (p->T == 0) return 0;
+  RotateArgs a{};
+  a.q = p->q, a.k = p->k, a.v = p->v, a.qw = p->q_weight, a.kw = p->k_weight, a.q_out = p->q_out, a.k_out = p->k_out, a.v_out = p->v_out;
+  for (int i = 0; i < 2; i++) a.q_s[i] = p->q_stride[i], a.k_s[i] = p->k_stride[i], a.v_s[i] = p->v_stride[i];
+  for (int i = 0; i < 3; i++) a.ks[i] = p->k_cache_stride[i], a.vs[i] = p->v_cache_stride[i];
+  a.positions = (const long long *)p->positions, a.slots = (const long long *)p->slots, a.inv_freq = p->inv_freq;
+  a.T = p->T, a.rows = p->slots ? p->pages * p->page_size : 0, a.NH = p->NH, a.KH = p->KH, a.D = p->D, a.R = p->rotary, a.interleaved = p->interleaved;
+  a.eps = p->eps, a.factor = p->factor, a.page = FastDiv(p->slots ? p->page_size : 1);
+  cudaError_t e;
+  if (p->dtype == LB200_F32) e = launch_early(qk_norm_rope_kernel<float>, dim3((unsigned)p->T), dim3(RT_THREADS), st, a);
+  else if (p->dtype == LB200_BF16) e = launch_early(qk_norm_rope_kernel<__nv_bfloat16>, dim3((unsigned)p->T), dim3(RT_THREADS), st, a);
+  else e = launch_early(qk_norm_rope_kernel<__half>, dim3((unsigned)p->T), dim3(RT_THREADS), st, a);
+  if (e != cudaSuccess) return fail((int)e, "light_b200: qk_norm_rope: %s", cudaGetErrorString(e));
+  return launched("qk_norm_rope");
+}
+
+int paged_step_status(unsigned int *bits) {
+  return (int)cudaMemcpyFromSymbol(bits, g_step_status, sizeof(*bits));
+}
+
+}  // namespace lb

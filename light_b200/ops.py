@@ -11,6 +11,7 @@ error, and so is a missing shared library.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -906,3 +907,222 @@ def Argmax(x: torch.Tensor) -> torch.Tensor:
 def decode_attn_status(device_index: int = 0) -> int:
     """1 if a decode-attention or append launch ever saw a position outside the cache (synchronises)."""
     return _lib.lib().light_b200_decode_attn_status(device_index)
+
+
+# --------------------------------------------------------------------------- many sequences over one paged key-value cache
+
+@dataclass
+class PagedStep:
+    """What ops.PagedAdvance gives for the tokens of one step."""
+    positions: torch.Tensor   # (tokens,) I64: place in its sequence; 0 behind the last token
+    slots: torch.Tensor       # (tokens,) I64: row of the pool; -1 for a token without one and behind the last
+    starts: torch.Tensor      # (B + 1,) I32: token rows of request b: [starts[b], starts[b + 1])
+    lens: torch.Tensor        # (B,) I32: lengths afterwards
+    granted: torch.Tensor     # (B,) I32: new_lens, or 0 for a request that got nothing
+    free_count: torch.Tensor  # (1,) I32: free pages afterwards
+
+
+def _i32(op: str, dev: torch.device, **ts: torch.Tensor) -> None:
+    for name, t in ts.items():
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"ops.{op}: {name} must be a contiguous I32 tensor on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _pages_args(op: str, block_table: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int):
+    """What both page operators check; (device index, B, a partly filled argument block)."""
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.numel() == 0 or block_table.stride(1) != 1 or \
+            (block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
+        raise ValueError(f"ops.{op}: block_table must be (B, W) I32 with whole rows, got {block_table.dtype} {tuple(block_table.shape)} strides {block_table.stride()}")
+    dev = _dev(block_table, op)
+    B, W = block_table.shape
+    _i32(op, block_table.device, lens=lens, free_pages=free_pages, free_count=free_count)
+    if lens.numel() != B or free_pages.dim() != 1 or free_pages.numel() == 0 or free_count.numel() != 1:
+        raise ValueError(f"ops.{op}: lens {tuple(lens.shape)}, free_pages {tuple(free_pages.shape)}, free_count {tuple(free_count.shape)} for {B} requests")
+    if page_size < 1:
+        raise ValueError(f"ops.{op}: page size {page_size}")
+    return dev, B, _lib.PagedPages(block_table=block_table.data_ptr(), lens=lens.data_ptr(), free_pages=free_pages.data_ptr(), free_count=free_count.data_ptr(),
+                                   table_stride=block_table.stride(0) if B > 1 else W, B=B, W=W, page_size=page_size, capacity=free_pages.numel())
+
+
+def PagedAdvance(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+                 tokens: int, inplace: bool = False) -> PagedStep:
+    """Pages, cache rows and positions for the step's new tokens, on the device in one launch (light_b200_paged_advance): request b's
+    new_lens[b] tokens follow its lens[b] cached ones; the pages that those do not reach come off the stack of free ones (free_pages I32,
+    its first free_count entries) and are written into block_table (B, W) I32.  A request gets all of its pages or none (PagedStep.granted;
+    ops.paged_status reports it).  `tokens`: rows of the batch, those behind the last token are padding (slot -1).  With `inplace` lens
+    and free_count hold the new values, else PagedStep does and they stay.  No gradients."""
+    dev, B, a = _pages_args("PagedAdvance", block_table, lens, free_pages, free_count, page_size)
+    _i32("PagedAdvance", block_table.device, new_lens=new_lens)
+    if new_lens.numel() != B or tokens < 0:
+        raise ValueError(f"ops.PagedAdvance: new_lens {tuple(new_lens.shape)} for {B} requests, {tokens} tokens")
+    rows = torch.empty((2, tokens), dtype=torch.int64, device=lens.device)
+    ints = torch.empty(3 * B + 2, dtype=torch.int32, device=lens.device)
+    starts, granted = ints[:B + 1], ints[B + 1:2 * B + 1]
+    lens_out, count_out = (lens, free_count) if inplace else (ints[2 * B + 1:3 * B + 1], ints[3 * B + 1:])
+    a.new_lens, a.lens_out, a.granted, a.starts, a.free_count_out = new_lens.data_ptr(), lens_out.data_ptr(), granted.data_ptr(), starts.data_ptr(), count_out.data_ptr()
+    a.positions, a.slots, a.tokens = rows.data_ptr(), rows.data_ptr() + 8 * tokens, tokens
+    _lib.check(_lib.lib().light_b200_paged_advance(C.byref(a), dev, _stream(dev)))
+    return PagedStep(rows[0], rows[1], starts, lens_out, granted, count_out)
+
+
+def PagedRelease(block_table: torch.Tensor, lens: torch.Tensor, done: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+                 inplace: bool = False):
+    """The pages of the requests marked in `done` (B,) bool back on the stack of free ones, in one launch (light_b200_paged_release); free_pages
+    gets the entries, the answer is (lens, free_count), the tensors themselves with `inplace`."""
+    dev, B, a = _pages_args("PagedRelease", block_table, lens, free_pages, free_count, page_size)
+    if done.dtype != torch.bool or done.numel() != B or not done.is_contiguous() or done.device != lens.device:
+        raise ValueError(f"ops.PagedRelease: done must be a contiguous bool tensor of {B} on {lens.device}, got {done.dtype} {tuple(done.shape)} on {done.device}")
+    lens_out, count_out = (lens, free_count) if inplace else (torch.empty_like(lens), torch.empty_like(free_count))
+    a.done, a.lens_out, a.free_count_out = done.data_ptr(), lens_out.data_ptr(), count_out.data_ptr()
+    _lib.check(_lib.lib().light_b200_paged_release(C.byref(a), dev, _stream(dev)))
+    return lens_out, count_out
+
+
+def RoPEFrequencies(rotary: int, base: float, scaling: Optional[str] = None, factor: float = 1.0, original: int = 0, low: float = 1.0, high: float = 4.0,
+                    beta_fast: float = 32.0, beta_slow: float = 1.0, device=None):
+    """Angles per position of the rotary / 2 pairs, base^(-2 i / rotary) as F64, and the factor on cos and sin: what ops.QKNormRoPE takes.
+    `scaling` stretches them for contexts `factor` times as long as the `original` ones:
+      "linear"  every frequency over factor
+      "ntk"     base * factor^(rotary / (rotary - 2)): the slowest pair over factor, the fastest as it was
+      "llama3"  pairs that turn fewer than `low` times in `original` positions over factor, more than `high` times as they were, a blend between
+      "yarn"    the same blend between beta_slow and beta_fast turns, linear in the pair's index; cos and sin times 0.1 ln(factor) + 1"""
+    if rotary < 2 or rotary % 2 or not base > 0 or not factor > 0:
+        raise ValueError(f"ops.RoPEFrequencies: rotary {rotary} (even), base {base}, factor {factor}")
+    if scaling in ("llama3", "yarn") and original <= 0:
+        raise ValueError(f"ops.RoPEFrequencies: {scaling} scaling needs the original context, got {original}")
+    i = torch.arange(0, rotary, 2, dtype=torch.float64)
+    if scaling == "ntk":
+        if rotary < 4:
+            raise ValueError("ops.RoPEFrequencies: ntk scaling needs two pairs or more")
+        base = base * factor ** (rotary / (rotary - 2))
+    freq, mult = base ** (-i / rotary), 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "llama3":
+        if not high > low:
+            raise ValueError(f"ops.RoPEFrequencies: low {low}, high {high}")
+        turns = original * freq / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        freq = freq * keep + freq / factor * (1 - keep)
+    elif scaling == "yarn":
+        if not base > 1:
+            raise ValueError(f"ops.RoPEFrequencies: yarn scaling needs a base above 1, got {base}")
+        at = [rotary * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (beta_fast, beta_slow)]  # the pair that turns so often
+        first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary - 1)
+        keep = 1 - ((i / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)
+        freq = freq * keep + freq / factor * (1 - keep)
+        mult = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"ops.RoPEFrequencies: scaling {scaling!r}: want linear, ntk, llama3 or yarn")
+    return freq.to(device if device is not None else "cuda"), mult
+
+
+def _head_rows(t: torch.Tensor) -> torch.Tensor:
+    """(T, heads, D) with the D elements of a head side by side: itself, or a copy."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _check_paged_cache(op: str, k_cache: torch.Tensor, v_cache: torch.Tensor, KH: int, D: int, dtype: torch.dtype, device: torch.device) -> None:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != KH or k_cache.shape[3] != D or k_cache.numel() == 0:
+        raise ValueError(f"ops.{op}: want caches (pages, {KH}, page size, {D}), got {tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.device != device or v_cache.device != device:
+        raise ValueError(f"ops.{op}: caches {k_cache.dtype} on {k_cache.device} / {v_cache.dtype} on {v_cache.device}, want {dtype} on {device}")
+    for c in (k_cache, v_cache):
+        if D > 1 and c.stride(3) != 1:
+            raise ValueError(f"ops.{op}: the {D} elements of a cache row must lie side by side, strides are {c.stride()}")
+
+
+def QKNormRoPE(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+               k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False, factor: float = 1.0, v: Optional[torch.Tensor] = None,
+               k_cache: Optional[torch.Tensor] = None, v_cache: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None):
+    """RMSNorm of every query and key head (where a weight is given), rotation at each token's position and, with a cache, the write of keys
+    and values to their rows, in one launch (light_b200_qk_norm_rope): q (T, NH, D), k, v (T, KH, D) F32 / BF16 / F16, any token and head
+    strides (views of one projection); positions (T,) I64; inv_freq F64 (rotary / 2) and factor from ops.RoPEFrequencies: the first
+    rotary elements of a head turn, in pairs (i, i + rotary / 2), or (2 i, 2 i + 1) with `interleaved`.  Caches (pages, KH, page size, D)
+    of any order, slots (T,) I64 (ops.PagedAdvance): key and value of a token with a negative slot go nowhere; of two tokens with one slot
+    either may stay.  Returns (q, k), k None where it went to the cache.  No gradients."""
+    for name, x in (("q", q), ("k", k)):
+        if x.dim() != 3 or x.shape[0] != q.shape[0] or x.shape[2] != q.shape[2] or x.dtype != q.dtype or x.device != q.device or x.shape[1] == 0 or x.shape[2] == 0:
+            raise ValueError(f"ops.QKNormRoPE: want q (T, NH, D) and k (T, KH, D) of one type, got {name} {tuple(x.shape)} {x.dtype} on {x.device} beside q {tuple(q.shape)} {q.dtype}")
+    if q.dtype not in _ACT:
+        raise ValueError(f"ops.QKNormRoPE: dtype {q.dtype} unsupported (F32 / BF16 / F16)")
+    (T, NH, D), KH = q.shape, k.shape[1]
+    dev = _dev(q, "QKNormRoPE")
+    if positions.dtype != torch.int64 or tuple(positions.shape) != (T,) or positions.device != q.device:
+        raise ValueError(f"ops.QKNormRoPE: positions must be I64 ({T},) on {q.device}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > D or inv_freq.device != q.device:
+        raise ValueError(f"ops.QKNormRoPE: inv_freq must be F64, at most {D // 2} of them, on {q.device}, got {inv_freq.dtype} {tuple(inv_freq.shape)} on {inv_freq.device}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype or w.device != q.device):
+            raise ValueError(f"ops.QKNormRoPE: {name} must be ({D},) {q.dtype} on {q.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")
+    given = [x is not None for x in (v, k_cache, v_cache, slots)]
+    if any(given) and not all(given):
+        raise ValueError("ops.QKNormRoPE: v, k_cache, v_cache and slots come together")
+    qh, kh, vh = _head_rows(q), _head_rows(k), None
+    pc, fc, qw, kw, sc = _whole(positions, inv_freq, q_weight, k_weight, slots)
+    q_out = torch.empty((T, NH, D), dtype=q.dtype, device=q.device)
+    k_out = None
+    a = _lib.QKNormRopeArgs(q=qh.data_ptr(), k=kh.data_ptr(), q_weight=0 if qw is None else qw.data_ptr(), k_weight=0 if kw is None else kw.data_ptr(), positions=pc.data_ptr(),
+                            inv_freq=fc.data_ptr(), q_out=q_out.data_ptr(), q_stride=qh.stride()[:2], k_stride=kh.stride()[:2], T=T, dtype=_ACT[q.dtype], NH=NH, KH=KH, D=D,
+                            rotary=2 * fc.numel(), interleaved=int(interleaved), page_size=1, eps=float(eps), factor=float(factor))
+    if slots is not None:
+        if v.shape != k.shape or v.dtype != q.dtype or v.device != q.device:
+            raise ValueError(f"ops.QKNormRoPE: v must be {tuple(k.shape)} {q.dtype} on {q.device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
+        if slots.dtype != torch.int64 or tuple(slots.shape) != (T,) or slots.device != q.device:
+            raise ValueError(f"ops.QKNormRoPE: slots must be I64 ({T},) on {q.device}, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+        _check_paged_cache("QKNormRoPE", k_cache, v_cache, KH, D, q.dtype, q.device)
+        for c in (k_cache, v_cache):
+            if any(n > 1 and s == 0 for n, s in zip(c.shape, c.stride())):
+                raise ValueError(f"ops.QKNormRoPE: cache rows must not share memory, strides are {c.stride()}")
+        vh = _head_rows(v)
+        a.v, a.v_stride, a.slots, a.k_out, a.v_out = vh.data_ptr(), vh.stride()[:2], sc.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        a.k_cache_stride, a.v_cache_stride, a.pages, a.page_size = k_cache.stride()[:3], v_cache.stride()[:3], k_cache.shape[0], k_cache.shape[2]
+    else:
+        k_out = torch.empty((T, KH, D), dtype=q.dtype, device=q.device)
+        a.k_out = k_out.data_ptr()
+    _lib.check(_lib.lib().light_b200_qk_norm_rope(C.byref(a), dev, _stream(dev)))
+    return q_out, k_out
+
+
+def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, scale: float, window: int = 0,
+                         softcap: float = 0.0) -> torch.Tensor:
+    """Attention of one new token of each sequence over a paged cache (light_b200_paged_decode_attn; ops.DecodeAttention is its counterpart over
+    contiguous caches of one position): q (B, NH, D) F32 / BF16 / F16, caches (pages, KH, page size, D) of q's type and any order of page,
+    head and row, block_table (B, W) I32, lens (B,) I32 valid keys of each sequence, the new token's among them -> (B, NH, D).  window: the
+    last `window` keys only; softcap: scores softcap * tanh(scale q.k / softcap).  A sequence without keys (or whose scores are all -inf)
+    gives zeros; lengths beyond the table and pages outside the cache are reported by ops.paged_status.  No gradients."""
+    if q.dim() != 3 or q.shape[1] == 0 or q.shape[2] == 0:
+        raise ValueError(f"ops.PagedDecodeAttention: want q (B, NH, HD), got {tuple(q.shape)}")
+    if q.dtype not in _ACT:
+        raise ValueError(f"ops.PagedDecodeAttention: dtype {q.dtype} unsupported (F32 / BF16 / F16)")
+    B, NH, D = q.shape
+    KH = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    dev = _dev(q, "PagedDecodeAttention")
+    _check_paged_cache("PagedDecodeAttention", k_cache, v_cache, KH, D, q.dtype, q.device)
+    if NH % KH:
+        raise ValueError(f"ops.PagedDecodeAttention: {NH} query heads over {KH} KV heads")
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] == 0 or block_table.dtype != torch.int32 or block_table.device != q.device:
+        raise ValueError(f"ops.PagedDecodeAttention: block_table must be I32 ({B}, W) on {q.device}, got {block_table.dtype} {tuple(block_table.shape)} on {block_table.device}")
+    if lens.dtype != torch.int32 or tuple(lens.shape) != (B,) or lens.device != q.device:
+        raise ValueError(f"ops.PagedDecodeAttention: lens must be I32 ({B},) on {q.device}, got {lens.dtype} {tuple(lens.shape)} on {lens.device}")
+    if window < 0 or not softcap >= 0:
+        raise ValueError(f"ops.PagedDecodeAttention: window {window}, softcap {softcap}")
+    W = block_table.shape[1]
+    qh, lc = _head_rows(q), lens.contiguous()
+    table = block_table if block_table.stride(1) == 1 and (B == 1 or block_table.stride(0) >= W) else block_table.contiguous()
+    out = torch.empty((B, NH, D), dtype=q.dtype, device=q.device)
+    a = _lib.PagedAttnArgs(q=qh.data_ptr(), k=k_cache.data_ptr(), v=v_cache.data_ptr(), block_table=table.data_ptr(), lens=lc.data_ptr(), out=out.data_ptr(),
+                           q_stride=qh.stride()[:2], k_stride=k_cache.stride()[:3], v_stride=v_cache.stride()[:3], table_stride=table.stride(0) if B > 1 else W,
+                           pages=k_cache.shape[0], dtype=_ACT[q.dtype], B=B, NH=NH, KH=KH, D=D, page_size=k_cache.shape[2], W=W, window=min(int(window), 0x7fffffff),
+                           scale=float(scale), softcap=float(softcap))
+    n = int(_lib.lib().light_b200_paged_attn_scratch_bytes(C.byref(a), dev))
+    own = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None  # of this call alone, on this stream's part of the caching allocator
+    a.scratch, a.scratch_bytes = 0 if own is None else own.data_ptr(), n
+    _lib.check(_lib.lib().light_b200_paged_decode_attn(C.byref(a), dev, _stream(dev)))
+    return out
+
+
+def paged_status(device_index: int = 0) -> int:
+    """What the paged operators met on this device so far (light_b200_paged_status; synchronises): 1 a length outside the table, 2 a page outside
+    the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of free pages."""
+    return _lib.lib().light_b200_paged_status(device_index)
