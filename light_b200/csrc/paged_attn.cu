@@ -98,11 +98,661 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
   }
 }
 
+// ------------------------------------------------------------------------------------ rows on 16 bytes, head sizes of whole 16s
+// The caches are read once (2 n KH D elements) and everything else is small, so the kernel is a stream: what it does is keep loads in
+// flight on every SM whatever the lengths are.
+//   * Work is cut evenly.  A unit is a sequence's KV head (with up to 16 of its query heads); its keys come in tiles of one block per warp.
+//     All tiles of all units in order are dealt to the CTAs in equal runs, a long sequence over many CTAs, many short ones to one.  Every CTA
+//     scans the lengths for itself.  A unit that one CTA holds whole is written out by it; pieces of one that is cut go to scratch
+//     as (max, sum, sum p v), at most two a CTA, and a second launch joins each unit's pieces in their order: no atomics, the same bits
+//     every time.
+//   * A warp is on its own: it copies its block of keys and values (16 rows of each, 8 of f32) into a ring of its own by 16-byte
+//     asynchronous copies, the next blocks' page numbers being read meanwhile, and folds blocks into its own running (max, sum, sum
+//     p v).  No barrier between warps but at the end of a unit.  Rows without a key are filled with zeros: a weight of 0 times what lies there
+//     must not be NaN.
+constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
+
+struct SplitArgs {
+  PagedArgs p;
+  int hpg, groups;    // query heads per unit, units per KV head
+  int4 *heads;        // per CTA: sequence, unit of it, pieces of the unit that begins there and goes on (0: none)
+  float *ml, *acc;    // [2 CTAs][HEADS][2], [2 CTAs][HEADS][D]
+};
+
+// 16-byte chunk c of row r of a block lies at chunk c ^ spread(r): eight rows of one chunk on all banks (ldmatrix), two rows of four
+// neighbouring chunks as well (the f32 kernel's lanes)
+__device__ __forceinline__ int spread(int r) { return (r & 1) << 2 | (r >> 1 & 3); }
+
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of an 8 x 8 matrix of 16-bit elements held by the warp
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(v));
+  return d;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) { mma16816(d, a[0], a[1], a[2], a[3], b0, b1); }
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two weights as 16-bit elements; a and b become what they were rounded to
+__device__ __forceinline__ uint32_t pack(float &a, float &b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  a = f.x, b = f.y;
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float &a, float &b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const uint32_t v = *reinterpret_cast<const uint32_t *>(&h);
+  a = __uint_as_float(v << 16), b = __uint_as_float(v & 0xFFFF0000u);
+  return v;
+}
+
+// bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
+//   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
+//   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
+//   P is rounded to the cache's type, as the instruction wants it: 2^-8 (bf16) or 2^-11 of each weight, no more than the output's own rounding;
+//   the sum below the fraction adds the rounded weights, so that they sum to one.
+template <typename T_, int DP_, int NT>
+struct MmaBlock {
+  using T = T_;
+  static constexpr int DP = DP_, KB = 16, HEADS = 8 * NT, ROWB = DP * 2, PR = DP + 4, EXTRA = 0;
+  uint32_t q[DP / 16][NT][2];
+  float o[DP / 16][NT][4], m[NT][2], l[NT][2];
+
+  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *, int) {
+    const PagedArgs &a = s.p;
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int h = 8 * nt + r;
+      const T *p = static_cast<const T *>(a.q) + b * a.q_s[0] + (kh * a.G + h0 + h) * a.q_s[1] + 2 * c;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ks++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) q[ks][nt][e] = h < count && ks * 16 < a.D ? *reinterpret_cast<const uint32_t *>(p + 16 * ks + 8 * e) : 0u;
+#pragma unroll
+      for (int e = 0; e < 2; e++) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[t][nt][e] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void block(const PagedArgs &a, const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *, int) {
+    const int lane = threadIdx.x & 31, r = lane >> 2;
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[nt][e] = 0.f;
+    const int turn = spread(lane & 7);
+    const uint32_t krow = kbase + (lane & 15) * ROWB, vrow = kbase + KB * ROWB + ((lane & 7) + (lane >> 4) * 8) * ROWB;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ks++)
+      if (ks * 16 < a.D) {
+        uint32_t f[4];
+        ldm4(f, krow + (((2 * ks + (lane >> 4)) ^ turn) << 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) mma(s[nt], f, q[ks][nt][0], q[ks][nt][1], T());
+      }
+    uint32_t p[NT][2];
+    float corr[NT][2];
+    bool same = true;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[nt][e] = valid >> (r + 8 * (e >> 1)) & 1 ? score(s[nt][e]) : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        mx = fmaxf(mx, m[nt][e]);
+        const float use = mx == -INFINITY ? 0.f : mx;  // no key above -inf so far: all weights 0
+        corr[nt][e] = exp2f(m[nt][e] - use);
+        same = same && mx == m[nt][e];
+        m[nt][e] = mx;
+        s[nt][e] = exp2f(s[nt][e] - use), s[nt][2 + e] = exp2f(s[nt][2 + e] - use);
+      }
+      const uint32_t lo = pack(s[nt][0], s[nt][1], T()), hi = pack(s[nt][2], s[nt][3], T());
+      p[nt][0] = transposed(lo), p[nt][1] = transposed(hi);
+#pragma unroll
+      for (int e = 0; e < 2; e++) l[nt][e] = fmaf(l[nt][e], corr[nt][e], s[nt][e] + s[nt][2 + e]);
+    }
+    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+      for (int t = 0; t < DP / 16; t++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[t][nt][e] *= corr[nt][e & 1];
+    }
+#pragma unroll
+    for (int t = 0; t < DP / 16; t++)
+      if (t * 16 < a.D) {
+        uint32_t f[4];
+        ldm4_trans(f, vrow + (((2 * t + (lane >> 3 & 1)) ^ turn) << 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) mma(o[t][nt], f, p[nt][0], p[nt][1], T());
+      }
+  }
+
+  __device__ __forceinline__ void store(float *part, int D) {  // [HEADS][PR]: max, sum, -, -, D dims
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float sum = l[nt][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        float *row = part + (8 * nt + 2 * c + e) * PR;
+        if (r == 0) row[0] = m[nt][e], row[1] = sum;
+#pragma unroll
+        for (int t = 0; t < DP / 16; t++)
+          if (t * 16 < D) row[4 + 16 * t + r] = o[t][nt][e], row[4 + 16 * t + r + 8] = o[t][nt][2 + e];
+      }
+  }
+};
+
+// f32: a block of 8 keys, f32 products.  For the scores a lane has a key and a quarter of its chunks (the queries are broadcasts from shared
+// memory); the four lanes of a key hand each other halves of their heads until each has its own complete.  The weights go through
+// shared memory, and for the values a lane owns chunks of dims (of 64 dims: and every other key).
+template <int DP_, int GH>
+struct F32Block {
+  using T = float;
+  static constexpr int DP = DP_, KB = 8, HEADS = GH, ROWB = DP * 4, PR = DP + 4;
+  static constexpr int OWN = GH < 4 ? 1 : GH / 4, NC = DP < 128 ? 1 : DP / 128, SPLIT = DP < 128 ? 128 / DP : 1;  // heads of a lane; chunks; keys side by side
+  static constexpr int QS = GH * DP * 4, PS = KB * GH * 4 + GH * 4, EXTRA = QS + PA_WARPS * PS;  // queries | per warp: weights, corrections
+  float acc[GH][NC][4], m[OWN], l[OWN];
+
+  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *extra, int) {
+    const PagedArgs &a = s.p;
+    float *qs = reinterpret_cast<float *>(extra);
+    for (int i = threadIdx.x; i < GH * DP; i += PA_THREADS) {
+      const int h = i / DP, d = i % DP;
+      qs[i] = h < count && d < a.D ? static_cast<const float *>(a.q)[b * a.q_s[0] + (kh * a.G + h0 + h) * a.q_s[1] + d] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < OWN; i++) m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+    for (int h = 0; h < GH; h++)
+#pragma unroll
+      for (int i = 0; i < NC; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[h][i][e] = 0.f;
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ static int first_head(int lane) { return GH >= 4 ? (lane & 2 ? GH / 2 : 0) + (lane & 1 ? GH / 4 : 0) : GH == 2 ? lane >> 1 & 1 : 0; }
+
+  __device__ __forceinline__ void block(const PagedArgs &a, const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *extra, int warp) {
+    const int lane = threadIdx.x & 31, key = lane >> 2, qd = lane & 3;
+    const float *qs = reinterpret_cast<const float *>(extra);
+    float *ps = reinterpret_cast<float *>(extra + QS + warp * PS), *cs = ps + KB * GH;
+    float d[GH];
+#pragma unroll
+    for (int h = 0; h < GH; h++) d[h] = 0.f;
+    const uint32_t krow = kbase + key * ROWB;
+    const int turn = spread(key);
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++)
+      if (i * 16 < a.D) {
+        const int c = qd + 4 * i;
+        const uint4 w = lds128(krow + ((c ^ turn) << 4));
+        const float4 k = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+#pragma unroll
+        for (int h = 0; h < GH; h++) {
+          const float4 q = *reinterpret_cast<const float4 *>(qs + h * DP + 4 * c);
+          d[h] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, d[h]))));
+        }
+      }
+    int cnt = GH;
+#pragma unroll
+    for (int x = 2; x >= 1; x >>= 1) {
+      if (cnt > 1) {
+        const int half = cnt / 2;
+        const bool up = lane & x;
+#pragma unroll
+        for (int i = 0; i < GH / 2; i++)
+          if (i < half) {
+            const float send = up ? d[i] : d[i + half], keep = up ? d[i + half] : d[i];
+            d[i] = keep + __shfl_xor_sync(0xffffffffu, send, x);
+          }
+        cnt = half;
+      } else {
+        d[0] += __shfl_xor_sync(0xffffffffu, d[0], x);
+      }
+    }
+    const int h0 = first_head(lane);
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < OWN; i++) {
+      const float s = valid >> key & 1 ? score(d[i]) : -INFINITY;
+      float mx = s;
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      mx = fmaxf(mx, m[i]);
+      const float use = mx == -INFINITY ? 0.f : mx, corr = exp2f(m[i] - use), p = exp2f(s - use);
+      same = same && mx == m[i];
+      m[i] = mx, l[i] = fmaf(l[i], corr, p);
+      ps[key * GH + h0 + i] = p;
+      if (key == 0) cs[h0 + i] = corr;
+    }
+    __syncwarp();
+    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+      for (int h = 0; h < GH; h++) {
+        const float c = cs[h];
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[h][i][e] *= c;
+      }
+    }
+    constexpr int LANES = 32 / SPLIT;  // of a row
+#pragma unroll
+    for (int k0 = 0; k0 < KB; k0 += SPLIT) {
+      const int k = k0 + lane / LANES;
+      float p[GH];
+      if constexpr (GH >= 4) {
+#pragma unroll
+        for (int h = 0; h < GH; h += 4) {
+          const float4 x = *reinterpret_cast<const float4 *>(ps + k * GH + h);
+          p[h] = x.x, p[h + 1] = x.y, p[h + 2] = x.z, p[h + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < GH; h++) p[h] = ps[k * GH + h];
+      }
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+        const int c = lane % LANES + 32 * i;
+        if (c * 4 < a.D) {
+          const uint4 w = lds128(kbase + (KB + k) * ROWB + ((c ^ spread(k)) << 4));
+          const float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
+#pragma unroll
+          for (int h = 0; h < GH; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[h][i][e] = fmaf(p[h], v[e], acc[h][i][e]);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(float *part, int D) {
+    const int lane = threadIdx.x & 31, h0 = first_head(lane);
+#pragma unroll
+    for (int i = 0; i < OWN; i++) {
+      float sum = l[i];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (lane < 4) part[(h0 + i) * PR] = m[i], part[(h0 + i) * PR + 1] = sum;
+    }
+    constexpr int LANES = 32 / SPLIT;
+#pragma unroll
+    for (int h = 0; h < GH; h++)
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int x = LANES; x < 32; x <<= 1) acc[h][i][e] += __shfl_xor_sync(0xffffffffu, acc[h][i][e], x);
+        const int c = lane % LANES + 32 * i;
+        if (lane < LANES && c * 4 < D) *reinterpret_cast<float4 *>(part + h * PR + 4 + 4 * c) = make_float4(acc[h][i][0], acc[h][i][1], acc[h][i][2], acc[h][i][3]);
+      }
+  }
+};
+
+template <typename P>
+struct SplitCfg {
+  static constexpr int CTAS = P::DP == 64 ? 3 : P::DP == 128 ? 2 : 1;  // per SM
+  static constexpr int TILE = PA_WARPS * P::KB, STAGE = 2 * P::KB * P::ROWB, PART = PA_WARPS * P::HEADS * P::PR * 4;
+  static constexpr int ROOM = (228 * 1024) / CTAS - 1024 - 256;        // shared memory of a CTA beside what is static
+  static constexpr int stages(int s) { return PART + P::EXTRA + PA_WARPS * s * STAGE <= ROOM ? s : stages(s - 1); }
+  static constexpr int S = stages(4);
+  static constexpr int RING = PA_WARPS * S * STAGE, SMEM = RING + PART + P::EXTRA;
+  static_assert(S >= 2, "a ring of two blocks or more");
+};
+
+struct Cursor {
+  int b, u, tile, n, j0, tiles;  // sequence, unit of it, tile of that; its length, first key, tiles per unit
+  template <int TILE>
+  __device__ __forceinline__ void at(const PagedArgs &a, int b_) {
+    b = b_, n = length_of(a, b_), j0 = first_of(a, n), tiles = (n - j0 + TILE - 1) / TILE;
+  }
+  template <int TILE>
+  __device__ __forceinline__ void next(const PagedArgs &a, int units) {  // (there is a next tile)
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++u < units) return;
+    u = 0;
+    do at<TILE>(a, b + 1);
+    while (tiles == 0);
+  }
+};
+
+template <typename P>
+__global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kernel(SplitArgs s) {
+  using C = SplitCfg<P>;
+  using T = typename P::T;
+  constexpr int KB = P::KB, TILE = C::TILE, S = C::S, ROWB = P::ROWB;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long scan[PA_WARPS];
+  __shared__ int from[3];  // where this CTA's tiles begin: sequence, unit, tile
+  __shared__ uint32_t masks[PA_WARPS][S];
+  pdl_launch_dependents();
+  pdl_wait();
+  const PagedArgs &a = s.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x, units = a.KH * s.groups;
+  unsigned odd = 0;
+
+  // ---- this CTA's run of tiles
+  const int per = (a.B + PA_THREADS - 1) / PA_THREADS, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
+  auto tiles_of = [&](int b) {
+    const int n = length_of(a, b);
+    return (n - first_of(a, n) + TILE - 1) / TILE;
+  };
+  long long sum = 0;
+  for (int b = lo; b < hi; b++) {
+    if (cta == 0 && a.lens[b] != length_of(a, b)) odd |= PAGED_LENGTH;
+    sum += tiles_of(b);
+  }
+  long long incl = sum;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, x);
+    if (lane >= x) incl += v;
+  }
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  long long before = incl - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; w++) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  total *= units;
+  const int dealt = (int)min((long long)ctas, total);  // CTAs with tiles: the first ones, one or more each, so that a unit's pieces lie in a row
+  const long long t0 = cta < dealt ? total * cta / dealt : 0;
+  const int steps = cta < dealt ? (int)(total * (cta + 1) / dealt - t0) : 0;
+  if (steps > 0 && before * units <= t0 && t0 < (before + sum) * units) {
+    int b = lo, n = tiles_of(b);
+    while ((before + n) * units <= t0) before += n, n = tiles_of(++b);
+    const int r = (int)(t0 - before * units);
+    from[0] = b, from[1] = r / n, from[2] = r % n;
+  }
+  // sequences without keys
+  for (int b = cta; b < a.B; b += ctas)
+    if (tiles_of(b) == 0)
+      for (int i = tid; i < a.NH * a.D; i += PA_THREADS) static_cast<T *>(a.out)[(long long)b * a.NH * a.D + i] = from_f32<T>(0.f);
+  __syncthreads();
+  int4 head = make_int4(0, 0, 0, 0);
+
+  if (steps > 0) {
+    Cursor now, far;  // what is folded, and what is fetched
+    now.at<TILE>(a, from[0]);
+    now.u = from[1], now.tile = from[2];
+    far = now;
+    const uint32_t ring = umma::smem_u32(smem) + warp * S * C::STAGE;
+    float *part = reinterpret_cast<float *>(smem + C::RING);
+    unsigned char *extra = smem + C::RING + C::PART;
+
+    struct Row {
+      int pg, row, kh;
+      bool valid;
+    };
+    auto peek = [&]() {  // the page of this lane's key of the block at `far` (lanes from KB on repeat)
+      Row r;
+      const int j = far.j0 + far.tile * TILE + warp * KB + (lane & (KB - 1));
+      const int w = a.page.div(j);
+      r.valid = j < far.n, r.row = j - w * a.page.d, r.kh = far.u / s.groups;
+      r.pg = r.valid ? a.table[far.b * a.table_stride + w] : -1;
+      return r;
+    };
+    constexpr int E = 16 / (int)sizeof(T), CHUNKS = P::DP / E, LANES = CHUNKS < 32 ? CHUNKS : 32, RPI = 32 / LANES, CPL = CHUNKS / LANES;
+    auto issue = [&](const Row &r, int slot) {
+      const bool ok = r.valid && r.pg >= 0 && r.pg < a.pages;
+      if (r.valid && !ok) odd |= PAGED_PAGE;
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << KB) - 1);
+      if (lane == 0) masks[warp][slot] = mask;
+      const long long ko = ok ? r.pg * a.ks[0] + r.kh * a.ks[1] + r.row * a.ks[2] : 0, vo = ok ? r.pg * a.vs[0] + r.kh * a.vs[1] + r.row * a.vs[2] : 0;
+      const uint32_t dst = ring + slot * C::STAGE;
+#pragma unroll
+      for (int i = 0; i < KB / RPI; i++) {
+        const int row = i * RPI + lane / LANES;
+        const T *kp = static_cast<const T *>(a.k) + __shfl_sync(0xffffffffu, ko, row), *vp = static_cast<const T *>(a.v) + __shfl_sync(0xffffffffu, vo, row);
+        const uint32_t n = mask >> row & 1 ? 16 : 0;
+#pragma unroll
+        for (int x = 0; x < CPL; x++) {
+          const int c = lane % LANES + 32 * x;
+          if (c * E < a.D) {
+            const uint32_t to = dst + row * ROWB + ((c ^ spread(row)) << 4);
+            cp_async16_part(to, kp + c * E, n);
+            cp_async16_part(to + KB * ROWB, vp + c * E, n);
+          }
+        }
+      }
+    };
+
+    Row next;
+    {
+      Row first[S - 1];
+#pragma unroll
+      for (int i = 0; i < S - 1; i++)
+        if (i < steps) {
+          if (i) far.next<TILE>(a, units);
+          first[i] = peek();
+        }
+#pragma unroll
+      for (int i = 0; i < S - 1; i++) {
+        if (i < steps) issue(first[i], i);
+        cp_async_commit();
+      }
+      if (S - 1 < steps) far.next<TILE>(a, units), next = peek();
+    }
+
+    const Scorer score(a.scale, a.softcap);
+    P state;
+    bool fresh = true, begins = false;
+    long long unit0 = 0;  // the unit's first tile among all
+    int slot = 0, fill = S - 1;
+    for (int step = 0; step < steps; step++) {
+      cp_async_wait<S - 2>();
+      __syncwarp();  // the block is there for all lanes, and all are done with the one before
+      if (step + S - 1 < steps) {
+        issue(next, fill);
+        if (step + S < steps) far.next<TILE>(a, units), next = peek();
+      }
+      cp_async_commit();
+      const int kh = now.u / s.groups, h0 = (now.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
+      if (fresh) {
+        begins = now.tile == 0, unit0 = t0 + step - now.tile, fresh = false;
+        state.begin(s, now.b, kh, h0, count, extra, warp);
+      }
+      state.block(a, score, ring + slot * C::STAGE, masks[warp][slot], extra, warp);
+      slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
+      const bool ends = now.tile + 1 == now.tiles;
+      if (ends || step + 1 == steps) {
+        // ---- the warps' parts of the unit
+        state.store(part + warp * P::HEADS * P::PR, a.D);
+        __syncthreads();
+        const bool whole = begins && ends;
+        const int place = 2 * cta + (begins ? 1 : 0);
+        for (int h = warp; h < count; h += PA_WARPS) {
+          const float *row = part + h * P::PR;
+          float top = -INFINITY, L = 0.f, e[PA_WARPS];
+#pragma unroll
+          for (int w = 0; w < PA_WARPS; w++) top = fmaxf(top, row[w * P::HEADS * P::PR]);
+          const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int w = 0; w < PA_WARPS; w++) e[w] = exp2f(row[w * P::HEADS * P::PR] - use), L = fmaf(e[w], row[w * P::HEADS * P::PR + 1], L);
+          const long long at = (long long)place * P::HEADS + h;
+          if (!whole && lane == 0) s.ml[2 * at] = top, s.ml[2 * at + 1] = L;
+          for (int d = lane; d < a.D; d += 32) {
+            float A = 0.f;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; w++) A = fmaf(e[w], row[w * P::HEADS * P::PR + 4 + d], A);
+            if (whole) static_cast<T *>(a.out)[((long long)now.b * a.NH + kh * a.G + h0 + h) * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
+            else s.acc[at * a.D + d] = A;
+          }
+        }
+        if (begins && !ends) head = make_int4(now.b, now.u, (int)(((unit0 + now.tiles) * dealt - 1) / total) - cta + 1, 0);
+        __syncthreads();  // part is free again
+        fresh = true;
+      }
+      if (step + 1 < steps) now.next<TILE>(a, units);
+    }
+    cp_async_wait<0>();
+  }
+  if (s.heads && tid == 0) s.heads[cta] = head;
+  if (odd) atomicOr(&g_attn_status, odd);
+}
+
+// The pieces of a unit that was cut, in order: piece 0 is the second of the CTA where it begins, piece i the first of the i-th CTA after it.
+// A CTA per head; a warp takes every eighth piece.
+constexpr int PJ_WARPS = 8, PJ_MAX = 1024;  // pieces: no more than CTAs of the first launch
+
+template <typename T>
+__global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(SplitArgs s, int HEADS) {
+  __shared__ float weight[PJ_MAX], tops[PJ_WARPS], sums[PJ_WARPS], part[PJ_WARPS][PL_MAX_D];
+  pdl_launch_dependents();
+  pdl_wait();
+  const PagedArgs &a = s.p;
+  const int4 head = s.heads[blockIdx.x];
+  const int n = head.z, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kh = head.y / s.groups, h0 = (head.y - kh * s.groups) * s.hpg;
+  if (n == 0 || h >= min(s.hpg, a.G - h0)) return;
+  auto place = [&](int i) { return (long long)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * HEADS + h; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += PJ_WARPS * 32) top = fmaxf(top, s.ml[2 * place(i)]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < PJ_WARPS; w++) top = fmaxf(top, tops[w]);
+  if (top == -INFINITY) top = 0.f;
+  float L = 0.f;
+  for (int i = threadIdx.x; i < n; i += PJ_WARPS * 32) {
+    const float e = exp2f(s.ml[2 * place(i)] - top);
+    weight[i] = e, L = fmaf(e, s.ml[2 * place(i) + 1], L);
+  }
+  L = warp_sum(L);
+  if (lane == 0) sums[warp] = L;
+  __syncthreads();
+  L = 0.f;
+#pragma unroll
+  for (int w = 0; w < PJ_WARPS; w++) L += sums[w];
+  float acc[PL_MAX_D / 32];
+#pragma unroll
+  for (int e = 0; e < PL_MAX_D / 32; e++) acc[e] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < n; i += PJ_WARPS) {
+    const float w = weight[i];
+    const float *row = s.acc + place(i) * a.D;
+#pragma unroll
+    for (int x = 0; x < PL_MAX_D / 128; x++)
+      if (4 * lane + 128 * x < a.D) {
+        const float4 v = *reinterpret_cast<const float4 *>(row + 4 * lane + 128 * x);
+        acc[4 * x] = fmaf(w, v.x, acc[4 * x]), acc[4 * x + 1] = fmaf(w, v.y, acc[4 * x + 1]);
+        acc[4 * x + 2] = fmaf(w, v.z, acc[4 * x + 2]), acc[4 * x + 3] = fmaf(w, v.w, acc[4 * x + 3]);
+      }
+  }
+#pragma unroll
+  for (int x = 0; x < PL_MAX_D / 128; x++)
+    if (4 * lane + 128 * x < a.D)
+#pragma unroll
+      for (int e = 0; e < 4; e++) part[warp][4 * lane + 128 * x + e] = acc[4 * x + e];
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.D; d += PJ_WARPS * 32) {
+    float A = 0.f;
+#pragma unroll
+    for (int w = 0; w < PJ_WARPS; w++) A += part[w][d];
+    static_cast<T *>(a.out)[((long long)head.x * a.NH + kh * a.G + h0 + h) * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
+  }
+}
+
+// How a call is cut: heads per unit, CTAs, whether a unit can be cut, and the scratch that takes.
+struct Cut {
+  bool streamed;       // the kernel above, else the one for any stride
+  int hpg, groups, DP, HEADS, ctas;
+  bool joined;
+  size_t ml_at, acc_at, bytes;
+};
+
+Cut cut_of(const lb200_paged_attn_args *p) {
+  Cut c{};
+  const int size = p->dtype == LB200_F32 ? 4 : 2, G = p->NH / p->KH;
+  uint64_t off = (uint64_t)(uintptr_t)p->q | (uint64_t)(uintptr_t)p->k | (uint64_t)(uintptr_t)p->v;
+  for (int i = 0; i < 2; i++) off |= (uint64_t)p->q_stride[i] * size;
+  for (int i = 0; i < 3; i++) off |= (uint64_t)p->k_stride[i] * size | (uint64_t)p->v_stride[i] * size;
+  c.streamed = p->D % 16 == 0 && !(off & 15);
+  if (!c.streamed) return c;
+  c.groups = (G + 15) / 16, c.hpg = (G + c.groups - 1) / c.groups, c.groups = (G + c.hpg - 1) / c.hpg;
+  c.DP = p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256;
+  c.HEADS = p->dtype == LB200_F32 ? (c.hpg <= 1 ? 1 : c.hpg <= 2 ? 2 : c.hpg <= 4 ? 4 : c.hpg <= 8 ? 8 : 16) : (c.hpg <= 8 ? 8 : 16);
+  const int tile = PA_WARPS * (p->dtype == LB200_F32 ? 8 : 16), per_sm = c.DP == 64 ? 3 : c.DP == 128 ? 2 : 1;
+  long long keys = (long long)p->W * p->page_size;
+  if (p->window > 0 && p->window < keys) keys = p->window;
+  const long long tiles = (keys + tile - 1) / tile, all = tiles * p->KH * c.groups, slots = (long long)per_sm * sm_count();
+  c.ctas = (int)(all >= slots || all * p->B >= slots ? (slots < PJ_MAX ? slots : PJ_MAX) : all * p->B);
+  c.joined = tiles > 1;
+  if (c.joined) {
+    c.ml_at = ((size_t)c.ctas * sizeof(int4) + 255) & ~(size_t)255;
+    c.acc_at = (c.ml_at + (size_t)c.ctas * 2 * c.HEADS * 2 * 4 + 255) & ~(size_t)255;
+    c.bytes = c.acc_at + (size_t)c.ctas * 2 * c.HEADS * p->D * 4;
+  }
+  return c;
+}
+
+template <typename P>
+int launch_split(const SplitArgs &s, const Cut &c, cudaStream_t st) {
+  auto kern = paged_attn_kernel<P>;
+  static DeviceOnce once;
+  cudaError_t e = once.ensure([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<P>::SMEM); });
+  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)c.ctas), cfg.blockDim = dim3(PA_THREADS), cfg.dynamicSmemBytes = SplitCfg<P>::SMEM, cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, s);
+  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
+  if (int rc = launched("paged_decode_attn")) return rc;
+  if (!c.joined) return 0;
+  e = launch_early(paged_join_kernel<typename P::T>, dim3((unsigned)c.ctas, (unsigned)c.hpg), dim3(PJ_WARPS * 32), st, s, c.HEADS);
+  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
+  return launched("paged_decode_attn (join)");
+}
+
+template <int DP>
+int launch_dtype(const SplitArgs &s, const Cut &c, int dtype, cudaStream_t st) {
+  if (dtype == LB200_BF16) return c.HEADS == 8 ? launch_split<MmaBlock<__nv_bfloat16, DP, 1>>(s, c, st) : launch_split<MmaBlock<__nv_bfloat16, DP, 2>>(s, c, st);
+  if (dtype == LB200_F16) return c.HEADS == 8 ? launch_split<MmaBlock<__half, DP, 1>>(s, c, st) : launch_split<MmaBlock<__half, DP, 2>>(s, c, st);
+  switch (c.HEADS) {
+    case 1: return launch_split<F32Block<DP, 1>>(s, c, st);
+    case 2: return launch_split<F32Block<DP, 2>>(s, c, st);
+    case 4: return launch_split<F32Block<DP, 4>>(s, c, st);
+    case 8: return launch_split<F32Block<DP, 8>>(s, c, st);
+    default: return launch_split<F32Block<DP, 16>>(s, c, st);
+  }
+}
+
 }  // namespace
 
 unsigned long long paged_attn_scratch_bytes(const lb200_paged_attn_args *p) {
-  (void)p;
-  return 0;
+  return p->B > 0 ? cut_of(p).bytes : 0;
 }
 
 int paged_attn_check(const lb200_paged_attn_args *p) {
@@ -112,7 +762,7 @@ int paged_attn_check(const lb200_paged_attn_args *p) {
       p->table_stride < p->W || !(p->softcap >= 0.f))
     return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: B %d NH %d KH %d D %d (at most %d) page size %d table %d pages %lld window %d softcap %g", p->B, p->NH, p->KH,
                 p->D, PL_MAX_D, p->page_size, p->W, (long long)p->pages, p->window, (double)p->softcap);
-  if ((long long)p->W * p->page_size > 0x7fffffffll || p->pages > 0x7fffffffll || (long long)p->B * p->NH > 0x7fffffffll)
+  if ((long long)p->W * p->page_size > 0x7ffffc00ll || p->pages > 0x7fffffffll || (long long)p->B * p->NH > 0x7fffffffll)
     return fail(LB200_E_TOO_LARGE, "light_b200: paged_decode_attn: %d pages of %d rows per sequence, %lld pages, %d x %d heads: want fewer than 2^31 of each", p->W,
                 p->page_size, (long long)p->pages, p->B, p->NH);
   if (p->B > 0 && (!p->q || !p->k || !p->v || !p->block_table || !p->lens || !p->out)) return fail(LB200_E_NULL, "light_b200: paged_decode_attn: null pointer");
@@ -127,6 +777,19 @@ int paged_decode_attn(const lb200_paged_attn_args *p, cudaStream_t st) {
   for (int i = 0; i < 3; i++) a.ks[i] = p->k_stride[i], a.vs[i] = p->v_stride[i];
   a.table_stride = p->table_stride, a.pages = p->pages, a.B = p->B, a.NH = p->NH, a.KH = p->KH, a.G = p->NH / p->KH, a.D = p->D, a.W = p->W, a.window = p->window;
   a.scale = p->scale, a.softcap = p->softcap, a.page = FastDiv(p->page_size);
+  const Cut c = cut_of(p);
+  if (c.streamed) {
+    if (c.bytes && (!p->scratch || p->scratch_bytes < c.bytes || ((uintptr_t)p->scratch & 255)))
+      return fail(p->scratch ? LB200_E_SHAPE : LB200_E_NULL, "light_b200: paged_decode_attn: %llu bytes of scratch, want %llu, 256-byte aligned", p->scratch_bytes,
+                  (unsigned long long)c.bytes);
+    SplitArgs s{};
+    s.p = a, s.hpg = c.hpg, s.groups = c.groups;
+    if (c.joined) {
+      s.heads = static_cast<int4 *>(p->scratch);
+      s.ml = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + c.ml_at), s.acc = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + c.acc_at);
+    }
+    return c.DP == 64 ? launch_dtype<64>(s, c, p->dtype, st) : c.DP == 128 ? launch_dtype<128>(s, c, p->dtype, st) : launch_dtype<256>(s, c, p->dtype, st);
+  }
   const dim3 grid((unsigned)(p->B * p->NH)), block(PL_WARPS * 32);
   cudaError_t e = p->dtype == LB200_F32    ? launch_early(paged_attn_any_kernel<float>, grid, block, st, a)
                   : p->dtype == LB200_BF16 ? launch_early(paged_attn_any_kernel<__nv_bfloat16>, grid, block, st, a)
