@@ -308,6 +308,154 @@ PyObject *moe_gemm(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   return give(light_b200_moe_gemm_scratch(&m, s.t->const_data_ptr<float>(), (int)bR, (int)bC, own_bytes ? own.data_ptr() : nullptr, own_bytes, dev, st), out);
 }
 
+// ---- many sequences over one paged cache
+bool i32_of(const at::Tensor &t, int dev, int64_t n) {  // a contiguous I32 tensor of n elements
+  return t.is_cuda() && t.scalar_type() == at::kInt && t.is_contiguous() && t.get_device() == dev && t.numel() == n;
+}
+// (B, W) I32 with whole rows -> the row stride, 0 if it is none
+int64_t table_of(const at::Tensor &t) {
+  if (!t.is_cuda() || t.dim() != 2 || t.scalar_type() != at::kInt || t.numel() == 0 || t.stride(1) != 1 || (t.size(0) > 1 && t.stride(0) < t.size(1))) return 0;
+  return t.size(0) > 1 ? t.stride(0) : t.size(1);
+}
+bool heads_of(const at::Tensor &t, int64_t T, int64_t D, at::ScalarType dt, int dev) {  // (T, heads, D), the elements of a head side by side
+  return t.is_cuda() && t.dim() == 3 && t.size(0) == T && t.size(1) > 0 && t.size(2) == D && t.scalar_type() == dt && t.get_device() == dev && (t.stride(2) == 1 || D == 1) &&
+         !t.requires_grad();
+}
+bool cache_of(const at::Tensor &k, const at::Tensor &v, int64_t KH, int64_t D, at::ScalarType dt, int dev, bool written) {
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.size(1) != KH || k.size(3) != D || k.numel() == 0) return false;
+  for (const at::Tensor *c : {&k, &v}) {
+    if (!c->is_cuda() || c->scalar_type() != dt || c->get_device() != dev || c->requires_grad() || (D > 1 && c->stride(3) != 1)) return false;
+    for (int i = 0; written && i < 4; i++)
+      if (c->size(i) > 1 && c->stride(i) == 0) return false;
+  }
+  return true;
+}
+PyObject *tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject *t = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor &x : ts) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(x));
+  return t;
+}
+
+// (block table, lens, new lens, free pages, free count, page size, tokens, inplace) -> (positions, slots, starts, lens, granted, free count)
+PyObject *paged_advance(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  ARGS(8)
+  Arg t, l, n, f, c;
+  long long page, tokens;
+  NEED(t.ok(a[0]) && l.ok(a[1]) && n.ok(a[2]) && f.ok(a[3]) && c.ok(a[4]) && long_of(a[5], page) && long_of(a[6], tokens));
+  const int inplace = PyObject_IsTrue(a[7]);
+  if (inplace < 0) return nullptr;
+  const int64_t stride = table_of(*t.t);
+  NEED(stride > 0);
+  const int dev = t.t->get_device();
+  const int64_t B = t.t->size(0), W = t.t->size(1), cap = f.t->numel();
+  NEED(i32_of(*l.t, dev, B) && i32_of(*n.t, dev, B) && i32_of(*c.t, dev, 1) && f.t->dim() == 1 && cap > 0 && cap < (1ll << 31) && i32_of(*f.t, dev, cap));
+  NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31) && tokens >= 0);
+  const auto i32 = l.t->options(), i64 = i32.dtype(at::kLong);
+  at::Tensor pos = at::empty({tokens}, i64), slots = at::empty({tokens}, i64), starts = at::empty({B + 1}, i32), granted = at::empty({B}, i32);
+  at::Tensor lens = inplace ? *l.t : at::empty({B}, i32), count = inplace ? *c.t : at::empty({1}, i32);
+  lb200_paged_pages p{};
+  p.block_table = t.t->data_ptr<int>(), p.lens = l.t->const_data_ptr<int>(), p.new_lens = n.t->const_data_ptr<int>(), p.free_pages = f.t->data_ptr<int>();
+  p.free_count = c.t->const_data_ptr<int>(), p.lens_out = lens.data_ptr<int>(), p.granted = granted.data_ptr<int>(), p.starts = starts.data_ptr<int>();
+  p.free_count_out = count.data_ptr<int>(), p.positions = pos.data_ptr<int64_t>(), p.slots = slots.data_ptr<int64_t>();
+  p.table_stride = stride, p.tokens = tokens, p.B = (int)B, p.W = (int)W, p.page_size = (int)page, p.capacity = (int)cap;
+  if (light_b200_paged_advance(&p, dev, stream_of(dev)) != 0) Py_RETURN_NONE;
+  return tuple_of({pos, slots, starts, lens, granted, count});
+}
+
+// (block table, lens, done, free pages, free count, page size, inplace) -> (lens, free count)
+PyObject *paged_release(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  ARGS(7)
+  Arg t, l, d, f, c;
+  long long page;
+  NEED(t.ok(a[0]) && l.ok(a[1]) && d.ok(a[2]) && f.ok(a[3]) && c.ok(a[4]) && long_of(a[5], page));
+  const int inplace = PyObject_IsTrue(a[6]);
+  if (inplace < 0) return nullptr;
+  const int64_t stride = table_of(*t.t);
+  NEED(stride > 0);
+  const int dev = t.t->get_device();
+  const int64_t B = t.t->size(0), W = t.t->size(1), cap = f.t->numel();
+  NEED(i32_of(*l.t, dev, B) && i32_of(*c.t, dev, 1) && f.t->dim() == 1 && cap > 0 && cap < (1ll << 31) && i32_of(*f.t, dev, cap) && d.t->is_cuda() && d.t->is_contiguous() &&
+       d.t->scalar_type() == at::kBool && d.t->numel() == B && d.t->get_device() == dev);
+  NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31));
+  at::Tensor lens = inplace ? *l.t : at::empty({B}, l.t->options()), count = inplace ? *c.t : at::empty({1}, l.t->options());
+  lb200_paged_pages p{};
+  p.block_table = t.t->data_ptr<int>(), p.lens = l.t->const_data_ptr<int>(), p.done = (const uint8_t *)d.t->const_data_ptr(), p.free_pages = f.t->data_ptr<int>();
+  p.free_count = c.t->const_data_ptr<int>(), p.lens_out = lens.data_ptr<int>(), p.free_count_out = count.data_ptr<int>();
+  p.table_stride = stride, p.B = (int)B, p.W = (int)W, p.page_size = (int)page, p.capacity = (int)cap;
+  if (light_b200_paged_release(&p, dev, stream_of(dev)) != 0) Py_RETURN_NONE;
+  return tuple_of({lens, count});
+}
+
+// (q, k, positions, frequencies, q weight or None, k weight or None, eps, interleaved, factor, v, k cache, v cache, slots: all four or None) -> (q, k or None)
+PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  ARGS(13)
+  Arg q, k, pos, freq, w[2], v, kc, vc, sl;
+  NEED(q.ok(a[0]) && k.ok(a[1]) && pos.ok(a[2]) && freq.ok(a[3]) && PyFloat_Check(a[6]) && PyFloat_Check(a[8]));
+  const int interleaved = PyObject_IsTrue(a[7]);
+  if (interleaved < 0) return nullptr;
+  NEED(q.t->is_cuda() && q.t->dim() == 3);
+  const int dev = q.t->get_device();
+  const auto dt = q.t->scalar_type();
+  const int64_t T = q.t->size(0), NH = q.t->size(1), D = q.t->size(2);
+  NEED(act_of(*q.t) >= 0 && T > 0 && D > 0 && heads_of(*q.t, T, D, dt, dev) && heads_of(*k.t, T, D, dt, dev));
+  const int64_t KH = k.t->size(1), R = 2 * freq.t->numel();
+  NEED(pos.t->is_cuda() && pos.t->scalar_type() == at::kLong && pos.t->dim() == 1 && pos.t->size(0) == T && pos.t->is_contiguous() && pos.t->get_device() == dev);
+  NEED(cuda_contig(*freq.t) && freq.t->scalar_type() == at::kDouble && freq.t->dim() == 1 && R <= D && freq.t->get_device() == dev);
+  for (int i = 0; i < 2; i++)
+    if (a[4 + i] != Py_None)
+      NEED(w[i].ok(a[4 + i]) && cuda_contig(*w[i].t) && w[i].t->scalar_type() == dt && w[i].t->dim() == 1 && w[i].t->size(0) == D && w[i].t->get_device() == dev);
+  const bool cached = a[12] != Py_None;
+  for (int i = 9; i < 12; i++) NEED((a[i] != Py_None) == cached);
+  lb200_qk_norm_rope_args p{};
+  if (cached) {
+    NEED(v.ok(a[9]) && kc.ok(a[10]) && vc.ok(a[11]) && sl.ok(a[12]) && heads_of(*v.t, T, D, dt, dev) && v.t->size(1) == KH && cache_of(*kc.t, *vc.t, KH, D, dt, dev, true));
+    NEED(sl.t->is_cuda() && sl.t->scalar_type() == at::kLong && sl.t->dim() == 1 && sl.t->size(0) == T && sl.t->is_contiguous() && sl.t->get_device() == dev);
+    p.v = v.t->const_data_ptr(), p.slots = sl.t->const_data_ptr<int64_t>(), p.k_out = kc.t->data_ptr(), p.v_out = vc.t->data_ptr();
+    for (int i = 0; i < 3; i++) p.k_cache_stride[i] = kc.t->stride(i), p.v_cache_stride[i] = vc.t->stride(i);
+    for (int i = 0; i < 2; i++) p.v_stride[i] = v.t->stride(i);
+    p.pages = kc.t->size(0), p.page_size = (int)kc.t->size(2);
+  }
+  at::Tensor q_out = at::empty({T, NH, D}, q.t->options()), k_out;
+  if (!cached) k_out = at::empty({T, KH, D}, q.t->options()), p.k_out = k_out.data_ptr(), p.page_size = 1;
+  p.q = q.t->const_data_ptr(), p.k = k.t->const_data_ptr(), p.q_weight = w[0].t ? w[0].t->const_data_ptr() : nullptr, p.k_weight = w[1].t ? w[1].t->const_data_ptr() : nullptr;
+  p.positions = pos.t->const_data_ptr<int64_t>(), p.inv_freq = freq.t->const_data_ptr<double>(), p.q_out = q_out.data_ptr();
+  for (int i = 0; i < 2; i++) p.q_stride[i] = q.t->stride(i), p.k_stride[i] = k.t->stride(i);
+  p.T = T, p.dtype = act_of(*q.t), p.NH = (int)NH, p.KH = (int)KH, p.D = (int)D, p.rotary = (int)R, p.interleaved = interleaved;
+  p.eps = (float)PyFloat_AsDouble(a[6]), p.factor = (float)PyFloat_AsDouble(a[8]);
+  if (light_b200_qk_norm_rope(&p, dev, stream_of(dev)) != 0) Py_RETURN_NONE;
+  PyObject *t = PyTuple_New(2);
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(q_out));
+  if (cached) Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(t, 1, cached ? Py_None : THPVariable_Wrap(k_out));
+  return t;
+}
+
+// (q, k cache, v cache, block table, lens, scale, window, softcap) -> (B, NH, D)
+PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+  ARGS(8)
+  Arg q, k, v, t, l;
+  long long window;
+  NEED(q.ok(a[0]) && k.ok(a[1]) && v.ok(a[2]) && t.ok(a[3]) && l.ok(a[4]) && PyFloat_Check(a[5]) && long_of(a[6], window) && PyFloat_Check(a[7]));
+  NEED(q.t->is_cuda() && q.t->dim() == 3 && k.t->dim() == 4 && window >= 0 && window < (1ll << 31));
+  const int dev = q.t->get_device();
+  const auto dt = q.t->scalar_type();
+  const int64_t B = q.t->size(0), NH = q.t->size(1), D = q.t->size(2), KH = k.t->size(1), stride = table_of(*t.t);
+  NEED(act_of(*q.t) >= 0 && B > 0 && D > 0 && KH > 0 && NH % KH == 0 && heads_of(*q.t, B, D, dt, dev) && cache_of(*k.t, *v.t, KH, D, dt, dev, false));
+  NEED(stride > 0 && t.t->size(0) == B && t.t->size(1) < (1ll << 31) && t.t->get_device() == dev && l.t->dim() == 1 && i32_of(*l.t, dev, B) && k.t->size(2) < (1ll << 31));
+  at::Tensor out = at::empty({B, NH, D}, q.t->options()), own;
+  lb200_paged_attn_args p{};
+  p.q = q.t->const_data_ptr(), p.k = k.t->const_data_ptr(), p.v = v.t->const_data_ptr(), p.block_table = t.t->const_data_ptr<int>(), p.lens = l.t->const_data_ptr<int>();
+  p.out = out.data_ptr();
+  for (int i = 0; i < 2; i++) p.q_stride[i] = q.t->stride(i);
+  for (int i = 0; i < 3; i++) p.k_stride[i] = k.t->stride(i), p.v_stride[i] = v.t->stride(i);
+  p.table_stride = stride, p.pages = k.t->size(0), p.dtype = act_of(*q.t), p.B = (int)B, p.NH = (int)NH, p.KH = (int)KH, p.D = (int)D, p.page_size = (int)k.t->size(2);
+  p.W = (int)t.t->size(1), p.window = (int)window, p.scale = (float)PyFloat_AsDouble(a[5]), p.softcap = (float)PyFloat_AsDouble(a[7]);
+  p.scratch_bytes = light_b200_paged_attn_scratch_bytes(&p, dev);
+  if (p.scratch_bytes) own = at::empty({(int64_t)p.scratch_bytes}, q.t->options().dtype(at::kByte)), p.scratch = own.data_ptr();
+  return give(light_b200_paged_decode_attn(&p, dev, stream_of(dev)), out);
+}
+
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -325,6 +473,10 @@ PyMethodDef kMethods[] = {FN(set_workspace, "registers a device's workspace size
                           FN(moe_route, "top-k experts of each token and the pairs sorted by expert"),
                           FN(moe_gemm, "grouped x . W^T"),
                           FN(decode_attention, "append + rotary embedding + attention"),
+                          FN(paged_advance, "pages, slots and positions of a step's tokens"),
+                          FN(paged_release, "pages of finished requests"),
+                          FN(qk_norm_rope, "norm, rotation and cache rows of queries and keys"),
+                          FN(paged_attention, "attention of one token over a paged cache"),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "native host path of light_b200", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

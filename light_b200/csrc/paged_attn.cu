@@ -694,8 +694,9 @@ Cut cut_of(const lb200_paged_attn_args *p) {
   Cut c{};
   const int size = p->dtype == LB200_F32 ? 4 : 2, G = p->NH / p->KH;
   uint64_t off = (uint64_t)(uintptr_t)p->q | (uint64_t)(uintptr_t)p->k | (uint64_t)(uintptr_t)p->v;
-  for (int i = 0; i < 2; i++) off |= (uint64_t)p->q_stride[i] * size;
-  for (int i = 0; i < 3; i++) off |= (uint64_t)p->k_stride[i] * size | (uint64_t)p->v_stride[i] * size;
+  const long long nq[2] = {p->B, p->NH}, nk[3] = {p->pages, p->KH, p->page_size};
+  for (int i = 0; i < 2; i++) off |= nq[i] > 1 ? (uint64_t)p->q_stride[i] * size : 0;  // (the stride of an extent of one moves nothing)
+  for (int i = 0; i < 3; i++) off |= nk[i] > 1 ? (uint64_t)p->k_stride[i] * size | (uint64_t)p->v_stride[i] * size : 0;
   c.streamed = p->D % 16 == 0 && !(off & 15);
   if (!c.streamed) return c;
   c.groups = (G + 15) / 16, c.hpg = (G + c.groups - 1) / c.groups, c.groups = (G + c.hpg - 1) / c.hpg;

@@ -951,6 +951,9 @@ def PagedAdvance(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.
     its first free_count entries) and are written into block_table (B, W) I32.  A request gets all of its pages or none (PagedStep.granted;
     ops.paged_status reports it).  `tokens`: rows of the batch, those behind the last token are padding (slot -1).  With `inplace` lens
     and free_count hold the new values, else PagedStep does and they stay.  No gradients."""
+    r = _host.paged_advance(block_table, lens, new_lens, free_pages, free_count, page_size, tokens, inplace)
+    if r is not None:
+        return PagedStep(*r[:3], lens, r[4], free_count) if inplace else PagedStep(*r)
     dev, B, a = _pages_args("PagedAdvance", block_table, lens, free_pages, free_count, page_size)
     _i32("PagedAdvance", block_table.device, new_lens=new_lens)
     if new_lens.numel() != B or tokens < 0:
@@ -969,6 +972,9 @@ def PagedRelease(block_table: torch.Tensor, lens: torch.Tensor, done: torch.Tens
                  inplace: bool = False):
     """The pages of the requests marked in `done` (B,) bool back on the stack of free ones, in one launch (light_b200_paged_release); free_pages
     gets the entries, the answer is (lens, free_count), the tensors themselves with `inplace`."""
+    r = _host.paged_release(block_table, lens, done, free_pages, free_count, page_size, inplace)
+    if r is not None:
+        return (lens, free_count) if inplace else r
     dev, B, a = _pages_args("PagedRelease", block_table, lens, free_pages, free_count, page_size)
     if done.dtype != torch.bool or done.numel() != B or not done.is_contiguous() or done.device != lens.device:
         raise ValueError(f"ops.PagedRelease: done must be a contiguous bool tensor of {B} on {lens.device}, got {done.dtype} {tuple(done.shape)} on {done.device}")
@@ -1041,6 +1047,9 @@ def QKNormRoPE(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fr
     rotary elements of a head turn, in pairs (i, i + rotary / 2), or (2 i, 2 i + 1) with `interleaved`.  Caches (pages, KH, page size, D)
     of any order, slots (T,) I64 (ops.PagedAdvance): key and value of a token with a negative slot go nowhere; of two tokens with one slot
     either may stay.  Returns (q, k), k None where it went to the cache.  No gradients."""
+    r = _host.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, factor, v, k_cache, v_cache, slots)
+    if r is not None:
+        return r
     for name, x in (("q", q), ("k", k)):
         if x.dim() != 3 or x.shape[0] != q.shape[0] or x.shape[2] != q.shape[2] or x.dtype != q.dtype or x.device != q.device or x.shape[1] == 0 or x.shape[2] == 0:
             raise ValueError(f"ops.QKNormRoPE: want q (T, NH, D) and k (T, KH, D) of one type, got {name} {tuple(x.shape)} {x.dtype} on {x.device} beside q {tuple(q.shape)} {q.dtype}")
@@ -1091,6 +1100,9 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     head and row, block_table (B, W) I32, lens (B,) I32 valid keys of each sequence, the new token's among them -> (B, NH, D).  window: the
     last `window` keys only; softcap: scores softcap * tanh(scale q.k / softcap).  A sequence without keys (or whose scores are all -inf)
     gives zeros; lengths beyond the table and pages outside the cache are reported by ops.paged_status.  No gradients."""
+    y = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap)
+    if y is not None:
+        return y
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[2] == 0:
         raise ValueError(f"ops.PagedDecodeAttention: want q (B, NH, HD), got {tuple(q.shape)}")
     if q.dtype not in _ACT:
