@@ -311,6 +311,193 @@ __global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) 
   }
 }
 
+// Rows that can be cut into chunks of CB bytes.  A warp takes a token (or, of few tokens, some of a token's heads); lg lanes take a head, two chunks
+// each, chosen so that the pairs of the rotation are in one lane: chunk c and the one R / 2 elements on, or any two where the pairs are
+// neighbours.  So a head is read and written once, in whole sectors, its mean square is log2(lg) shuffles, and an angle's sine and cosine
+// stay in registers for all heads of the token.  Bound by the memory: 2 (NH + 2 KH) D elements per token.
+constexpr int RC_WARPS = 4, RC_AHEAD = 2;  // heads of a lane that are on their way together
+
+struct Chunks {
+  int lg, split, first, count;  // lanes per head, warps per token; chunks that a lane's second lies behind its first; chunks per head
+};
+
+template <int CB>
+struct Raw {
+  uint32_t w[CB / 4];
+};
+template <int CB>
+__device__ __forceinline__ Raw<CB> ld_raw(const void *p) {
+  Raw<CB> r;
+  if constexpr (CB == 16) {
+    const uint4 v = __ldcs(static_cast<const uint4 *>(p));
+    r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+  } else if constexpr (CB == 8) {
+    const uint2 v = __ldcs(static_cast<const uint2 *>(p));
+    r.w[0] = v.x, r.w[1] = v.y;
+  } else {
+    r.w[0] = __ldcs(static_cast<const uint32_t *>(p));
+  }
+  return r;
+}
+template <int CB>
+__device__ __forceinline__ void st_raw(void *p, const Raw<CB> &r) {
+  if constexpr (CB == 16) *static_cast<uint4 *>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  else if constexpr (CB == 8) *static_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
+  else *static_cast<uint32_t *>(p) = r.w[0];
+}
+template <typename T, int CB>
+__device__ __forceinline__ void unpack(const Raw<CB> &r, float (&f)[CB / sizeof(T)]) {
+#pragma unroll
+  for (int i = 0; i < CB / 4; i++) {
+    if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(r.w[i]);
+    else {
+      const T *h = reinterpret_cast<const T *>(&r.w[i]);
+      f[2 * i] = to_f32(h[0]), f[2 * i + 1] = to_f32(h[1]);
+    }
+  }
+}
+template <typename T, int CB>
+__device__ __forceinline__ Raw<CB> packed(const float (&f)[CB / sizeof(T)]) {
+  Raw<CB> r;
+#pragma unroll
+  for (int i = 0; i < CB / 4; i++) {
+    if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(f[i]);
+    else {
+      T *h = reinterpret_cast<T *>(&r.w[i]);
+      h[0] = from_f32<T>(f[2 * i]), h[1] = from_f32<T>(f[2 * i + 1]);
+    }
+  }
+  return r;
+}
+
+template <typename T, int CB>
+__global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(RotateArgs a, Chunks ch) {
+  constexpr int E = CB / (int)sizeof(T);
+  __shared__ float2 trig[RC_WARPS][RT_MAX_D / 2];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.R >> 1;
+  const long long id = (long long)blockIdx.x * RC_WARPS + warp, t = id / ch.split;
+  if (t >= a.T) return;
+  const int part = (int)(id - t * ch.split), gl = lane & (ch.lg - 1), per = 32 / ch.lg;
+  // this lane's chunks, -1 for none
+  int c0, c1;
+  bool turns;  // half layout: the lane's two chunks are pairs
+  if (a.interleaved) {
+    turns = false, c0 = gl < ch.count ? gl : -1, c1 = gl < ch.first && gl + ch.first < ch.count ? gl + ch.first : -1;
+    if (gl >= ch.first) c0 = -1;
+  } else {
+    turns = gl < ch.first;
+    c0 = turns ? gl : 2 * ch.first + 2 * (gl - ch.first), c1 = turns ? gl + ch.first : c0 + 1;
+    if (c0 >= ch.count) c0 = -1;
+    if (c1 >= ch.count) c1 = -1;
+  }
+  const long long pos = a.positions[t];
+  long long slot = -1;
+  int page = 0, row = 0;
+  if (a.slots) {
+    slot = a.slots[t];
+    if (slot >= a.rows) {
+      if (lane == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
+      slot = -1;
+    }
+    if (slot >= 0) page = (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
+  }
+  const int heads = a.slots ? (slot >= 0 ? a.NH + 2 * a.KH : a.NH) : a.NH + a.KH;
+  const T *q = static_cast<const T *>(a.q) + t * a.q_s[0], *k = static_cast<const T *>(a.k) + t * a.k_s[0], *v = static_cast<const T *>(a.v) + t * a.v_s[0];
+  const int h0 = part * per + lane / ch.lg, step = ch.split * per;
+  auto fetch = [&](int h, Raw<CB> &x, Raw<CB> &y) {
+    if (h >= heads) return;
+    const T *p = h < a.NH ? q + h * a.q_s[1] : h < a.NH + a.KH ? k + (h - a.NH) * a.k_s[1] : v + (h - a.NH - a.KH) * a.v_s[1];
+    if (c0 >= 0) x = ld_raw<CB>(p + c0 * E);
+    if (c1 >= 0) y = ld_raw<CB>(p + c1 * E);
+  };
+  Raw<CB> x[RC_AHEAD], y[RC_AHEAD];
+#pragma unroll
+  for (int i = 0; i < RC_AHEAD; i++) x[i] = Raw<CB>{}, y[i] = Raw<CB>{}, fetch(h0 + i * step, x[i], y[i]);
+  for (int i = lane; i < half; i += 32) {
+    const float2 cs = cos_sin(pos, a.inv_freq[i]);
+    trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
+  }
+  __syncwarp();
+  float2 cs[E];
+  unsigned turned = 0;  // interleaved: bit j: pair j of the first chunk turns; E / 2 + j: of the second
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    int i = c0 * E + e;
+    bool on = turns;
+    if (a.interleaved) {
+      const int c = e < E / 2 ? c0 : c1;
+      i = c * (E / 2) + e % (E > 1 ? E / 2 : 1), on = c >= 0 && i < half;
+      turned |= (unsigned)on << e;
+    }
+    cs[e] = on ? trig[warp][i] : make_float2(1.f, 0.f);
+  }
+  Raw<CB> wq0{}, wq1{}, wk0{}, wk1{};
+  if (a.qw) {
+    const T *w = static_cast<const T *>(a.qw);
+    if (c0 >= 0) wq0 = ld_raw<CB>(w + c0 * E);
+    if (c1 >= 0) wq1 = ld_raw<CB>(w + c1 * E);
+  }
+  if (a.kw) {
+    const T *w = static_cast<const T *>(a.kw);
+    if (c0 >= 0) wk0 = ld_raw<CB>(w + c0 * E);
+    if (c1 >= 0) wk1 = ld_raw<CB>(w + c1 * E);
+  }
+  for (int base = part * per; base < heads; base += RC_AHEAD * step) {
+#pragma unroll
+    for (int i = 0; i < RC_AHEAD; i++) {
+      const int h = base + lane / ch.lg + i * step;
+      const bool is_q = h < a.NH, is_v = h >= a.NH + a.KH;
+      const void *w = is_q ? a.qw : a.kw;
+      float f[E], g[E];
+      unpack<T, CB>(x[i], f), unpack<T, CB>(y[i], g);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; e++) ss = fmaf(f[e], f[e], ss);
+#pragma unroll
+      for (int e = 0; e < E; e++) ss = fmaf(g[e], g[e], ss);
+      if (a.qw || a.kw)
+        for (int o = ch.lg >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      Raw<CB> u = x[i], z = y[i];
+      if (!is_v) {
+        if (w) {
+          const float inv = rsqrtf(ss / (float)a.D + a.eps);
+          float wf[E], wg[E];
+          unpack<T, CB>(is_q ? wq0 : wk0, wf), unpack<T, CB>(is_q ? wq1 : wk1, wg);
+#pragma unroll
+          for (int e = 0; e < E; e++) f[e] = f[e] * inv * wf[e], g[e] = g[e] * inv * wg[e];
+        }
+        if (a.interleaved) {
+#pragma unroll
+          for (int e = 0; e + 1 < E; e += 2) {
+            const float2 p = cs[e / 2], r = cs[E / 2 + e / 2];
+            const float f0 = f[e] * p.x - f[e + 1] * p.y, f1 = f[e] * p.y + f[e + 1] * p.x, g0 = g[e] * r.x - g[e + 1] * r.y, g1 = g[e] * r.y + g[e + 1] * r.x;
+            if (turned >> (e / 2) & 1) f[e] = f0, f[e + 1] = f1;
+            if (turned >> (E / 2 + e / 2) & 1) g[e] = g0, g[e + 1] = g1;
+          }
+        } else if (turns) {
+#pragma unroll
+          for (int e = 0; e < E; e++) {
+            const float f0 = f[e] * cs[e].x - g[e] * cs[e].y, g0 = f[e] * cs[e].y + g[e] * cs[e].x;
+            f[e] = f0, g[e] = g0;
+          }
+        }
+        u = packed<T, CB>(f), z = packed<T, CB>(g);
+      }
+      if (h < heads) {
+        const int kh = is_v ? h - a.NH - a.KH : h - a.NH;
+        T *to = is_q   ? static_cast<T *>(a.q_out) + (t * a.NH + h) * a.D
+                : is_v ? static_cast<T *>(a.v_out) + page * a.vs[0] + kh * a.vs[1] + row * a.vs[2]
+                       : static_cast<T *>(a.k_out) + (a.slots ? page * a.ks[0] + kh * a.ks[1] + row * a.ks[2] : (t * a.KH + kh) * a.D);
+        if (c0 >= 0) st_raw<CB>(to + c0 * E, u);
+        if (c1 >= 0) st_raw<CB>(to + c1 * E, z);
+      }
+      fetch(h + RC_AHEAD * step, x[i], y[i]);
+    }
+  }
+}
+
 }  // namespace
 
 int paged_pages_check(const lb200_paged_pages *p, const char *what, bool release) {
@@ -363,6 +550,20 @@ int qk_norm_rope_check(const lb200_qk_norm_rope_args *p) {
   return 0;
 }
 
+template <typename T>
+static cudaError_t launch_cb(const RotateArgs &a, const Chunks &ch, int cb, unsigned ctas, cudaStream_t st) {
+  return cb == 16  ? launch_early(qk_norm_rope_chunks_kernel<T, 16>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch)
+         : cb == 8 ? launch_early(qk_norm_rope_chunks_kernel<T, 8>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch)
+                   : launch_early(qk_norm_rope_chunks_kernel<T, 4>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch);
+}
+static int launch_chunks(const RotateArgs &a, const Chunks &ch, int cb, int dtype, unsigned ctas, cudaStream_t st) {
+  const cudaError_t e = dtype == LB200_F32    ? launch_cb<float>(a, ch, cb, ctas, st)
+                        : dtype == LB200_BF16 ? launch_cb<__nv_bfloat16>(a, ch, cb, ctas, st)
+                                              : launch_cb<__half>(a, ch, cb, ctas, st);
+  if (e != cudaSuccess) return fail((int)e, "light_b200: qk_norm_rope: %s", cudaGetErrorString(e));
+  return launched("qk_norm_rope");
+}
+
 int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
   if (p->T == 0) return 0;
   RotateArgs a{};
@@ -372,6 +573,32 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
   a.positions = (const long long *)p->positions, a.slots = (const long long *)p->slots, a.inv_freq = p->inv_freq;
   a.T = p->T, a.rows = p->slots ? p->pages * p->page_size : 0, a.NH = p->NH, a.KH = p->KH, a.D = p->D, a.R = p->rotary, a.interleaved = p->interleaved;
   a.eps = p->eps, a.factor = p->factor, a.page = FastDiv(p->slots ? p->page_size : 1);
+  // chunks as large as the addresses and the distance of a pair's elements allow
+  const int size = p->dtype == LB200_F32 ? 4 : 2;
+  uint64_t off = (uint64_t)(uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->q_out | (uintptr_t)p->k_out | (uintptr_t)p->q_weight | (uintptr_t)p->k_weight | (uint64_t)p->D * size;
+  for (int i = 0; i < 2; i++) off |= (uint64_t)p->q_stride[i] * size | (uint64_t)p->k_stride[i] * size;
+  if (p->slots) {
+    off |= (uintptr_t)p->v | (uintptr_t)p->v_out;
+    for (int i = 0; i < 2; i++) off |= (uint64_t)p->v_stride[i] * size;
+    for (int i = 0; i < 3; i++) off |= (uint64_t)p->k_cache_stride[i] * size | (uint64_t)p->v_cache_stride[i] * size;
+  }
+  if (!p->interleaved) off |= (uint64_t)(p->rotary / 2) * size;
+  int cb = off & 15 ? off & 7 ? off & 3 ? 0 : 4 : 8 : 16;
+  if (p->interleaved && cb < 2 * size) cb = 0;
+  if (cb) {
+    Chunks ch{};
+    ch.count = p->D * size / cb;
+    ch.first = p->interleaved ? (ch.count + 1) / 2 : p->rotary / 2 * size / cb;
+    const int lanes = p->interleaved ? ch.first : ch.first + (ch.count - 2 * ch.first + 1) / 2;
+    for (ch.lg = 1; ch.lg < lanes;) ch.lg *= 2;
+    if (ch.lg <= 32) {
+      // warps per token: until there are eight for every SM, each with a round of heads or more
+      const int heads = p->NH + p->KH * (p->slots ? 2 : 1), rounds = (heads * ch.lg + 31) / 32;
+      for (ch.split = 1; ch.split < rounds && p->T * ch.split < 8ll * sm_count();) ch.split++;
+      const long long ctas = (p->T * ch.split + RC_WARPS - 1) / RC_WARPS;
+      if (ctas <= 0x7fffffffll) return launch_chunks(a, ch, cb, p->dtype, (unsigned)ctas, st);
+    }
+  }
   cudaError_t e;
   if (p->dtype == LB200_F32) e = launch_early(qk_norm_rope_kernel<float>, dim3((unsigned)p->T), dim3(RT_THREADS), st, a);
   else if (p->dtype == LB200_BF16) e = launch_early(qk_norm_rope_kernel<__nv_bfloat16>, dim3((unsigned)p->T), dim3(RT_THREADS), st, a);
