@@ -32,13 +32,19 @@ __device__ __forceinline__ int length_of(const PagedArgs &a, int b) {
 }
 __device__ __forceinline__ int first_of(const PagedArgs &a, int n) { return a.window > 0 ? max(0, n - a.window) : 0; }
 
+__device__ __forceinline__ float ex2(float x) {  // relative error 2^-22; results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // A score in units of log2 e.  tanh z = 1 - 2 / (e^(2 z) + 1): absolute error of a few 2^-24, which is what a score's error counts by.
 struct Scorer {
   float sc, cap;  // without a cap: scale log2 e; with one: 2 log2 e scale / cap, and cap log2 e
   __device__ Scorer(float scale, float softcap) : sc(softcap > 0.f ? 2.f * LOG2E * scale / softcap : scale * LOG2E), cap(softcap * LOG2E) {}
   __device__ __forceinline__ float operator()(float dot) const {
     const float x = dot * sc;
-    return cap > 0.f ? cap - cap * 2.f * __fdividef(1.f, exp2f(x) + 1.f) : x;
+    return cap > 0.f ? cap - cap * 2.f * __fdividef(1.f, ex2(x) + 1.f) : x;
   }
 };
 
@@ -73,7 +79,7 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
     for (int i = 0; i < P; i++)
       if (lane + 32 * i < a.D) d = fmaf(qf[i], to_f32(kr[lane + 32 * i]), d);
     const float s = score(warp_sum(d)), mx = fmaxf(m, s), use = mx == -INFINITY ? 0.f : mx;
-    const float corr = exp2f(m - use), p = exp2f(s - use);
+    const float corr = ex2(m - use), p = ex2(s - use);
     m = mx, l = fmaf(l, corr, p);
 #pragma unroll
     for (int i = 0; i < P; i++)
@@ -89,11 +95,11 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
   for (int w = 0; w < PL_WARPS; w++) top = fmaxf(top, part[w][0]);
   if (top == -INFINITY) top = 0.f;
 #pragma unroll
-  for (int w = 0; w < PL_WARPS; w++) L = fmaf(exp2f(part[w][0] - top), part[w][1], L);
+  for (int w = 0; w < PL_WARPS; w++) L = fmaf(ex2(part[w][0] - top), part[w][1], L);
   for (int d = threadIdx.x; d < a.D; d += PL_WARPS * 32) {
     float A = 0.f;
 #pragma unroll
-    for (int w = 0; w < PL_WARPS; w++) A = fmaf(exp2f(part[w][0] - top), part[w][2 + d], A);
+    for (int w = 0; w < PL_WARPS; w++) A = fmaf(ex2(part[w][0] - top), part[w][2 + d], A);
     static_cast<T *>(a.out)[(long long)blockIdx.x * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
   }
 }
@@ -101,20 +107,21 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 // ------------------------------------------------------------------------------------ rows on 16 bytes, head sizes of whole 16s
 // The caches are read once (2 n KH D elements) and everything else is small, so the kernel is a stream: what it does is keep loads in
 // flight on every SM whatever the lengths are.
-//   * Work is cut evenly.  A unit is a sequence's KV head (with up to 16 of its query heads); its keys come in tiles of one block per warp.
-//     All tiles of all units in order are dealt to the CTAs in equal runs, a long sequence over many CTAs, many short ones to one.  Every CTA
-//     scans the lengths for itself.  A unit that one CTA holds whole is written out by it; pieces of one that is cut go to scratch
-//     as (max, sum, sum p v), at most two a CTA, and a second launch joins each unit's pieces in their order: no atomics, the same bits
-//     every time.
-//   * A warp is on its own: it copies its block of keys and values (16 rows of each, 8 of f32) into a ring of its own by 16-byte
-//     asynchronous copies, the next blocks' page numbers being read meanwhile, and folds blocks into its own running (max, sum, sum
-//     p v).  No barrier between warps but at the end of a unit.  Rows without a key are filled with zeros: a weight of 0 times what lies there
-//     must not be NaN.
-constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
+//   * Work is cut evenly.  A unit is a sequence's KV head (with up to 16 of its query heads); its keys come in blocks of 16 rows (f32: 8).
+//     All blocks of all units in order are dealt to the warps in runs of equal cost, a long sequence over many, many short ones to one; what a
+//     unit costs beside its blocks counts as UNIT of them.  Every CTA scans the lengths for itself.
+//   * A warp is on its own: it copies its blocks of keys and values into a ring of its own by 16-byte asynchronous copies, the next
+//     blocks' page numbers being read meanwhile, folds them into a running (max, sum, sum p v), and writes a unit out that it holds whole.  Rows
+//     without a key are filled with zeros: a weight of 0 times what lies there must not be NaN.
+//   * Pieces of a unit that was cut are joined in their order, first those of a CTA's warps at its end, in shared memory; what goes on
+//     over CTAs goes to scratch, at most two pieces a CTA, and a second launch joins those: no atomics, the same bits every time.
+constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3;
 
 struct SplitArgs {
   PagedArgs p;
   int hpg, groups;    // query heads per unit, units per KV head
+  uint32_t ku[3], vu[3], unit;  // the cache's strides in units of so many bytes, in which every row's offset has 32 bits
+  bool alike;         // ku == vu
   int4 *heads;        // per CTA: sequence, unit of it, pieces of the unit that begins there and goes on (0: none)
   float *ml, *acc;    // [2 CTAs][HEADS][2], [2 CTAs][HEADS][D]
 };
@@ -167,7 +174,7 @@ struct MmaBlock {
   uint32_t q[DP / 16][NT][2];
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
 
-  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *, int) {
+  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *) {
     const PagedArgs &a = s.p;
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -187,30 +194,34 @@ struct MmaBlock {
     }
   }
 
-  __device__ __forceinline__ void block(const PagedArgs &a, const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *, int) {
+  __device__ __forceinline__ void block(const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
-    float s[NT][4];
+    float s[NT][4], s2[NT][4];  // (two sums: half the chain of dependent instructions)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = 0.f;
+      for (int e = 0; e < 4; e++) s[nt][e] = s2[nt][e] = 0.f;
     const int turn = spread(lane & 7);
     const uint32_t krow = kbase + (lane & 15) * ROWB, vrow = kbase + KB * ROWB + ((lane & 7) + (lane >> 4) * 8) * ROWB;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ks++)
-      if (ks * 16 < a.D) {
-        uint32_t f[4];
-        ldm4(f, krow + (((2 * ks + (lane >> 4)) ^ turn) << 4));
+    for (int ks = 0; ks < DP / 16; ks++) {
+      uint32_t f[4];
+      ldm4(f, krow + (((2 * ks + (lane >> 4)) ^ turn) << 4));
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) mma(s[nt], f, q[ks][nt][0], q[ks][nt][1], T());
-      }
+      for (int nt = 0; nt < NT; nt++) mma(ks & 1 ? s2[nt] : s[nt], f, q[ks][nt][0], q[ks][nt][1], T());
+    }
     uint32_t p[NT][2];
     float corr[NT][2];
     bool same = true;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = valid >> (r + 8 * (e >> 1)) & 1 ? score(s[nt][e]) : -INFINITY;
+      for (int e = 0; e < 4; e++) s[nt][e] = score(s[nt][e] + s2[nt][e]);
+      if (valid != 0xFFFFu) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (!(valid >> (r + 8 * (e >> 1)) & 1)) s[nt][e] = -INFINITY;
+      }
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         float mx = fmaxf(s[nt][e], s[nt][2 + e]);
@@ -218,10 +229,10 @@ struct MmaBlock {
         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
         mx = fmaxf(mx, m[nt][e]);
         const float use = mx == -INFINITY ? 0.f : mx;  // no key above -inf so far: all weights 0
-        corr[nt][e] = exp2f(m[nt][e] - use);
+        corr[nt][e] = ex2(m[nt][e] - use);
         same = same && mx == m[nt][e];
         m[nt][e] = mx;
-        s[nt][e] = exp2f(s[nt][e] - use), s[nt][2 + e] = exp2f(s[nt][2 + e] - use);
+        s[nt][e] = ex2(s[nt][e] - use), s[nt][2 + e] = ex2(s[nt][2 + e] - use);
       }
       const uint32_t lo = pack(s[nt][0], s[nt][1], T()), hi = pack(s[nt][2], s[nt][3], T());
       p[nt][0] = transposed(lo), p[nt][1] = transposed(hi);
@@ -237,13 +248,39 @@ struct MmaBlock {
           for (int e = 0; e < 4; e++) o[t][nt][e] *= corr[nt][e & 1];
     }
 #pragma unroll
-    for (int t = 0; t < DP / 16; t++)
-      if (t * 16 < a.D) {
-        uint32_t f[4];
-        ldm4_trans(f, vrow + (((2 * t + (lane >> 3 & 1)) ^ turn) << 4));
+    for (int t = 0; t < DP / 16; t++) {
+      uint32_t f[4];
+      ldm4_trans(f, vrow + (((2 * t + (lane >> 3 & 1)) ^ turn) << 4));
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) mma(o[t][nt], f, p[nt][0], p[nt][1], T());
+      for (int nt = 0; nt < NT; nt++) mma(o[t][nt], f, p[nt][0], p[nt][1], T());
+    }
+  }
+
+  // the result of `count` heads from `out` on
+  __device__ __forceinline__ void write(T *out, int count, int D, unsigned char *) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      float inv[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float sum = l[nt][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        l[nt][e] = sum, inv[e] = 1.f / sum;
       }
+      const bool none0 = l[nt][0] == 0.f, none1 = l[nt][1] == 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; t++)
+        if (t * 16 < D) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float x = none0 ? 0.f : o[t][nt][2 * e] * inv[0], y = none1 ? 0.f : o[t][nt][2 * e + 1] * inv[1];
+            const uint32_t v = transposed(pack(x, y, T()));  // head 8 nt + r, dims 2 c and 2 c + 1 of eight
+            if (8 * nt + r < count) *reinterpret_cast<uint32_t *>(out + (8 * nt + r) * D + 16 * t + 8 * e + 2 * c) = v;
+          }
+        }
+    }
   }
 
   __device__ __forceinline__ void store(float *part, int D) {  // [HEADS][PR]: max, sum, -, -, D dims
@@ -272,16 +309,20 @@ struct F32Block {
   using T = float;
   static constexpr int DP = DP_, KB = 8, HEADS = GH, ROWB = DP * 4, PR = DP + 4;
   static constexpr int OWN = GH < 4 ? 1 : GH / 4, NC = DP < 128 ? 1 : DP / 128, SPLIT = DP < 128 ? 128 / DP : 1;  // heads of a lane; chunks; keys side by side
-  static constexpr int QS = GH * DP * 4, PS = KB * GH * 4 + GH * 4, EXTRA = QS + PA_WARPS * PS;  // queries | per warp: weights, corrections
+  static constexpr int QS = GH * DP * 4, PS = (KB * GH * 4 + GH * 4 + 15) / 16 * 16, EXTRA = QS + PS;  // of a warp: queries | weights, corrections
   float acc[GH][NC][4], m[OWN], l[OWN];
 
-  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *extra, int) {
+  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *extra) {
     const PagedArgs &a = s.p;
-    float *qs = reinterpret_cast<float *>(extra);
-    for (int i = threadIdx.x; i < GH * DP; i += PA_THREADS) {
-      const int h = i / DP, d = i % DP;
-      qs[i] = h < count && d < a.D ? static_cast<const float *>(a.q)[b * a.q_s[0] + (kh * a.G + h0 + h) * a.q_s[1] + d] : 0.f;
+    float4 *qs = reinterpret_cast<float4 *>(extra);
+    __syncwarp();  // (the unit before is done with them)
+#pragma unroll 1
+    for (int i = threadIdx.x & 31; i < GH * DP / 4; i += 32) {
+      const int h = i / (DP / 4), c = i % (DP / 4);
+      qs[i] = h < count && 4 * c < a.D ? *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + b * a.q_s[0] + (kh * a.G + h0 + h) * a.q_s[1] + 4 * c)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < OWN; i++) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
@@ -290,32 +331,30 @@ struct F32Block {
       for (int i = 0; i < NC; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[h][i][e] = 0.f;
-    __syncthreads();
   }
 
   __device__ __forceinline__ static int first_head(int lane) { return GH >= 4 ? (lane & 2 ? GH / 2 : 0) + (lane & 1 ? GH / 4 : 0) : GH == 2 ? lane >> 1 & 1 : 0; }
 
-  __device__ __forceinline__ void block(const PagedArgs &a, const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *extra, int warp) {
+  __device__ __forceinline__ void block(const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *extra) {
     const int lane = threadIdx.x & 31, key = lane >> 2, qd = lane & 3;
     const float *qs = reinterpret_cast<const float *>(extra);
-    float *ps = reinterpret_cast<float *>(extra + QS + warp * PS), *cs = ps + KB * GH;
+    float *ps = reinterpret_cast<float *>(extra + QS), *cs = ps + KB * GH;
     float d[GH];
 #pragma unroll
     for (int h = 0; h < GH; h++) d[h] = 0.f;
     const uint32_t krow = kbase + key * ROWB;
     const int turn = spread(key);
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++)
-      if (i * 16 < a.D) {
-        const int c = qd + 4 * i;
-        const uint4 w = lds128(krow + ((c ^ turn) << 4));
-        const float4 k = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+    for (int i = 0; i < DP / 16; i++) {
+      const int c = qd + 4 * i;
+      const uint4 w = lds128(krow + ((c ^ turn) << 4));
+      const float4 k = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
 #pragma unroll
-        for (int h = 0; h < GH; h++) {
-          const float4 q = *reinterpret_cast<const float4 *>(qs + h * DP + 4 * c);
-          d[h] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, d[h]))));
-        }
+      for (int h = 0; h < GH; h++) {
+        const float4 q = *reinterpret_cast<const float4 *>(qs + h * DP + 4 * c);
+        d[h] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, d[h]))));
       }
+    }
     int cnt = GH;
 #pragma unroll
     for (int x = 2; x >= 1; x >>= 1) {
@@ -342,7 +381,7 @@ struct F32Block {
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       mx = fmaxf(mx, m[i]);
-      const float use = mx == -INFINITY ? 0.f : mx, corr = exp2f(m[i] - use), p = exp2f(s - use);
+      const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(m[i] - use), p = ex2(s - use);
       same = same && mx == m[i];
       m[i] = mx, l[i] = fmaf(l[i], corr, p);
       ps[key * GH + h0 + i] = p;
@@ -377,14 +416,42 @@ struct F32Block {
 #pragma unroll
       for (int i = 0; i < NC; i++) {
         const int c = lane % LANES + 32 * i;
-        if (c * 4 < a.D) {
-          const uint4 w = lds128(kbase + (KB + k) * ROWB + ((c ^ spread(k)) << 4));
-          const float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
+        const uint4 w = lds128(kbase + (KB + k) * ROWB + ((c ^ spread(k)) << 4));
+        const float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
 #pragma unroll
-          for (int h = 0; h < GH; h++)
+        for (int h = 0; h < GH; h++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[h][i][e] = fmaf(p[h], v[e], acc[h][i][e]);
-        }
+          for (int e = 0; e < 4; e++) acc[h][i][e] = fmaf(p[h], v[e], acc[h][i][e]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void write(float *out, int count, int D, unsigned char *extra) {
+    const int lane = threadIdx.x & 31, h0 = first_head(lane);
+    float *cs = reinterpret_cast<float *>(extra + QS) + KB * GH;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < OWN; i++) {
+      float sum = l[i];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (lane < 4) cs[h0 + i] = sum;
+    }
+    __syncwarp();
+    constexpr int LANES = 32 / SPLIT;
+#pragma unroll
+    for (int h = 0; h < GH; h++) {
+      const float sum = cs[h], inv = 1.f / sum;
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int x = LANES; x < 32; x <<= 1) acc[h][i][e] += __shfl_xor_sync(0xffffffffu, acc[h][i][e], x);
+        const int c = lane % LANES + 32 * i;
+        if (lane < LANES && c * 4 < D && h < count)
+          *reinterpret_cast<float4 *>(out + h * D + 4 * c) =
+              sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc[h][i][0] * inv, acc[h][i][1] * inv, acc[h][i][2] * inv, acc[h][i][3] * inv);
       }
     }
   }
@@ -413,31 +480,46 @@ struct F32Block {
   }
 };
 
+// shared memory of a CTA with rings of `stages` blocks, and how many CTAs of two blocks or more fit on an SM (three at most: registers)
+constexpr int split_smem(int size, int DP, int HEADS, int stages) {
+  const int rows = size == 2 ? 16 : 8, extra = size == 2 ? 0 : HEADS * DP * 4 + (rows * HEADS * 4 + HEADS * 4 + 15) / 16 * 16;
+  return PA_WARPS * (stages * 2 * rows * DP * size + HEADS * (DP + 4) * 4 + extra);
+}
+constexpr int split_room(int ctas) { return 228 * 1024 / ctas - 1024 - 512; }  // beside what is static
+constexpr int split_ctas(int size, int DP, int HEADS) {
+  int n = DP == 64 ? 3 : DP == 128 ? 2 : 1;
+  while (n > 1 && split_smem(size, DP, HEADS, 2) > split_room(n)) n--;
+  return n;
+}
+constexpr int split_stages(int size, int DP, int HEADS) {
+  int n = 4;
+  while (n > 2 && split_smem(size, DP, HEADS, n) > split_room(split_ctas(size, DP, HEADS))) n--;
+  return n;
+}
+
 template <typename P>
 struct SplitCfg {
-  static constexpr int CTAS = P::DP == 64 ? 3 : P::DP == 128 ? 2 : 1;  // per SM
-  static constexpr int TILE = PA_WARPS * P::KB, STAGE = 2 * P::KB * P::ROWB, PART = PA_WARPS * P::HEADS * P::PR * 4;
-  static constexpr int ROOM = (228 * 1024) / CTAS - 1024 - 256;        // shared memory of a CTA beside what is static
-  static constexpr int stages(int s) { return PART + P::EXTRA + PA_WARPS * s * STAGE <= ROOM ? s : stages(s - 1); }
-  static constexpr int S = stages(4);
-  static constexpr int RING = PA_WARPS * S * STAGE, SMEM = RING + PART + P::EXTRA;
-  static_assert(S >= 2, "a ring of two blocks or more");
+  static constexpr int SIZE = sizeof(typename P::T), CTAS = split_ctas(SIZE, P::DP, P::HEADS), S = split_stages(SIZE, P::DP, P::HEADS);
+  static constexpr int STAGE = 2 * P::KB * P::ROWB, RING = S * STAGE, PART = P::HEADS * P::PR * 4;  // of a warp
+  static constexpr int SMEM = PA_WARPS * (RING + PART + P::EXTRA);
+  static_assert(SMEM == split_smem(SIZE, P::DP, P::HEADS, S) && SMEM <= split_room(CTAS) && PART <= RING, "");
 };
 
 struct Cursor {
-  int b, u, tile, n, j0, tiles;  // sequence, unit of it, tile of that; its length, first key, tiles per unit
-  template <int TILE>
+  int b, u, block, n, j0, blocks;  // sequence, unit of it, block of that; its length, first key, blocks per unit
+  template <int KB>
   __device__ __forceinline__ void at(const PagedArgs &a, int b_) {
-    b = b_, n = length_of(a, b_), j0 = first_of(a, n), tiles = (n - j0 + TILE - 1) / TILE;
+    b = b_, n = length_of(a, b_), j0 = first_of(a, n), blocks = (n - j0 + KB - 1) / KB;
   }
-  template <int TILE>
-  __device__ __forceinline__ void next(const PagedArgs &a, int units) {  // (there is a next tile)
-    if (++tile < tiles) return;
-    tile = 0;
+  template <int KB>
+  __device__ __forceinline__ void next(const PagedArgs &a, int units, int hop) {  // (there is a next block)
+    block += hop;
+    if (block < blocks) return;
+    block = 0;
     if (++u < units) return;
     u = 0;
-    do at<TILE>(a, b + 1);
-    while (tiles == 0);
+    do at<KB>(a, b + 1);
+    while (blocks == 0);
   }
 };
 
@@ -445,67 +527,96 @@ template <typename P>
 __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kernel(SplitArgs s) {
   using C = SplitCfg<P>;
   using T = typename P::T;
-  constexpr int KB = P::KB, TILE = C::TILE, S = C::S, ROWB = P::ROWB;
+  constexpr int KB = P::KB, S = C::S, ROWB = P::ROWB;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long scan[PA_WARPS];
-  __shared__ int from[3];  // where this CTA's tiles begin: sequence, unit, tile
+  __shared__ longlong2 scan[PA_WARPS];
+  __shared__ int4 from[PA_WARPS + 1];              // where the warps' runs begin: sequence, unit, block
+  __shared__ long long place[PA_WARPS + 1], unit0[PA_WARPS + 1];  // the same among all blocks; where the unit begins in cost
   __shared__ uint32_t masks[PA_WARPS][S];
+  __shared__ int open0[PA_WARPS], open1[PA_WARPS];  // pieces: of a unit begun before the run, of the last begun in it: 0 none, 1 ends in it, 2 goes on
+  __shared__ int4 piece0[PA_WARPS], piece1[PA_WARPS];  // their sequence, unit, blocks
+  __shared__ long long cost1[PA_WARPS];             // where in cost the latter begins
   pdl_launch_dependents();
   pdl_wait();
   const PagedArgs &a = s.p;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x, units = a.KH * s.groups;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, units = a.KH * s.groups;
   unsigned odd = 0;
 
-  // ---- this CTA's run of tiles
+  // ---- the warps' runs.  Cost: UNIT, then one for each block, unit after unit; warp i of w has [total i / w, total (i + 1) / w).
   const int per = (a.B + PA_THREADS - 1) / PA_THREADS, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
-  auto tiles_of = [&](int b) {
+  auto blocks_of = [&](int b) {
     const int n = length_of(a, b);
-    return (n - first_of(a, n) + TILE - 1) / TILE;
+    return (n - first_of(a, n) + KB - 1) / KB;
   };
-  long long sum = 0;
+  longlong2 sum = make_longlong2(0, 0);  // blocks, cost: of one unit of each sequence
   for (int b = lo; b < hi; b++) {
     if (cta == 0 && a.lens[b] != length_of(a, b)) odd |= PAGED_LENGTH;
-    sum += tiles_of(b);
+    const int n = blocks_of(b);
+    sum.x += n, sum.y += n ? n + UNIT : 0;
   }
-  long long incl = sum;
+  longlong2 before = sum, total = make_longlong2(0, 0);
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, x);
-    if (lane >= x) incl += v;
+    const long long v = __shfl_up_sync(0xffffffffu, before.x, x), w = __shfl_up_sync(0xffffffffu, before.y, x);
+    if (lane >= x) before.x += v, before.y += w;
   }
-  if (lane == 31) scan[warp] = incl;
+  if (lane == 31) scan[warp] = before;
+  if (tid < PA_WARPS) open0[tid] = open1[tid] = 0;
   __syncthreads();
-  long long before = incl - sum, total = 0;
+  before.x -= sum.x, before.y -= sum.y;
 #pragma unroll
   for (int w = 0; w < PA_WARPS; w++) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
+    if (w < warp) before.x += scan[w].x, before.y += scan[w].y;
+    total.x += scan[w].x, total.y += scan[w].y;
   }
-  total *= units;
-  const int dealt = (int)min((long long)ctas, total);  // CTAs with tiles: the first ones, one or more each, so that a unit's pieces lie in a row
-  const long long t0 = cta < dealt ? total * cta / dealt : 0;
-  const int steps = cta < dealt ? (int)(total * (cta + 1) / dealt - t0) : 0;
-  if (steps > 0 && before * units <= t0 && t0 < (before + sum) * units) {
-    int b = lo, n = tiles_of(b);
-    while ((before + n) * units <= t0) before += n, n = tiles_of(++b);
-    const int r = (int)(t0 - before * units);
-    from[0] = b, from[1] = r / n, from[2] = r % n;
+  total.x *= units, total.y *= units;
+  // CTAs with work: the first ones, PA_WARPS blocks' cost or more each
+  const int dealt = (int)min((long long)gridDim.x, max(total.y / PA_WARPS, 1ll)), runs = dealt * PA_WARPS;
+  const bool small = total.y <= 0x7fffffffll;  // (the 64-bit division takes four times as long)
+  const long long quota = small ? (long long)((unsigned)total.y / (unsigned)runs) : total.y / runs, rest = total.y - quota * runs;
+  auto start_of = [&](int i) { return i * quota + min((long long)i, rest); };
+#pragma unroll 1
+  for (int i = 0; i <= PA_WARPS; i++) {
+    const long long x = cta < dealt ? start_of(cta * PA_WARPS + i) : total.y;
+    if (x >= total.y) {
+      if (tid == 0) from[i] = make_int4(-1, 0, 0, 0), place[i] = total.x;
+    } else if (before.y * units <= x && x < (before.y + sum.y) * units) {
+      longlong2 c = before;
+      int b = lo, n = blocks_of(b);
+      while ((c.y + (n ? n + UNIT : 0)) * units <= x) c.x += n, c.y += n ? n + UNIT : 0, n = blocks_of(++b);
+      from[i] = make_int4(b, n, 0, 0), place[i] = c.x * units, unit0[i] = c.y * units;
+    }
+  }
+  __syncthreads();
+  if (tid <= PA_WARPS && from[tid].x >= 0) {  // the sequence, its blocks and where it begins -> the unit and block
+    const int n = from[tid].y;
+    const long long x = start_of(cta * PA_WARPS + tid), r = x - unit0[tid];
+    const int u = small ? (int)((unsigned)r / (unsigned)(n + UNIT)) : (int)(r / (n + UNIT)), in = (int)(r - (long long)u * (n + UNIT)), block = max(in - UNIT, 0);
+    from[tid] = make_int4(from[tid].x, u, block, n), place[tid] += (long long)u * n + block, unit0[tid] = x - in;
   }
   // sequences without keys
-  for (int b = cta; b < a.B; b += ctas)
-    if (tiles_of(b) == 0)
+  for (int b = cta; b < a.B; b += gridDim.x)
+    if (blocks_of(b) == 0)
       for (int i = tid; i < a.NH * a.D; i += PA_THREADS) static_cast<T *>(a.out)[(long long)b * a.NH * a.D + i] = from_f32<T>(0.f);
   __syncthreads();
-  int4 head = make_int4(0, 0, 0, 0);
 
+  // A CTA inside one unit deals its blocks to the warps in turn, so that they read side by side; else a warp has its own run.
+  const int all = (int)min(place[PA_WARPS] - place[0], 0x7fffffffll);
+  const bool inside = all > 0 && from[0].z + all <= from[0].w;
+  const int steps = inside ? (all - warp + PA_WARPS - 1) / PA_WARPS : (int)(place[warp + 1] - place[warp]), hop = inside ? PA_WARPS : 1;
+  unsigned char *const ring = smem + warp * C::RING, *const extra = smem + PA_WARPS * (C::RING + C::PART) + warp * P::EXTRA;
+  float *const part = reinterpret_cast<float *>(smem + PA_WARPS * C::RING + warp * C::PART);
   if (steps > 0) {
     Cursor now, far;  // what is folded, and what is fetched
-    now.at<TILE>(a, from[0]);
-    now.u = from[1], now.tile = from[2];
+    const int4 at = from[inside ? 0 : warp];
+    now.at<KB>(a, at.x);
+    now.u = at.y, now.block = at.z + (inside ? warp : 0);
     far = now;
-    const uint32_t ring = umma::smem_u32(smem) + warp * S * C::STAGE;
-    float *part = reinterpret_cast<float *>(smem + C::RING);
-    unsigned char *extra = smem + C::RING + C::PART;
+    const uint32_t ring_at = umma::smem_u32(ring);
+    if (a.D < P::DP) {  // chunks past the head: nothing is copied there, and the products run over them
+      for (int i = lane; i < C::RING / 16; i += 32) reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
+    }
 
     struct Row {
       int pg, row, kh;
@@ -513,32 +624,51 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
     };
     auto peek = [&]() {  // the page of this lane's key of the block at `far` (lanes from KB on repeat)
       Row r;
-      const int j = far.j0 + far.tile * TILE + warp * KB + (lane & (KB - 1));
+      const int j = far.j0 + far.block * KB + (lane & (KB - 1));
       const int w = a.page.div(j);
       r.valid = j < far.n, r.row = j - w * a.page.d, r.kh = far.u / s.groups;
       r.pg = r.valid ? a.table[far.b * a.table_stride + w] : -1;
       return r;
     };
     constexpr int E = 16 / (int)sizeof(T), CHUNKS = P::DP / E, LANES = CHUNKS < 32 ? CHUNKS : 32, RPI = 32 / LANES, CPL = CHUNKS / LANES;
+    const char *const k0 = static_cast<const char *>(a.k) + lane % LANES * 16, *const v0 = static_cast<const char *>(a.v) + lane % LANES * 16;
     auto issue = [&](const Row &r, int slot) {
       const bool ok = r.valid && r.pg >= 0 && r.pg < a.pages;
       if (r.valid && !ok) odd |= PAGED_PAGE;
       const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << KB) - 1);
       if (lane == 0) masks[warp][slot] = mask;
-      const long long ko = ok ? r.pg * a.ks[0] + r.kh * a.ks[1] + r.row * a.ks[2] : 0, vo = ok ? r.pg * a.vs[0] + r.kh * a.vs[1] + r.row * a.vs[2] : 0;
-      const uint32_t dst = ring + slot * C::STAGE;
+      const uint32_t ko = ok ? r.pg * s.ku[0] + r.kh * s.ku[1] + r.row * s.ku[2] : 0;
+      const uint32_t dst = ring_at + slot * C::STAGE;
+      if (mask == (1u << KB) - 1 && s.alike) {
 #pragma unroll
-      for (int i = 0; i < KB / RPI; i++) {
-        const int row = i * RPI + lane / LANES;
-        const T *kp = static_cast<const T *>(a.k) + __shfl_sync(0xffffffffu, ko, row), *vp = static_cast<const T *>(a.v) + __shfl_sync(0xffffffffu, vo, row);
-        const uint32_t n = mask >> row & 1 ? 16 : 0;
+        for (int i = 0; i < KB / RPI; i++) {
+          const int row = i * RPI + lane / LANES;
+          const uint32_t off = __shfl_sync(0xffffffffu, ko, row);
+          const char *kp = k0 + (unsigned long long)off * s.unit, *vp = v0 + (unsigned long long)off * s.unit;
 #pragma unroll
-        for (int x = 0; x < CPL; x++) {
-          const int c = lane % LANES + 32 * x;
-          if (c * E < a.D) {
-            const uint32_t to = dst + row * ROWB + ((c ^ spread(row)) << 4);
-            cp_async16_part(to, kp + c * E, n);
-            cp_async16_part(to + KB * ROWB, vp + c * E, n);
+          for (int x = 0; x < CPL; x++) {
+            const int c = lane % LANES + 32 * x;
+            if (c * E < a.D) {
+              const uint32_t to = dst + row * ROWB + ((c ^ spread(row)) << 4);
+              cp_async16(to, kp + x * 512);
+              cp_async16(to + KB * ROWB, vp + x * 512);
+            }
+          }
+        }
+      } else {
+        const uint32_t vo = ok ? r.pg * s.vu[0] + r.kh * s.vu[1] + r.row * s.vu[2] : 0;
+#pragma unroll 1
+        for (int i = 0; i < KB / RPI; i++) {
+          const int row = i * RPI + lane / LANES;
+          const uint32_t n = mask >> row & 1 ? 16 : 0;
+          const char *kp = k0 + (unsigned long long)__shfl_sync(0xffffffffu, ko, row) * s.unit, *vp = v0 + (unsigned long long)__shfl_sync(0xffffffffu, vo, row) * s.unit;
+          for (int x = 0; x < CPL; x++) {
+            const int c = lane % LANES + 32 * x;
+            if (c * E < a.D) {
+              const uint32_t to = dst + row * ROWB + ((c ^ spread(row)) << 4);
+              cp_async16_part(to, kp + x * 512, n);
+              cp_async16_part(to + KB * ROWB, vp + x * 512, n);
+            }
           }
         }
       }
@@ -550,7 +680,7 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
 #pragma unroll
       for (int i = 0; i < S - 1; i++)
         if (i < steps) {
-          if (i) far.next<TILE>(a, units);
+          if (i) far.next<KB>(a, units, hop);
           first[i] = peek();
         }
 #pragma unroll
@@ -558,64 +688,95 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
         if (i < steps) issue(first[i], i);
         cp_async_commit();
       }
-      if (S - 1 < steps) far.next<TILE>(a, units), next = peek();
+      if (S - 1 < steps) far.next<KB>(a, units, hop), next = peek();
     }
 
     const Scorer score(a.scale, a.softcap);
     P state;
     bool fresh = true, begins = false;
-    long long unit0 = 0;  // the unit's first tile among all
+    long long begun = unit0[inside ? 0 : warp];  // where the unit begins in cost
     int slot = 0, fill = S - 1;
     for (int step = 0; step < steps; step++) {
       cp_async_wait<S - 2>();
       __syncwarp();  // the block is there for all lanes, and all are done with the one before
       if (step + S - 1 < steps) {
         issue(next, fill);
-        if (step + S < steps) far.next<TILE>(a, units), next = peek();
+        if (step + S < steps) far.next<KB>(a, units, hop), next = peek();
       }
       cp_async_commit();
       const int kh = now.u / s.groups, h0 = (now.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
-      if (fresh) {
-        begins = now.tile == 0, unit0 = t0 + step - now.tile, fresh = false;
-        state.begin(s, now.b, kh, h0, count, extra, warp);
-      }
-      state.block(a, score, ring + slot * C::STAGE, masks[warp][slot], extra, warp);
+      if (fresh) begins = now.block == 0, fresh = false, state.begin(s, now.b, kh, h0, count, extra);
+      state.block(score, ring_at + slot * C::STAGE, masks[warp][slot], extra);
       slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
-      const bool ends = now.tile + 1 == now.tiles;
+      // (inside one unit its end belongs to the last warp's piece, whoever has the last block)
+      const bool ends = inside ? step + 1 == steps && warp == min(PA_WARPS, all) - 1 && from[0].z + all == now.blocks : now.block + 1 == now.blocks;
       if (ends || step + 1 == steps) {
-        // ---- the warps' parts of the unit
-        state.store(part + warp * P::HEADS * P::PR, a.D);
-        __syncthreads();
-        const bool whole = begins && ends;
-        const int place = 2 * cta + (begins ? 1 : 0);
-        for (int h = warp; h < count; h += PA_WARPS) {
-          const float *row = part + h * P::PR;
-          float top = -INFINITY, L = 0.f, e[PA_WARPS];
-#pragma unroll
-          for (int w = 0; w < PA_WARPS; w++) top = fmaxf(top, row[w * P::HEADS * P::PR]);
-          const float use = top == -INFINITY ? 0.f : top;
-#pragma unroll
-          for (int w = 0; w < PA_WARPS; w++) e[w] = exp2f(row[w * P::HEADS * P::PR] - use), L = fmaf(e[w], row[w * P::HEADS * P::PR + 1], L);
-          const long long at = (long long)place * P::HEADS + h;
-          if (!whole && lane == 0) s.ml[2 * at] = top, s.ml[2 * at + 1] = L;
-          for (int d = lane; d < a.D; d += 32) {
-            float A = 0.f;
-#pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) A = fmaf(e[w], row[w * P::HEADS * P::PR + 4 + d], A);
-            if (whole) static_cast<T *>(a.out)[((long long)now.b * a.NH + kh * a.G + h0 + h) * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
-            else s.acc[at * a.D + d] = A;
-          }
+        if (begins && ends && !inside) {
+          state.write(static_cast<T *>(a.out) + ((long long)now.b * a.NH + kh * a.G + h0) * a.D, count, a.D, extra);
+        } else if (begins) {  // (the run's end: its ring is free once the last copies have landed)
+          cp_async_wait<0>();
+          __syncwarp();
+          state.store(reinterpret_cast<float *>(ring), a.D);
+          if (lane == 0) open1[warp] = ends ? 1 : 2, piece1[warp] = make_int4(now.b, now.u, now.blocks, 0), cost1[warp] = begun;
+        } else {
+          state.store(part, a.D);
+          if (lane == 0) open0[warp] = ends ? 1 : 2, piece0[warp] = make_int4(now.b, now.u, now.blocks, 0);
         }
-        if (begins && !ends) head = make_int4(now.b, now.u, (int)(((unit0 + now.tiles) * dealt - 1) / total) - cta + 1, 0);
-        __syncthreads();  // part is free again
-        fresh = true;
+        fresh = true, begun += now.blocks + UNIT;
       }
-      if (step + 1 < steps) now.next<TILE>(a, units);
+      if (step + 1 < steps) now.next<KB>(a, units, hop);
     }
     cp_async_wait<0>();
   }
-  if (s.heads && tid == 0) s.heads[cta] = head;
   if (odd) atomicOr(&g_attn_status, odd);
+  __syncthreads();
+
+  // ---- the CTA's pieces: a run's first belongs to a unit begun before it, its last to one that goes on in the next warp's first
+  int4 head = make_int4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int p = 0; p < 2 * PA_WARPS;) {  // piece p: of warp p / 2, the one begun before its run or (late) the one that goes on
+    const int w0 = p >> 1;
+    const bool late = p & 1;
+    if (!(late ? open1[w0] : open0[w0])) {
+      p++;
+      continue;
+    }
+    int w1 = w0;
+    bool goes_on = (late ? open1[w0] : open0[w0]) == 2;
+    while (goes_on && w1 + 1 < PA_WARPS && open0[w1 + 1]) goes_on = open0[++w1] == 2;
+    const int4 who = late ? piece1[w0] : piece0[w0];
+    const int kh = who.y / s.groups, h0 = (who.y - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
+    const bool whole = late && !goes_on;
+    const float *const row0 = reinterpret_cast<const float *>(late ? smem + w0 * C::RING : smem + PA_WARPS * C::RING + w0 * C::PART);
+    auto row = [&](int i, int h) { return (i == 0 ? row0 : reinterpret_cast<const float *>(smem + PA_WARPS * C::RING + (w0 + i) * C::PART)) + h * P::PR; };
+    for (int h = warp; h < count; h += PA_WARPS) {
+      float top = -INFINITY, L = 0.f, e[PA_WARPS];
+#pragma unroll
+      for (int i = 0; i < PA_WARPS; i++)
+        if (i <= w1 - w0) top = fmaxf(top, row(i, h)[0]);
+      const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < PA_WARPS; i++)
+        if (i <= w1 - w0) e[i] = ex2(row(i, h)[0] - use), L = fmaf(e[i], row(i, h)[1], L);
+      const long long at = (2ll * cta + late) * P::HEADS + h;
+      if (!whole && lane == 0) s.ml[2 * at] = top, s.ml[2 * at + 1] = L;
+      for (int d = lane; d < a.D; d += 32) {
+        float A = 0.f;
+#pragma unroll
+        for (int i = 0; i < PA_WARPS; i++)
+          if (i <= w1 - w0) A = fmaf(e[i], row(i, h)[4 + d], A);
+        if (whole) static_cast<T *>(a.out)[((long long)who.x * a.NH + kh * a.G + h0 + h) * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
+        else s.acc[at * a.D + d] = A;
+      }
+    }
+    if (late && goes_on) {  // the run that has its last block, and so the CTAs that it goes over
+      const long long x = cost1[w0] + UNIT + who.z - 1, wide = rest * (quota + 1);
+      const long long run = x < wide ? x / (quota + 1) : rest + (x - wide) / quota;
+      head = make_int4(who.x, who.y, (int)(run / PA_WARPS) - cta + 1, 0);
+    }
+    p = w1 > w0 ? 2 * w1 + 1 : p + 1;
+  }
+  if (s.heads && tid == 0) s.heads[cta] = head;
 }
 
 // The pieces of a unit that was cut, in order: piece 0 is the second of the CTA where it begins, piece i the first of the i-th CTA after it.
@@ -644,7 +805,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(SplitArgs s, 
   if (top == -INFINITY) top = 0.f;
   float L = 0.f;
   for (int i = threadIdx.x; i < n; i += PJ_WARPS * 32) {
-    const float e = exp2f(s.ml[2 * place(i)] - top);
+    const float e = ex2(s.ml[2 * place(i)] - top);
     weight[i] = e, L = fmaf(e, s.ml[2 * place(i) + 1], L);
   }
   L = warp_sum(L);
@@ -687,27 +848,40 @@ struct Cut {
   bool streamed;       // the kernel above, else the one for any stride
   int hpg, groups, DP, HEADS, ctas;
   bool joined;
+  uint32_t unit;
   size_t ml_at, acc_at, bytes;
 };
 
 Cut cut_of(const lb200_paged_attn_args *p) {
   Cut c{};
   const int size = p->dtype == LB200_F32 ? 4 : 2, G = p->NH / p->KH;
-  uint64_t off = (uint64_t)(uintptr_t)p->q | (uint64_t)(uintptr_t)p->k | (uint64_t)(uintptr_t)p->v;
+  uint64_t off = (uint64_t)(uintptr_t)p->q | (uint64_t)(uintptr_t)p->k | (uint64_t)(uintptr_t)p->v | (uint64_t)(uintptr_t)p->out;
   const long long nq[2] = {p->B, p->NH}, nk[3] = {p->pages, p->KH, p->page_size};
   for (int i = 0; i < 2; i++) off |= nq[i] > 1 ? (uint64_t)p->q_stride[i] * size : 0;  // (the stride of an extent of one moves nothing)
   for (int i = 0; i < 3; i++) off |= nk[i] > 1 ? (uint64_t)p->k_stride[i] * size | (uint64_t)p->v_stride[i] * size : 0;
-  c.streamed = p->D % 16 == 0 && !(off & 15);
+  // a row's offset in the largest unit that divides all strides has to fit 32 bits: with rows of 32 bytes or more, 128 GB
+  uint64_t all = 0, far[2] = {0, 0};
+  for (int i = 0; i < 3; i++)
+    if (nk[i] > 1) {
+      all |= (uint64_t)p->k_stride[i] * size | (uint64_t)p->v_stride[i] * size;
+      far[0] += (uint64_t)(nk[i] - 1) * (uint64_t)p->k_stride[i] * size, far[1] += (uint64_t)(nk[i] - 1) * (uint64_t)p->v_stride[i] * size;
+      if (p->k_stride[i] < 0 || p->v_stride[i] < 0) off |= 1;
+    }
+  c.unit = 16;
+  while (c.unit < 4096 && !(all & c.unit)) c.unit *= 2;
+  c.streamed = p->D % 16 == 0 && !(off & 15) && (far[0] > far[1] ? far[0] : far[1]) / c.unit <= 0xffffffffull;
   if (!c.streamed) return c;
-  c.groups = (G + 15) / 16, c.hpg = (G + c.groups - 1) / c.groups, c.groups = (G + c.hpg - 1) / c.hpg;
   c.DP = p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256;
-  c.HEADS = p->dtype == LB200_F32 ? (c.hpg <= 1 ? 1 : c.hpg <= 2 ? 2 : c.hpg <= 4 ? 4 : c.hpg <= 8 ? 8 : 16) : (c.hpg <= 8 ? 8 : 16);
-  const int tile = PA_WARPS * (p->dtype == LB200_F32 ? 8 : 16), per_sm = c.DP == 64 ? 3 : c.DP == 128 ? 2 : 1;
+  const int most = size == 4 && c.DP == 256 ? 8 : 16;  // heads per unit: what shared memory and registers hold
+  c.groups = (G + most - 1) / most, c.hpg = (G + c.groups - 1) / c.groups, c.groups = (G + c.hpg - 1) / c.hpg;
+  c.HEADS = size == 4 ? (c.hpg <= 1 ? 1 : c.hpg <= 2 ? 2 : c.hpg <= 4 ? 4 : c.hpg <= 8 ? 8 : 16) : (c.hpg <= 8 ? 8 : 16);
   long long keys = (long long)p->W * p->page_size;
   if (p->window > 0 && p->window < keys) keys = p->window;
-  const long long tiles = (keys + tile - 1) / tile, all = tiles * p->KH * c.groups, slots = (long long)per_sm * sm_count();
-  c.ctas = (int)(all >= slots || all * p->B >= slots ? (slots < PJ_MAX ? slots : PJ_MAX) : all * p->B);
-  c.joined = tiles > 1;
+  const long long blocks = (keys + (size == 4 ? 7 : 15)) / (size == 4 ? 8 : 16), slots = (long long)split_ctas(size, c.DP, c.HEADS) * sm_count();
+  const double most_work = (double)p->B * p->KH * c.groups * (double)(blocks + UNIT) / PA_WARPS;  // CTAs' worth, were every sequence as long as the table
+  c.ctas = (int)(slots < PJ_MAX ? slots : PJ_MAX);
+  if (most_work < c.ctas) c.ctas = most_work < 1 ? 1 : (int)most_work;
+  c.joined = blocks > 1 && c.ctas > 1;
   if (c.joined) {
     c.ml_at = ((size_t)c.ctas * sizeof(int4) + 255) & ~(size_t)255;
     c.acc_at = (c.ml_at + (size_t)c.ctas * 2 * c.HEADS * 2 * 4 + 255) & ~(size_t)255;
@@ -746,8 +920,10 @@ int launch_dtype(const SplitArgs &s, const Cut &c, int dtype, cudaStream_t st) {
     case 2: return launch_split<F32Block<DP, 2>>(s, c, st);
     case 4: return launch_split<F32Block<DP, 4>>(s, c, st);
     case 8: return launch_split<F32Block<DP, 8>>(s, c, st);
-    default: return launch_split<F32Block<DP, 16>>(s, c, st);
   }
+  if constexpr (DP < 256) return launch_split<F32Block<DP, 16>>(s, c, st);
+  return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: %d heads per unit", c.HEADS);
+
 }
 
 }  // namespace
@@ -784,7 +960,13 @@ int paged_decode_attn(const lb200_paged_attn_args *p, cudaStream_t st) {
       return fail(p->scratch ? LB200_E_SHAPE : LB200_E_NULL, "light_b200: paged_decode_attn: %llu bytes of scratch, want %llu, 256-byte aligned", p->scratch_bytes,
                   (unsigned long long)c.bytes);
     SplitArgs s{};
-    s.p = a, s.hpg = c.hpg, s.groups = c.groups;
+    s.p = a, s.hpg = c.hpg, s.groups = c.groups, s.unit = c.unit, s.alike = true;
+    const long long nk[3] = {p->pages, p->KH, p->page_size};
+    const int size = p->dtype == LB200_F32 ? 4 : 2;
+    for (int i = 0; i < 3; i++) {
+      s.ku[i] = nk[i] > 1 ? (uint32_t)((uint64_t)p->k_stride[i] * size / c.unit) : 0, s.vu[i] = nk[i] > 1 ? (uint32_t)((uint64_t)p->v_stride[i] * size / c.unit) : 0;
+      s.alike = s.alike && s.ku[i] == s.vu[i];
+    }
     if (c.joined) {
       s.heads = static_cast<int4 *>(p->scratch);
       s.ml = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + c.ml_at), s.acc = reinterpret_cast<float *>(static_cast<char *>(p->scratch) + c.acc_at);
