@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 //     without a key are filled with zeros: a weight of 0 times what lies there must not be NaN.
 //   * Pieces of a unit that was cut are joined in their order, first those of a CTA's warps at its end, in shared memory; what goes on
 //     over CTAs goes to scratch, at most two pieces a CTA, and a second launch joins those: no atomics, the same bits every time.
-constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3;
+constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 8;
 
 struct SplitArgs {
   PagedArgs p;
@@ -523,11 +523,108 @@ struct Cursor {
   }
 };
 
+// What a warp's copies take: the page of its lane's key, then a block of rows into a slot of its ring.
+struct Row {
+  int pg, row, kh;
+  bool valid;
+};
+
+template <typename P>
+struct Feeder {
+  using C = SplitCfg<P>;
+  using T = typename P::T;
+  static constexpr int E = 16 / (int)sizeof(T), CHUNKS = P::DP / E, LANES = CHUNKS < 32 ? CHUNKS : 32, RPI = 32 / LANES, CPL = CHUNKS / LANES;
+  const SplitArgs &s;
+  uint32_t *masks;   // [S]: the keys of each slot's block that there are
+  uint32_t ring;
+  const char *k0, *v0;
+  unsigned odd = 0;
+
+  __device__ __forceinline__ Feeder(const SplitArgs &s_, unsigned char *ring_, uint32_t *masks_) : s(s_), masks(masks_), ring(umma::smem_u32(ring_)) {
+    const int lane = threadIdx.x & 31;
+    k0 = static_cast<const char *>(s.p.k) + lane % LANES * 16, v0 = static_cast<const char *>(s.p.v) + lane % LANES * 16;
+    if (s.p.D < P::DP) {  // chunks past the head: nothing is copied there, and the products run over them
+      for (int i = lane; i < C::RING / 16; i += 32) reinterpret_cast<uint4 *>(ring_)[i] = make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
+    }
+  }
+  __device__ __forceinline__ Row peek(const Cursor &c) const {  // (lanes from KB on repeat)
+    const PagedArgs &a = s.p;
+    Row r;
+    const int j = c.j0 + c.block * P::KB + (threadIdx.x & (P::KB - 1)), w = a.page.div(j);
+    r.valid = j < c.n, r.row = j - w * a.page.d, r.kh = c.u / s.groups;
+    r.pg = r.valid ? a.table[c.b * a.table_stride + w] : -1;
+    return r;
+  }
+  __device__ __forceinline__ void issue(const Row &r, int slot) {
+    const PagedArgs &a = s.p;
+    constexpr int KB = P::KB;
+    const int lane = threadIdx.x & 31;
+    const bool ok = r.valid && r.pg >= 0 && r.pg < a.pages;
+    if (r.valid && !ok) odd |= PAGED_PAGE;
+    const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << KB) - 1);
+    if (lane == 0) masks[slot] = mask;
+    const uint32_t ko = ok ? r.pg * s.ku[0] + r.kh * s.ku[1] + r.row * s.ku[2] : 0;
+    const uint32_t dst = ring + slot * C::STAGE;
+    if (mask == (1u << KB) - 1 && s.alike) {
+#pragma unroll
+      for (int i = 0; i < KB / RPI; i++) {
+        const int row = i * RPI + lane / LANES;
+        const uint32_t off = __shfl_sync(0xffffffffu, ko, row);
+        const char *kp = k0 + (unsigned long long)off * s.unit, *vp = v0 + (unsigned long long)off * s.unit;
+#pragma unroll
+        for (int x = 0; x < CPL; x++) {
+          const int c = lane % LANES + 32 * x;
+          if (c * E < a.D) {
+            const uint32_t to = dst + row * P::ROWB + ((c ^ spread(row)) << 4);
+            cp_async16(to, kp + x * 512);
+            cp_async16(to + KB * P::ROWB, vp + x * 512);
+          }
+        }
+      }
+    } else {
+      const uint32_t vo = ok ? r.pg * s.vu[0] + r.kh * s.vu[1] + r.row * s.vu[2] : 0;
+#pragma unroll 1
+      for (int i = 0; i < KB / RPI; i++) {
+        const int row = i * RPI + lane / LANES;
+        const uint32_t n = mask >> row & 1 ? 16 : 0;
+        const char *kp = k0 + (unsigned long long)__shfl_sync(0xffffffffu, ko, row) * s.unit, *vp = v0 + (unsigned long long)__shfl_sync(0xffffffffu, vo, row) * s.unit;
+        for (int x = 0; x < CPL; x++) {
+          const int c = lane % LANES + 32 * x;
+          if (c * E < a.D) {
+            const uint32_t to = dst + row * P::ROWB + ((c ^ spread(row)) << 4);
+            cp_async16_part(to, kp + x * 512, n);
+            cp_async16_part(to + KB * P::ROWB, vp + x * 512, n);
+          }
+        }
+      }
+    }
+  }
+  // the first S - 1 of `steps` blocks on their way, and the next one's page
+  __device__ __forceinline__ Row fill(Cursor &far, int units, int hop, int steps) {
+    constexpr int S = C::S;
+    Row first[S - 1], next;
+#pragma unroll
+    for (int i = 0; i < S - 1; i++)
+      if (i < steps) {
+        if (i) far.next<P::KB>(s.p, units, hop);
+        first[i] = peek(far);
+      }
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) {
+      if (i < steps) issue(first[i], i);
+      cp_async_commit();
+    }
+    if (S - 1 < steps) far.next<P::KB>(s.p, units, hop), next = peek(far);
+    return next;
+  }
+};
+
 template <typename P>
 __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kernel(SplitArgs s) {
   using C = SplitCfg<P>;
   using T = typename P::T;
-  constexpr int KB = P::KB, S = C::S, ROWB = P::ROWB;
+  constexpr int KB = P::KB, S = C::S;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ longlong2 scan[PA_WARPS];
   __shared__ int4 from[PA_WARPS + 1];              // where the warps' runs begin: sequence, unit, block
@@ -612,101 +709,24 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
     now.at<KB>(a, at.x);
     now.u = at.y, now.block = at.z + (inside ? warp : 0);
     far = now;
-    const uint32_t ring_at = umma::smem_u32(ring);
-    if (a.D < P::DP) {  // chunks past the head: nothing is copied there, and the products run over them
-      for (int i = lane; i < C::RING / 16; i += 32) reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
-      __syncwarp();
-    }
-
-    struct Row {
-      int pg, row, kh;
-      bool valid;
-    };
-    auto peek = [&]() {  // the page of this lane's key of the block at `far` (lanes from KB on repeat)
-      Row r;
-      const int j = far.j0 + far.block * KB + (lane & (KB - 1));
-      const int w = a.page.div(j);
-      r.valid = j < far.n, r.row = j - w * a.page.d, r.kh = far.u / s.groups;
-      r.pg = r.valid ? a.table[far.b * a.table_stride + w] : -1;
-      return r;
-    };
-    constexpr int E = 16 / (int)sizeof(T), CHUNKS = P::DP / E, LANES = CHUNKS < 32 ? CHUNKS : 32, RPI = 32 / LANES, CPL = CHUNKS / LANES;
-    const char *const k0 = static_cast<const char *>(a.k) + lane % LANES * 16, *const v0 = static_cast<const char *>(a.v) + lane % LANES * 16;
-    auto issue = [&](const Row &r, int slot) {
-      const bool ok = r.valid && r.pg >= 0 && r.pg < a.pages;
-      if (r.valid && !ok) odd |= PAGED_PAGE;
-      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << KB) - 1);
-      if (lane == 0) masks[warp][slot] = mask;
-      const uint32_t ko = ok ? r.pg * s.ku[0] + r.kh * s.ku[1] + r.row * s.ku[2] : 0;
-      const uint32_t dst = ring_at + slot * C::STAGE;
-      if (mask == (1u << KB) - 1 && s.alike) {
-#pragma unroll
-        for (int i = 0; i < KB / RPI; i++) {
-          const int row = i * RPI + lane / LANES;
-          const uint32_t off = __shfl_sync(0xffffffffu, ko, row);
-          const char *kp = k0 + (unsigned long long)off * s.unit, *vp = v0 + (unsigned long long)off * s.unit;
-#pragma unroll
-          for (int x = 0; x < CPL; x++) {
-            const int c = lane % LANES + 32 * x;
-            if (c * E < a.D) {
-              const uint32_t to = dst + row * ROWB + ((c ^ spread(row)) << 4);
-              cp_async16(to, kp + x * 512);
-              cp_async16(to + KB * ROWB, vp + x * 512);
-            }
-          }
-        }
-      } else {
-        const uint32_t vo = ok ? r.pg * s.vu[0] + r.kh * s.vu[1] + r.row * s.vu[2] : 0;
-#pragma unroll 1
-        for (int i = 0; i < KB / RPI; i++) {
-          const int row = i * RPI + lane / LANES;
-          const uint32_t n = mask >> row & 1 ? 16 : 0;
-          const char *kp = k0 + (unsigned long long)__shfl_sync(0xffffffffu, ko, row) * s.unit, *vp = v0 + (unsigned long long)__shfl_sync(0xffffffffu, vo, row) * s.unit;
-          for (int x = 0; x < CPL; x++) {
-            const int c = lane % LANES + 32 * x;
-            if (c * E < a.D) {
-              const uint32_t to = dst + row * ROWB + ((c ^ spread(row)) << 4);
-              cp_async16_part(to, kp + x * 512, n);
-              cp_async16_part(to + KB * ROWB, vp + x * 512, n);
-            }
-          }
-        }
-      }
-    };
-
-    Row next;
-    {
-      Row first[S - 1];
-#pragma unroll
-      for (int i = 0; i < S - 1; i++)
-        if (i < steps) {
-          if (i) far.next<KB>(a, units, hop);
-          first[i] = peek();
-        }
-#pragma unroll
-      for (int i = 0; i < S - 1; i++) {
-        if (i < steps) issue(first[i], i);
-        cp_async_commit();
-      }
-      if (S - 1 < steps) far.next<KB>(a, units, hop), next = peek();
-    }
-
+    Feeder<P> feed(s, ring, masks[warp]);
+    Row next = feed.fill(far, units, hop, steps);
     const Scorer score(a.scale, a.softcap);
     P state;
     bool fresh = true, begins = false;
     long long begun = unit0[inside ? 0 : warp];  // where the unit begins in cost
     int slot = 0, fill = S - 1;
     for (int step = 0; step < steps; step++) {
+      const int kh = now.u / s.groups, h0 = (now.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
+      if (fresh) begins = now.block == 0, fresh = false, state.begin(s, now.b, kh, h0, count, extra);
       cp_async_wait<S - 2>();
       __syncwarp();  // the block is there for all lanes, and all are done with the one before
       if (step + S - 1 < steps) {
-        issue(next, fill);
-        if (step + S < steps) far.next<KB>(a, units, hop), next = peek();
+        feed.issue(next, fill);
+        if (step + S < steps) far.next<KB>(a, units, hop), next = feed.peek(far);
       }
       cp_async_commit();
-      const int kh = now.u / s.groups, h0 = (now.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
-      if (fresh) begins = now.block == 0, fresh = false, state.begin(s, now.b, kh, h0, count, extra);
-      state.block(score, ring_at + slot * C::STAGE, masks[warp][slot], extra);
+      state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
       slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
       // (inside one unit its end belongs to the last warp's piece, whoever has the last block)
       const bool ends = inside ? step + 1 == steps && warp == min(PA_WARPS, all) - 1 && from[0].z + all == now.blocks : now.block + 1 == now.blocks;
@@ -727,6 +747,7 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
       if (step + 1 < steps) now.next<KB>(a, units, hop);
     }
     cp_async_wait<0>();
+    odd |= feed.odd;
   }
   if (odd) atomicOr(&g_attn_status, odd);
   __syncthreads();
@@ -777,6 +798,100 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
     p = w1 > w0 ? 2 * w1 + 1 : p + 1;
   }
   if (s.heads && tid == 0) s.heads[cta] = head;
+}
+
+// Few units of few blocks: a cluster of up to eight CTAs takes a unit, its warps the blocks in turn, and the parts meet in the CTAs' shared memory:
+// one launch, no scratch, no schedule to work out, which is what counts when there is little to read.
+template <typename P>
+__global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_cluster_kernel(SplitArgs s, int ks) {
+  using C = SplitCfg<P>;
+  using T = typename P::T;
+  constexpr int KB = P::KB, S = C::S;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint32_t masks[PA_WARPS][S];
+  pdl_launch_dependents();
+  pdl_wait();
+  const PagedArgs &a = s.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, units = a.KH * s.groups, rank = blockIdx.x % ks, b = blockIdx.x / ks / units;
+  Cursor far;
+  far.at<KB>(a, b);
+  far.u = blockIdx.x / ks - b * units, far.block = rank * PA_WARPS + warp;
+  const int hop = ks * PA_WARPS, blocks = far.blocks, steps = (blocks - far.block + hop - 1) / hop;  // (rounds to 0 from below)
+  const int kh = far.u / s.groups, h0 = (far.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
+  T *const out = static_cast<T *>(a.out) + ((long long)b * a.NH + kh * a.G + h0) * a.D;
+  if (tid == 0 && rank == 0 && far.u == 0 && a.lens[b] != far.n) atomicOr(&g_attn_status, (unsigned)PAGED_LENGTH);
+  if (blocks == 0) {  // (the whole cluster)
+    for (int i = rank * PA_THREADS + tid; i < count * a.D; i += ks * PA_THREADS) out[i] = from_f32<T>(0.f);
+    return;
+  }
+  unsigned char *const ring = smem + warp * C::RING, *const extra = smem + PA_WARPS * (C::RING + C::PART) + warp * P::EXTRA;
+  float *const part = reinterpret_cast<float *>(smem + PA_WARPS * C::RING + warp * C::PART);
+  P state;
+  {
+    Feeder<P> feed(s, ring, masks[warp]);
+    Row next = feed.fill(far, units, hop, steps);
+    state.begin(s, b, kh, h0, count, extra);
+    const Scorer score(a.scale, a.softcap);
+    int slot = 0, fill = S - 1;
+    for (int step = 0; step < steps; step++) {
+      cp_async_wait<S - 2>();
+      __syncwarp();
+      if (step + S - 1 < steps) {
+        feed.issue(next, fill);
+        if (step + S < steps) far.next<KB>(a, units, hop), next = feed.peek(far);
+      }
+      cp_async_commit();
+      state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
+      slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
+    }
+    cp_async_wait<0>();
+    if (feed.odd) atomicOr(&g_attn_status, feed.odd);
+  }
+  state.store(part, a.D);
+  __syncthreads();
+  const float *const parts = reinterpret_cast<const float *>(smem + PA_WARPS * C::RING);
+  float *const mine = reinterpret_cast<float *>(smem);  // [HEADS][PR] of this CTA, over its drained rings
+  for (int h = warp; h < count; h += PA_WARPS) {
+    const float *row = parts + h * P::PR;
+    float top = -INFINITY, L = 0.f, e[PA_WARPS];
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++) top = fmaxf(top, row[w * P::HEADS * P::PR]);
+    const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++) e[w] = ex2(row[w * P::HEADS * P::PR] - use), L = fmaf(e[w], row[w * P::HEADS * P::PR + 1], L);
+    if (ks > 1 && lane == 0) mine[h * P::PR] = top, mine[h * P::PR + 1] = L;
+    for (int d = lane; d < a.D; d += 32) {
+      float A = 0.f;
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; w++) A = fmaf(e[w], row[w * P::HEADS * P::PR + 4 + d], A);
+      if (ks > 1) mine[h * P::PR + 4 + d] = A;
+      else out[h * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
+    }
+  }
+  if (ks == 1) return;
+  umma::cluster_sync();
+  const int all = count * a.D, lo = all * rank / ks, hi = all * (rank + 1) / ks;
+  const uint32_t base = umma::smem_u32(mine);
+  for (int i = lo + tid; i < hi; i += PA_THREADS) {
+    const int h = i / a.D, d = i - h * a.D;
+    float m[8], l[8], v[8], top = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; r++) {  // all remote loads at once
+      const uint32_t row = umma::map_to_rank(base, (uint32_t)(r < ks ? r : 0)) + (uint32_t)(h * P::PR) * 4u;
+      m[r] = r < ks ? umma::ld_cluster_f32(row) : -INFINITY, l[r] = umma::ld_cluster_f32(row + 4u), v[r] = umma::ld_cluster_f32(row + 16u + (uint32_t)d * 4u);
+    }
+#pragma unroll
+    for (int r = 0; r < 8; r++) top = fmaxf(top, m[r]);
+    if (top == -INFINITY) top = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; r++)
+      if (r < ks) {
+        const float e = ex2(m[r] - top);
+        L = fmaf(e, l[r], L), A = fmaf(e, v[r], A);
+      }
+    out[i] = from_f32<T>(L == 0.f ? 0.f : A / L);
+  }
+  umma::cluster_sync();  // nobody leaves while a peer still reads its part
 }
 
 // The pieces of a unit that was cut, in order: piece 0 is the second of the CTA where it begins, piece i the first of the i-th CTA after it.
@@ -847,6 +962,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(SplitArgs s, 
 struct Cut {
   bool streamed;       // the kernel above, else the one for any stride
   int hpg, groups, DP, HEADS, ctas;
+  int ks;              // CTAs of a cluster that takes a unit; 0: the split kernel
   bool joined;
   uint32_t unit;
   size_t ml_at, acc_at, bytes;
@@ -878,6 +994,10 @@ Cut cut_of(const lb200_paged_attn_args *p) {
   long long keys = (long long)p->W * p->page_size;
   if (p->window > 0 && p->window < keys) keys = p->window;
   const long long blocks = (keys + (size == 4 ? 7 : 15)) / (size == 4 ? 8 : 16), slots = (long long)split_ctas(size, c.DP, c.HEADS) * sm_count();
+  const long long n_units = (long long)p->B * p->KH * c.groups;
+  for (c.ks = 1; c.ks < 8 && n_units * (c.ks + 1) <= slots && blocks > c.ks * PA_WARPS;) c.ks++;
+  if (n_units * c.ks <= slots && blocks <= (long long)c.ks * PA_WARPS * CLUSTER_BLOCKS) return c;
+  c.ks = 0;
   const double most_work = (double)p->B * p->KH * c.groups * (double)(blocks + UNIT) / PA_WARPS;  // CTAs' worth, were every sequence as long as the table
   c.ctas = (int)(slots < PJ_MAX ? slots : PJ_MAX);
   if (most_work < c.ctas) c.ctas = most_work < 1 ? 1 : (int)most_work;
@@ -891,7 +1011,27 @@ Cut cut_of(const lb200_paged_attn_args *p) {
 }
 
 template <typename P>
+int launch_cluster(const SplitArgs &s, const Cut &c, cudaStream_t st) {
+  auto kern = paged_attn_cluster_kernel<P>;
+  static DeviceOnce once;
+  cudaError_t e = once.ensure([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<P>::SMEM); });
+  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(s.p.B * s.p.KH * s.groups * c.ks)), cfg.blockDim = dim3(PA_THREADS), cfg.dynamicSmemBytes = SplitCfg<P>::SMEM, cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)c.ks, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = c.ks > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, s, c.ks);
+  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
+  return launched("paged_decode_attn");
+}
+
+template <typename P>
 int launch_split(const SplitArgs &s, const Cut &c, cudaStream_t st) {
+  if (c.ks) return launch_cluster<P>(s, c, st);
   auto kern = paged_attn_kernel<P>;
   static DeviceOnce once;
   cudaError_t e = once.ensure([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<P>::SMEM); });
