@@ -23,7 +23,7 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
 // n / d for 0 <= n < 2^31: n m >> (31 + s) with 2^s >= d and m = ceil(2^(31 + s) / d).  m d exceeds 2^(31 + s) by less than d <= 2^s, so the
-// product's excess stays under 2^(31 + s).
+// product's excess stays under 2^(31 + s).  (2 n has 32 bits: the upper half of 2 n m is n m >> 31.)
 struct FastDiv {
   uint32_t m = 0;
   int s = 0, d = 1;
@@ -32,7 +32,7 @@ struct FastDiv {
     while ((1ll << s) < d) s++;
     m = (uint32_t)(((1ull << (31 + s)) + (unsigned)d - 1) / (unsigned)d);
   }
-  __device__ __forceinline__ int div(int n) const { return (int)(((unsigned long long)(unsigned)n * m) >> (31 + s)); }
+  __device__ __forceinline__ int div(int n) const { return (int)(__umulhi((unsigned)n << 1, m) >> s); }
 };
 
 }  // namespace

@@ -42,10 +42,8 @@ __device__ __forceinline__ float ex2(float x) {  // relative error 2^-22; result
 struct Scorer {
   float sc, cap;  // without a cap: scale log2 e; with one: 2 log2 e scale / cap, and cap log2 e
   __device__ Scorer(float scale, float softcap) : sc(softcap > 0.f ? 2.f * LOG2E * scale / softcap : scale * LOG2E), cap(softcap * LOG2E) {}
-  __device__ __forceinline__ float operator()(float dot) const {
-    const float x = dot * sc;
-    return cap > 0.f ? cap - cap * 2.f * __fdividef(1.f, ex2(x) + 1.f) : x;
-  }
+  __device__ __forceinline__ float operator()(float dot) const { return cap > 0.f ? capped(dot * sc) : dot * sc; }
+  __device__ __forceinline__ float capped(float x) const { return cap - cap * 2.f * __fdividef(1.f, ex2(x) + 1.f); }
 };
 
 // ------------------------------------------------------------------------------------ any head size, any stride
@@ -216,7 +214,11 @@ struct MmaBlock {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = score(s[nt][e] + s2[nt][e]);
+      for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s2[nt][e]) * score.sc;
+      if (score.cap > 0.f) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[nt][e] = score.capped(s[nt][e]);
+      }
       if (valid != 0xFFFFu) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -506,19 +508,22 @@ struct SplitCfg {
 };
 
 struct Cursor {
-  int b, u, block, n, j0, blocks;  // sequence, unit of it, block of that; its length, first key, blocks per unit
+  int b, kh, hg, block, n, j0, blocks;  // sequence, KV head, unit of that, block; the sequence's length, first key, blocks per unit
   template <int KB>
   __device__ __forceinline__ void at(const PagedArgs &a, int b_) {
     b = b_, n = length_of(a, b_), j0 = first_of(a, n), blocks = (n - j0 + KB - 1) / KB;
   }
+  __device__ __forceinline__ void unit(int u, int groups) { kh = u / groups, hg = u - kh * groups; }
   template <int KB>
-  __device__ __forceinline__ void next(const PagedArgs &a, int units, int hop) {  // (there is a next block)
+  __device__ __forceinline__ void next(const SplitArgs &s, int hop) {  // (there is a next block)
     block += hop;
     if (block < blocks) return;
     block = 0;
-    if (++u < units) return;
-    u = 0;
-    do at<KB>(a, b + 1);
+    if (++hg < s.groups) return;
+    hg = 0;
+    if (++kh < s.p.KH) return;
+    kh = 0;
+    do at<KB>(s.p, b + 1);
     while (blocks == 0);
   }
 };
@@ -552,7 +557,7 @@ struct Feeder {
     const PagedArgs &a = s.p;
     Row r;
     const int j = c.j0 + c.block * P::KB + (threadIdx.x & (P::KB - 1)), w = a.page.div(j);
-    r.valid = j < c.n, r.row = j - w * a.page.d, r.kh = c.u / s.groups;
+    r.valid = j < c.n, r.row = j - w * a.page.d, r.kh = c.kh;
     r.pg = r.valid ? a.table[c.b * a.table_stride + w] : -1;
     return r;
   }
@@ -601,13 +606,13 @@ struct Feeder {
     }
   }
   // the first S - 1 of `steps` blocks on their way, and the next one's page
-  __device__ __forceinline__ Row fill(Cursor &far, int units, int hop, int steps) {
+  __device__ __forceinline__ Row fill(Cursor &far, int hop, int steps) {
     constexpr int S = C::S;
     Row first[S - 1], next;
 #pragma unroll
     for (int i = 0; i < S - 1; i++)
       if (i < steps) {
-        if (i) far.next<P::KB>(s.p, units, hop);
+        if (i) far.next<P::KB>(s, hop);
         first[i] = peek(far);
       }
 #pragma unroll
@@ -615,7 +620,7 @@ struct Feeder {
       if (i < steps) issue(first[i], i);
       cp_async_commit();
     }
-    if (S - 1 < steps) far.next<P::KB>(s.p, units, hop), next = peek(far);
+    if (S - 1 < steps) far.next<P::KB>(s, hop), next = peek(far);
     return next;
   }
 };
@@ -707,23 +712,22 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
     Cursor now, far;  // what is folded, and what is fetched
     const int4 at = from[inside ? 0 : warp];
     now.at<KB>(a, at.x);
-    now.u = at.y, now.block = at.z + (inside ? warp : 0);
+    now.unit(at.y, s.groups), now.block = at.z + (inside ? warp : 0);
     far = now;
     Feeder<P> feed(s, ring, masks[warp]);
-    Row next = feed.fill(far, units, hop, steps);
+    Row next = feed.fill(far, hop, steps);
     const Scorer score(a.scale, a.softcap);
     P state;
     bool fresh = true, begins = false;
     long long begun = unit0[inside ? 0 : warp];  // where the unit begins in cost
     int slot = 0, fill = S - 1;
     for (int step = 0; step < steps; step++) {
-      const int kh = now.u / s.groups, h0 = (now.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
-      if (fresh) begins = now.block == 0, fresh = false, state.begin(s, now.b, kh, h0, count, extra);
+      if (fresh) begins = now.block == 0, fresh = false, state.begin(s, now.b, now.kh, now.hg * s.hpg, min(s.hpg, a.G - now.hg * s.hpg), extra);
       cp_async_wait<S - 2>();
       __syncwarp();  // the block is there for all lanes, and all are done with the one before
       if (step + S - 1 < steps) {
         feed.issue(next, fill);
-        if (step + S < steps) far.next<KB>(a, units, hop), next = feed.peek(far);
+        if (step + S < steps) far.next<KB>(s, hop), next = feed.peek(far);
       }
       cp_async_commit();
       state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
@@ -732,19 +736,20 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
       const bool ends = inside ? step + 1 == steps && warp == min(PA_WARPS, all) - 1 && from[0].z + all == now.blocks : now.block + 1 == now.blocks;
       if (ends || step + 1 == steps) {
         if (begins && ends && !inside) {
-          state.write(static_cast<T *>(a.out) + ((long long)now.b * a.NH + kh * a.G + h0) * a.D, count, a.D, extra);
+          const int h0 = now.hg * s.hpg;
+          state.write(static_cast<T *>(a.out) + ((long long)now.b * a.NH + now.kh * a.G + h0) * a.D, min(s.hpg, a.G - h0), a.D, extra);
         } else if (begins) {  // (the run's end: its ring is free once the last copies have landed)
           cp_async_wait<0>();
           __syncwarp();
           state.store(reinterpret_cast<float *>(ring), a.D);
-          if (lane == 0) open1[warp] = ends ? 1 : 2, piece1[warp] = make_int4(now.b, now.u, now.blocks, 0), cost1[warp] = begun;
+          if (lane == 0) open1[warp] = ends ? 1 : 2, piece1[warp] = make_int4(now.b, now.kh * s.groups + now.hg, now.blocks, 0), cost1[warp] = begun;
         } else {
           state.store(part, a.D);
-          if (lane == 0) open0[warp] = ends ? 1 : 2, piece0[warp] = make_int4(now.b, now.u, now.blocks, 0);
+          if (lane == 0) open0[warp] = ends ? 1 : 2, piece0[warp] = make_int4(now.b, now.kh * s.groups + now.hg, now.blocks, 0);
         }
         fresh = true, begun += now.blocks + UNIT;
       }
-      if (step + 1 < steps) now.next<KB>(a, units, hop);
+      if (step + 1 < steps) now.next<KB>(s, hop);
     }
     cp_async_wait<0>();
     odd |= feed.odd;
@@ -815,11 +820,11 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, units = a.KH * s.groups, rank = blockIdx.x % ks, b = blockIdx.x / ks / units;
   Cursor far;
   far.at<KB>(a, b);
-  far.u = blockIdx.x / ks - b * units, far.block = rank * PA_WARPS + warp;
+  far.unit(blockIdx.x / ks - b * units, s.groups), far.block = rank * PA_WARPS + warp;
   const int hop = ks * PA_WARPS, blocks = far.blocks, steps = (blocks - far.block + hop - 1) / hop;  // (rounds to 0 from below)
-  const int kh = far.u / s.groups, h0 = (far.u - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
+  const int kh = far.kh, h0 = far.hg * s.hpg, count = min(s.hpg, a.G - h0);
   T *const out = static_cast<T *>(a.out) + ((long long)b * a.NH + kh * a.G + h0) * a.D;
-  if (tid == 0 && rank == 0 && far.u == 0 && a.lens[b] != far.n) atomicOr(&g_attn_status, (unsigned)PAGED_LENGTH);
+  if (tid == 0 && rank == 0 && kh == 0 && far.hg == 0 && a.lens[b] != far.n) atomicOr(&g_attn_status, (unsigned)PAGED_LENGTH);
   if (blocks == 0) {  // (the whole cluster)
     for (int i = rank * PA_THREADS + tid; i < count * a.D; i += ks * PA_THREADS) out[i] = from_f32<T>(0.f);
     return;
@@ -829,7 +834,7 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
   P state;
   {
     Feeder<P> feed(s, ring, masks[warp]);
-    Row next = feed.fill(far, units, hop, steps);
+    Row next = feed.fill(far, hop, steps);
     state.begin(s, b, kh, h0, count, extra);
     const Scorer score(a.scale, a.softcap);
     int slot = 0, fill = S - 1;
@@ -838,7 +843,7 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
       __syncwarp();
       if (step + S - 1 < steps) {
         feed.issue(next, fill);
-        if (step + S < steps) far.next<KB>(a, units, hop), next = feed.peek(far);
+        if (step + S < steps) far.next<KB>(s, hop), next = feed.peek(far);
       }
       cp_async_commit();
       state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
