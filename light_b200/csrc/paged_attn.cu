@@ -120,7 +120,7 @@ struct SplitArgs {
   int hpg, groups;    // query heads per unit, units per KV head
   uint32_t ku[3], vu[3], unit;  // the cache's strides in units of so many bytes, in which every row's offset has 32 bits
   bool alike;         // ku == vu
-  int4 *heads;        // per CTA: sequence, unit of it, pieces of the unit that begins there and goes on (0: none)
+  int4 *heads;        // per CTA, of the unit that begins there and goes on: sequence, first query head, heads, pieces (0: none)
   float *ml, *acc;    // [2 CTAs][HEADS][2], [2 CTAs][HEADS][D]
 };
 
@@ -504,20 +504,23 @@ struct SplitCfg {
   static constexpr int SIZE = sizeof(typename P::T), CTAS = split_ctas(SIZE, P::DP, P::HEADS), S = split_stages(SIZE, P::DP, P::HEADS);
   static constexpr int STAGE = 2 * P::KB * P::ROWB, RING = S * STAGE, PART = P::HEADS * P::PR * 4;  // of a warp
   static constexpr int SMEM = PA_WARPS * (RING + PART + P::EXTRA);
-  static_assert(SMEM == split_smem(SIZE, P::DP, P::HEADS, S) && SMEM <= split_room(CTAS) && PART <= RING, "");
+  static_assert(SMEM == split_smem(SIZE, P::DP, P::HEADS, S) && SMEM <= split_room(CTAS) && PART <= RING && PA_WARPS * PART >= PA_THREADS * 4, "");
 };
 
 struct Cursor {
   int b, kh, hg, block, n, j0, blocks;  // sequence, KV head, unit of that, block; the sequence's length, first key, blocks per unit
+  int left;                             // cost of the run from this block on; none left: no block
   template <int KB>
   __device__ __forceinline__ void at(const PagedArgs &a, int b_) {
     b = b_, n = length_of(a, b_), j0 = first_of(a, n), blocks = (n - j0 + KB - 1) / KB;
   }
-  __device__ __forceinline__ void unit(int u, int groups) { kh = u / groups, hg = u - kh * groups; }
+  __device__ __forceinline__ void unit(int u, int groups) { kh = groups == 1 ? u : u / groups, hg = u - kh * groups; }
   template <int KB>
-  __device__ __forceinline__ void next(const SplitArgs &s, int hop) {  // (there is a next block)
-    block += hop;
+  __device__ __forceinline__ void next(const SplitArgs &s, int hop) {
+    block += hop, left -= hop;
     if (block < blocks) return;
+    left -= UNIT;
+    if (left <= 0) return;
     block = 0;
     if (++hg < s.groups) return;
     hg = 0;
@@ -527,6 +530,17 @@ struct Cursor {
     while (blocks == 0);
   }
 };
+
+// four neighbouring elements of an output: v / L
+template <typename T>
+__device__ __forceinline__ void store4(T *out, const float (&v)[4], float L) {
+  const float inv = 1.f / L;
+  alignas(16) T x[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) x[e] = from_f32<T>(L == 0.f ? 0.f : v[e] * inv);
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(x);
+  else *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(x);
+}
 
 // What a warp's copies take: the page of its lane's key, then a block of rows into a slot of its ring.
 struct Row {
@@ -605,23 +619,29 @@ struct Feeder {
       }
     }
   }
-  // the first S - 1 of `steps` blocks on their way, and the next one's page
-  __device__ __forceinline__ Row fill(Cursor &far, int hop, int steps) {
+  // the run's first S - 1 blocks on their way, and the next one's page
+  __device__ __forceinline__ Row fill(Cursor &far, int hop) {
     constexpr int S = C::S;
     Row first[S - 1], next;
+    int have = 0;
 #pragma unroll
     for (int i = 0; i < S - 1; i++)
-      if (i < steps) {
-        if (i) far.next<P::KB>(s, hop);
-        first[i] = peek(far);
-      }
+      if (far.left > 0) first[i] = peek(far), have = i + 1, far.next<P::KB>(s, hop);
 #pragma unroll
     for (int i = 0; i < S - 1; i++) {
-      if (i < steps) issue(first[i], i);
+      if (i < have) issue(first[i], i);
       cp_async_commit();
     }
-    if (S - 1 < steps) far.next<P::KB>(s, hop), next = peek(far);
+    if (far.left > 0) next = peek(far);
     return next;
+  }
+  __device__ __forceinline__ void more(Cursor &far, Row &next, int hop, int slot) {
+    if (far.left > 0) {
+      issue(next, slot);
+      far.next<P::KB>(s, hop);
+      if (far.left > 0) next = peek(far);
+    }
+    cp_async_commit();
   }
 };
 
@@ -631,12 +651,10 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
   using T = typename P::T;
   constexpr int KB = P::KB, S = C::S;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ longlong2 scan[PA_WARPS];
-  __shared__ int4 from[PA_WARPS + 1];              // where the warps' runs begin: sequence, unit, block
-  __shared__ long long place[PA_WARPS + 1], unit0[PA_WARPS + 1];  // the same among all blocks; where the unit begins in cost
+  __shared__ int scan[PA_WARPS];
   __shared__ uint32_t masks[PA_WARPS][S];
   __shared__ int open0[PA_WARPS], open1[PA_WARPS];  // pieces: of a unit begun before the run, of the last begun in it: 0 none, 1 ends in it, 2 goes on
-  __shared__ int4 piece0[PA_WARPS], piece1[PA_WARPS];  // their sequence, unit, blocks
+  __shared__ int4 piece0[PA_WARPS], piece1[PA_WARPS];  // their sequence, first query head, heads, blocks
   __shared__ long long cost1[PA_WARPS];             // where in cost the latter begins
   pdl_launch_dependents();
   pdl_wait();
@@ -644,112 +662,118 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, units = a.KH * s.groups;
   unsigned odd = 0;
 
-  // ---- the warps' runs.  Cost: UNIT, then one for each block, unit after unit; warp i of w has [total i / w, total (i + 1) / w).
+  // ---- the warps' runs.  Cost: UNIT, then one for each block, unit after unit; run i of r has [total i / r, total (i + 1) / r).
   const int per = (a.B + PA_THREADS - 1) / PA_THREADS, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
   auto blocks_of = [&](int b) {
     const int n = length_of(a, b);
     return (n - first_of(a, n) + KB - 1) / KB;
   };
-  longlong2 sum = make_longlong2(0, 0);  // blocks, cost: of one unit of each sequence
+  auto cost_of = [&](int n) { return n ? n + UNIT : 0; };
+  int *const chunk = reinterpret_cast<int *>(smem + PA_WARPS * C::RING);  // (over the parts, until the runs are known)
+  int sum = 0;  // of one unit of each of this thread's sequences (the host has seen to it that all of them sum to less than 2^31)
   for (int b = lo; b < hi; b++) {
     if (cta == 0 && a.lens[b] != length_of(a, b)) odd |= PAGED_LENGTH;
-    const int n = blocks_of(b);
-    sum.x += n, sum.y += n ? n + UNIT : 0;
+    sum += cost_of(blocks_of(b));
   }
-  longlong2 before = sum, total = make_longlong2(0, 0);
+  int before = sum;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, before.x, x), w = __shfl_up_sync(0xffffffffu, before.y, x);
-    if (lane >= x) before.x += v, before.y += w;
+    const int v = __shfl_up_sync(0xffffffffu, before, x);
+    if (lane >= x) before += v;
   }
   if (lane == 31) scan[warp] = before;
+  chunk[tid] = before - sum;
   if (tid < PA_WARPS) open0[tid] = open1[tid] = 0;
   __syncthreads();
-  before.x -= sum.x, before.y -= sum.y;
+  int base[PA_WARPS], each = 0;
 #pragma unroll
-  for (int w = 0; w < PA_WARPS; w++) {
-    if (w < warp) before.x += scan[w].x, before.y += scan[w].y;
-    total.x += scan[w].x, total.y += scan[w].y;
-  }
-  total.x *= units, total.y *= units;
+  for (int w = 0; w < PA_WARPS; w++) base[w] = each, each += scan[w];
+  const long long total = (long long)each * units;
   // CTAs with work: the first ones, PA_WARPS blocks' cost or more each
-  const int dealt = (int)min((long long)gridDim.x, max(total.y / PA_WARPS, 1ll)), runs = dealt * PA_WARPS;
-  const bool small = total.y <= 0x7fffffffll;  // (the 64-bit division takes four times as long)
-  const long long quota = small ? (long long)((unsigned)total.y / (unsigned)runs) : total.y / runs, rest = total.y - quota * runs;
+  const int dealt = (int)min((long long)gridDim.x, max(total / PA_WARPS, 1ll)), runs = dealt * PA_WARPS;
+  const bool small = total <= 0x7fffffffll;  // (the 64-bit division takes four times as long)
+  const long long quota = small ? (long long)((unsigned)total / (unsigned)runs) : total / runs, rest = total - quota * runs;
   auto start_of = [&](int i) { return i * quota + min((long long)i, rest); };
-#pragma unroll 1
-  for (int i = 0; i <= PA_WARPS; i++) {
-    const long long x = cta < dealt ? start_of(cta * PA_WARPS + i) : total.y;
-    if (x >= total.y) {
-      if (tid == 0) from[i] = make_int4(-1, 0, 0, 0), place[i] = total.x;
-    } else if (before.y * units <= x && x < (before.y + sum.y) * units) {
-      longlong2 c = before;
-      int b = lo, n = blocks_of(b);
-      while ((c.y + (n ? n + UNIT : 0)) * units <= x) c.x += n, c.y += n ? n + UNIT : 0, n = blocks_of(++b);
-      from[i] = make_int4(b, n, 0, 0), place[i] = c.x * units, unit0[i] = c.y * units;
-    }
-  }
-  __syncthreads();
-  if (tid <= PA_WARPS && from[tid].x >= 0) {  // the sequence, its blocks and where it begins -> the unit and block
-    const int n = from[tid].y;
-    const long long x = start_of(cta * PA_WARPS + tid), r = x - unit0[tid];
-    const int u = small ? (int)((unsigned)r / (unsigned)(n + UNIT)) : (int)(r / (n + UNIT)), in = (int)(r - (long long)u * (n + UNIT)), block = max(in - UNIT, 0);
-    from[tid] = make_int4(from[tid].x, u, block, n), place[tid] += (long long)u * n + block, unit0[tid] = x - in;
-  }
-  // sequences without keys
-  for (int b = cta; b < a.B; b += gridDim.x)
-    if (blocks_of(b) == 0)
-      for (int i = tid; i < a.NH * a.D; i += PA_THREADS) static_cast<T *>(a.out)[(long long)b * a.NH * a.D + i] = from_f32<T>(0.f);
-  __syncthreads();
-
+  struct Place {
+    int b, u, in, n;  // sequence, unit of it, cost of that before the place, blocks of the unit
+  };
+  auto locate = [&](long long x) {  // (x < total; the whole warp)
+    int t = -1;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++) t += __popc(__ballot_sync(0xffffffffu, (long long)(base[w] + chunk[32 * w + lane]) * units <= x));
+    int c = chunk[t];
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++)
+      if (t >> 5 == w) c += base[w];
+    Place p;
+    p.b = t * per, p.n = blocks_of(p.b);
+    while ((long long)(c + cost_of(p.n)) * units <= x) c += cost_of(p.n), p.n = blocks_of(++p.b);
+    const long long r = x - (long long)c * units;
+    p.u = small ? (int)((unsigned)r / (unsigned)(p.n + UNIT)) : (int)(r / (p.n + UNIT)), p.in = (int)(r - (long long)p.u * (p.n + UNIT));
+    return p;
+  };
   // A CTA inside one unit deals its blocks to the warps in turn, so that they read side by side; else a warp has its own run.
-  const int all = (int)min(place[PA_WARPS] - place[0], 0x7fffffffll);
-  const bool inside = all > 0 && from[0].z + all <= from[0].w;
-  const int steps = inside ? (all - warp + PA_WARPS - 1) / PA_WARPS : (int)(place[warp + 1] - place[warp]), hop = inside ? PA_WARPS : 1;
+  const bool works = cta < dealt && total > 0;
+  bool inside = false;
+  int all = 0, first = 0;  // inside: blocks, the first of them
+  long long begun = 0;     // where the unit at hand begins in cost
+  Cursor now;
+  now.left = 0;
+  if (works) {
+    const long long x0 = start_of(cta * PA_WARPS), x1 = start_of((cta + 1) * PA_WARPS);
+    Place p = locate(x0);
+    inside = x1 - x0 <= p.n + UNIT - p.in;
+    first = max(p.in - UNIT, 0);
+    if (inside) {
+      all = max((int)(x1 - x0) + p.in - UNIT, 0) - first, begun = x0 - p.in;
+      now.block = first + warp, now.left = all - warp;
+    } else {
+      const long long w0 = start_of(cta * PA_WARPS + warp), w1 = start_of(cta * PA_WARPS + warp + 1);
+      if (warp) p = locate(w0);
+      now.block = max(p.in - UNIT, 0), now.left = (int)(w1 - w0) - max(UNIT - p.in, 0), begun = w0 - p.in;
+    }
+    now.at<KB>(a, p.b);
+    now.unit(p.u, s.groups);
+  }
+  const int hop = inside ? PA_WARPS : 1;
+  __syncthreads();
   unsigned char *const ring = smem + warp * C::RING, *const extra = smem + PA_WARPS * (C::RING + C::PART) + warp * P::EXTRA;
   float *const part = reinterpret_cast<float *>(smem + PA_WARPS * C::RING + warp * C::PART);
-  if (steps > 0) {
-    Cursor now, far;  // what is folded, and what is fetched
-    const int4 at = from[inside ? 0 : warp];
-    now.at<KB>(a, at.x);
-    now.unit(at.y, s.groups), now.block = at.z + (inside ? warp : 0);
-    far = now;
+  if (now.left > 0) {
+    Cursor far = now;  // what is fetched, ahead of what is folded
     Feeder<P> feed(s, ring, masks[warp]);
-    Row next = feed.fill(far, hop, steps);
+    Row next = feed.fill(far, hop);
     const Scorer score(a.scale, a.softcap);
     P state;
     bool fresh = true, begins = false;
-    long long begun = unit0[inside ? 0 : warp];  // where the unit begins in cost
     int slot = 0, fill = S - 1;
-    for (int step = 0; step < steps; step++) {
+    while (now.left > 0) {
       if (fresh) begins = now.block == 0, fresh = false, state.begin(s, now.b, now.kh, now.hg * s.hpg, min(s.hpg, a.G - now.hg * s.hpg), extra);
       cp_async_wait<S - 2>();
       __syncwarp();  // the block is there for all lanes, and all are done with the one before
-      if (step + S - 1 < steps) {
-        feed.issue(next, fill);
-        if (step + S < steps) far.next<KB>(s, hop), next = feed.peek(far);
-      }
-      cp_async_commit();
+      feed.more(far, next, hop, fill);
       state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
       slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
+      const bool last = now.left <= hop;
       // (inside one unit its end belongs to the last warp's piece, whoever has the last block)
-      const bool ends = inside ? step + 1 == steps && warp == min(PA_WARPS, all) - 1 && from[0].z + all == now.blocks : now.block + 1 == now.blocks;
-      if (ends || step + 1 == steps) {
+      const bool ends = inside ? last && warp == min(PA_WARPS, all) - 1 && first + all == now.blocks : now.block + 1 == now.blocks;
+      if (ends || last) {
+        const int h0 = now.hg * s.hpg;
+        const int4 who = make_int4(now.b, now.kh * a.G + h0, min(s.hpg, a.G - h0), now.blocks);
         if (begins && ends && !inside) {
-          const int h0 = now.hg * s.hpg;
-          state.write(static_cast<T *>(a.out) + ((long long)now.b * a.NH + now.kh * a.G + h0) * a.D, min(s.hpg, a.G - h0), a.D, extra);
+          state.write(static_cast<T *>(a.out) + ((long long)now.b * a.NH + now.kh * a.G + h0) * a.D, who.z, a.D, extra);
         } else if (begins) {  // (the run's end: its ring is free once the last copies have landed)
           cp_async_wait<0>();
           __syncwarp();
           state.store(reinterpret_cast<float *>(ring), a.D);
-          if (lane == 0) open1[warp] = ends ? 1 : 2, piece1[warp] = make_int4(now.b, now.kh * s.groups + now.hg, now.blocks, 0), cost1[warp] = begun;
+          if (lane == 0) open1[warp] = ends ? 1 : 2, piece1[warp] = who, cost1[warp] = begun;
         } else {
           state.store(part, a.D);
-          if (lane == 0) open0[warp] = ends ? 1 : 2, piece0[warp] = make_int4(now.b, now.kh * s.groups + now.hg, now.blocks, 0);
+          if (lane == 0) open0[warp] = ends ? 1 : 2, piece0[warp] = who;
         }
         fresh = true, begun += now.blocks + UNIT;
       }
-      if (step + 1 < steps) now.next<KB>(s, hop);
+      now.next<KB>(s, hop);
     }
     cp_async_wait<0>();
     odd |= feed.odd;
@@ -759,50 +783,65 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
 
   // ---- the CTA's pieces: a run's first belongs to a unit begun before it, its last to one that goes on in the next warp's first
   int4 head = make_int4(0, 0, 0, 0);
+  unsigned kinds = 0;  // two bits a piece: of warp p / 2, the one begun before its run (p even), or the last begun in it
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; w++) kinds |= (unsigned)(open0[w] | open1[w] << 2) << (4 * w);
 #pragma unroll 1
-  for (int p = 0; p < 2 * PA_WARPS;) {  // piece p: of warp p / 2, the one begun before its run or (late) the one that goes on
-    const int w0 = p >> 1;
-    const bool late = p & 1;
-    if (!(late ? open1[w0] : open0[w0])) {
+  for (int p = 0; p < 2 * PA_WARPS;) {
+    const int w0 = p >> 1, late = p & 1;
+    unsigned kind = kinds >> (2 * p) & 3;
+    if (kind == 0) {
       p++;
       continue;
     }
-    int w1 = w0;
-    bool goes_on = (late ? open1[w0] : open0[w0]) == 2;
-    while (goes_on && w1 + 1 < PA_WARPS && open0[w1 + 1]) goes_on = open0[++w1] == 2;
+    int w1 = w0;  // the last warp that has a piece of the unit
+    while (kind == 2 && w1 + 1 < PA_WARPS && (kinds >> (4 * (w1 + 1)) & 3)) kind = kinds >> (4 * ++w1) & 3;
     const int4 who = late ? piece1[w0] : piece0[w0];
-    const int kh = who.y / s.groups, h0 = (who.y - kh * s.groups) * s.hpg, count = min(s.hpg, a.G - h0);
-    const bool whole = late && !goes_on;
+    const bool whole = late && kind == 1;
     const float *const row0 = reinterpret_cast<const float *>(late ? smem + w0 * C::RING : smem + PA_WARPS * C::RING + w0 * C::PART);
-    auto row = [&](int i, int h) { return (i == 0 ? row0 : reinterpret_cast<const float *>(smem + PA_WARPS * C::RING + (w0 + i) * C::PART)) + h * P::PR; };
-    for (int h = warp; h < count; h += PA_WARPS) {
+    const float *const row1 = reinterpret_cast<const float *>(smem + PA_WARPS * C::RING + w0 * C::PART);
+    for (int h = warp; h < who.z; h += PA_WARPS) {
+      const float *row[PA_WARPS];
+      float2 ml[PA_WARPS];
       float top = -INFINITY, L = 0.f, e[PA_WARPS];
 #pragma unroll
-      for (int i = 0; i < PA_WARPS; i++)
-        if (i <= w1 - w0) top = fmaxf(top, row(i, h)[0]);
+      for (int i = 0; i < PA_WARPS; i++) {
+        row[i] = (i == 0 ? row0 : row1 + i * (C::PART / 4)) + h * P::PR;
+        ml[i] = i <= w1 - w0 ? *reinterpret_cast<const float2 *>(row[i]) : make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[i].x);
+      }
       const float use = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int i = 0; i < PA_WARPS; i++)
-        if (i <= w1 - w0) e[i] = ex2(row(i, h)[0] - use), L = fmaf(e[i], row(i, h)[1], L);
+      for (int i = 0; i < PA_WARPS; i++) e[i] = ex2(ml[i].x - use), L = fmaf(e[i], ml[i].y, L);
       const long long at = (2ll * cta + late) * P::HEADS + h;
-      if (!whole && lane == 0) s.ml[2 * at] = top, s.ml[2 * at + 1] = L;
-      for (int d = lane; d < a.D; d += 32) {
-        float A = 0.f;
+      if (!whole && lane == 0) *reinterpret_cast<float2 *>(s.ml + 2 * at) = make_float2(top, L);
 #pragma unroll
-        for (int i = 0; i < PA_WARPS; i++)
-          if (i <= w1 - w0) A = fmaf(e[i], row(i, h)[4 + d], A);
-        if (whole) static_cast<T *>(a.out)[((long long)who.x * a.NH + kh * a.G + h0 + h) * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
-        else s.acc[at * a.D + d] = A;
-      }
+      for (int d = 4 * lane; d < P::DP; d += 128)
+        if (d < a.D) {
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < PA_WARPS; i++)
+            if (i <= w1 - w0) {
+              const float4 x = *reinterpret_cast<const float4 *>(row[i] + 4 + d);
+              v[0] = fmaf(e[i], x.x, v[0]), v[1] = fmaf(e[i], x.y, v[1]), v[2] = fmaf(e[i], x.z, v[2]), v[3] = fmaf(e[i], x.w, v[3]);
+            }
+          if (whole) store4(static_cast<T *>(a.out) + ((long long)who.x * a.NH + who.y + h) * a.D + d, v, L);
+          else *reinterpret_cast<float4 *>(s.acc + at * a.D + d) = make_float4(v[0], v[1], v[2], v[3]);
+        }
     }
-    if (late && goes_on) {  // the run that has its last block, and so the CTAs that it goes over
-      const long long x = cost1[w0] + UNIT + who.z - 1, wide = rest * (quota + 1);
-      const long long run = x < wide ? x / (quota + 1) : rest + (x - wide) / quota;
-      head = make_int4(who.x, who.y, (int)(run / PA_WARPS) - cta + 1, 0);
+    if (late && kind == 2) {  // the run that has its last block, and so the CTAs that it goes over
+      const long long x = cost1[w0] + UNIT + who.w - 1, wide = rest * (quota + 1);
+      const long long run = small ? (x < wide ? (unsigned)x / (unsigned)(quota + 1) : rest + (unsigned)(x - wide) / (unsigned)quota)
+                                  : (x < wide ? x / (quota + 1) : rest + (x - wide) / quota);
+      head = make_int4(who.x, who.y, who.z, (int)(run / PA_WARPS) - cta + 1);
     }
     p = w1 > w0 ? 2 * w1 + 1 : p + 1;
   }
   if (s.heads && tid == 0) s.heads[cta] = head;
+  // sequences without keys
+  for (int b = cta; b < a.B; b += gridDim.x)
+    if (blocks_of(b) == 0)
+      for (int i = tid; i < a.NH * a.D; i += PA_THREADS) static_cast<T *>(a.out)[(long long)b * a.NH * a.D + i] = from_f32<T>(0.f);
 }
 
 // Few units of few blocks: a cluster of up to eight CTAs takes a unit, its warps the blocks in turn, and the parts meet in the CTAs' shared memory:
@@ -821,7 +860,8 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
   Cursor far;
   far.at<KB>(a, b);
   far.unit(blockIdx.x / ks - b * units, s.groups), far.block = rank * PA_WARPS + warp;
-  const int hop = ks * PA_WARPS, blocks = far.blocks, steps = (blocks - far.block + hop - 1) / hop;  // (rounds to 0 from below)
+  const int hop = ks * PA_WARPS, blocks = far.blocks;
+  far.left = blocks - far.block;
   const int kh = far.kh, h0 = far.hg * s.hpg, count = min(s.hpg, a.G - h0);
   T *const out = static_cast<T *>(a.out) + ((long long)b * a.NH + kh * a.G + h0) * a.D;
   if (tid == 0 && rank == 0 && kh == 0 && far.hg == 0 && a.lens[b] != far.n) atomicOr(&g_attn_status, (unsigned)PAGED_LENGTH);
@@ -834,18 +874,15 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
   P state;
   {
     Feeder<P> feed(s, ring, masks[warp]);
-    Row next = feed.fill(far, hop, steps);
+    int left = far.left;
+    Row next = feed.fill(far, hop);
     state.begin(s, b, kh, h0, count, extra);
     const Scorer score(a.scale, a.softcap);
     int slot = 0, fill = S - 1;
-    for (int step = 0; step < steps; step++) {
+    for (; left > 0; left -= hop) {
       cp_async_wait<S - 2>();
       __syncwarp();
-      if (step + S - 1 < steps) {
-        feed.issue(next, fill);
-        if (step + S < steps) far.next<KB>(s, hop), next = feed.peek(far);
-      }
-      cp_async_commit();
+      feed.more(far, next, hop, fill);
       state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
       slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
     }
@@ -900,66 +937,97 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
 }
 
 // The pieces of a unit that was cut, in order: piece 0 is the second of the CTA where it begins, piece i the first of the i-th CTA after it.
-// A CTA per head; a warp takes every eighth piece.
-constexpr int PJ_WARPS = 8, PJ_MAX = 1024;  // pieces: no more than CTAs of the first launch
+// A warp takes a head of it, eight pieces at a time, all of whose loads are on their way together; a CTA's warps have one head of
+// neighbouring CTAs' units.  The pieces of a unit over many CTAs are shared out among the warps (no more than one such unit can begin in
+// eight neighbouring CTAs) and their results meet in shared memory.
+constexpr int PJ_WARPS = 8, PJ_BATCH = 8, PJ_FEW = 2 * PJ_BATCH;
 
-template <typename T>
-__global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(SplitArgs s, int HEADS) {
-  __shared__ float weight[PJ_MAX], tops[PJ_WARPS], sums[PJ_WARPS], part[PJ_WARPS][PL_MAX_D];
+template <typename T, int NV>  // heads of up to 128 NV
+__global__ void __launch_bounds__(PJ_WARPS * 32, NV == 1 ? 3 : 2) paged_join_kernel(SplitArgs s, int HEADS, int ctas) {
+  __shared__ float part[PJ_WARPS][128 * NV + 4];
+  __shared__ int many;  // the CTA whose unit has many pieces, or -1
   pdl_launch_dependents();
   pdl_wait();
   const PagedArgs &a = s.p;
-  const int4 head = s.heads[blockIdx.x];
-  const int n = head.z, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kh = head.y / s.groups, h0 = (head.y - kh * s.groups) * s.hpg;
-  if (n == 0 || h >= min(s.hpg, a.G - h0)) return;
-  auto place = [&](int i) { return (long long)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * HEADS + h; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += PJ_WARPS * 32) top = fmaxf(top, s.ml[2 * place(i)]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  if (lane == 0) tops[warp] = top;
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) many = -1;
   __syncthreads();
+  float top, L, acc[NV][4];
+  auto fold = [&](int cta, int n, int from, int step) {  // pieces from, from + 1, .. from + 7, from + step, ..
+    top = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int w = 0; w < PJ_WARPS; w++) top = fmaxf(top, tops[w]);
-  if (top == -INFINITY) top = 0.f;
-  float L = 0.f;
-  for (int i = threadIdx.x; i < n; i += PJ_WARPS * 32) {
-    const float e = ex2(s.ml[2 * place(i)] - top);
-    weight[i] = e, L = fmaf(e, s.ml[2 * place(i) + 1], L);
-  }
-  L = warp_sum(L);
-  if (lane == 0) sums[warp] = L;
-  __syncthreads();
-  L = 0.f;
+    for (int x = 0; x < NV; x++)
 #pragma unroll
-  for (int w = 0; w < PJ_WARPS; w++) L += sums[w];
-  float acc[PL_MAX_D / 32];
+      for (int e = 0; e < 4; e++) acc[x][e] = 0.f;
+#pragma unroll 1
+    for (int i0 = from; i0 < n; i0 += step) {
+      float2 ml[PJ_BATCH];
+      float4 v[PJ_BATCH][NV];
+      float mx = top;
 #pragma unroll
-  for (int e = 0; e < PL_MAX_D / 32; e++) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < n; i += PJ_WARPS) {
-    const float w = weight[i];
-    const float *row = s.acc + place(i) * a.D;
+      for (int j = 0; j < PJ_BATCH; j++) {
+        const int i = i0 + j;
+        ml[j] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int x = 0; x < PL_MAX_D / 128; x++)
-      if (4 * lane + 128 * x < a.D) {
-        const float4 v = *reinterpret_cast<const float4 *>(row + 4 * lane + 128 * x);
-        acc[4 * x] = fmaf(w, v.x, acc[4 * x]), acc[4 * x + 1] = fmaf(w, v.y, acc[4 * x + 1]);
-        acc[4 * x + 2] = fmaf(w, v.z, acc[4 * x + 2]), acc[4 * x + 3] = fmaf(w, v.w, acc[4 * x + 3]);
+        for (int x = 0; x < NV; x++) v[j][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < n) {
+          const long long at = (i == 0 ? 2ll * cta + 1 : 2ll * (cta + i)) * HEADS + h;
+          ml[j] = *reinterpret_cast<const float2 *>(s.ml + 2 * at);
+#pragma unroll
+          for (int x = 0; x < NV; x++)
+            if (4 * lane + 128 * x < a.D) v[j][x] = *reinterpret_cast<const float4 *>(s.acc + at * a.D + 4 * lane + 128 * x);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < PJ_BATCH; j++) mx = fmaxf(mx, ml[j].x);
+      const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(top - use);
+      top = mx, L *= corr;
+#pragma unroll
+      for (int x = 0; x < NV; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[x][e] *= corr;
+#pragma unroll
+      for (int j = 0; j < PJ_BATCH; j++) {
+        const float w = ex2(ml[j].x - use);
+        L = fmaf(w, ml[j].y, L);
+#pragma unroll
+        for (int x = 0; x < NV; x++)
+          acc[x][0] = fmaf(w, v[j][x].x, acc[x][0]), acc[x][1] = fmaf(w, v[j][x].y, acc[x][1]), acc[x][2] = fmaf(w, v[j][x].z, acc[x][2]), acc[x][3] = fmaf(w, v[j][x].w, acc[x][3]);
+      }
+    }
+  };
+  auto out_of = [&](const int4 &head) { return static_cast<T *>(a.out) + ((long long)head.x * a.NH + head.y + h) * a.D; };
+  const int cta = blockIdx.x * PJ_WARPS + warp;
+  const int4 head = cta < ctas ? s.heads[cta] : make_int4(0, 0, 0, 0);
+  if (head.w > PJ_FEW && h < head.z) {
+    if (lane == 0) many = cta;
+  } else if (head.w > 0 && h < head.z) {
+    fold(cta, head.w, 0, PJ_BATCH);
+#pragma unroll
+    for (int x = 0; x < NV; x++)
+      if (4 * lane + 128 * x < a.D) store4(out_of(head) + 4 * lane + 128 * x, acc[x], L);
   }
-#pragma unroll
-  for (int x = 0; x < PL_MAX_D / 128; x++)
-    if (4 * lane + 128 * x < a.D)
-#pragma unroll
-      for (int e = 0; e < 4; e++) part[warp][4 * lane + 128 * x + e] = acc[4 * x + e];
   __syncthreads();
+  if (many < 0) return;
+  const int4 big = s.heads[many];
+  T *const out = out_of(big);
+  fold(many, big.w, warp * PJ_BATCH, PJ_WARPS * PJ_BATCH);
+  if (lane == 0) part[warp][0] = top, part[warp][1] = L;
+#pragma unroll
+  for (int x = 0; x < NV; x++)
+    if (4 * lane + 128 * x < a.D) *reinterpret_cast<float4 *>(&part[warp][4 + 4 * lane + 128 * x]) = make_float4(acc[x][0], acc[x][1], acc[x][2], acc[x][3]);
+  __syncthreads();
+  top = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < PJ_WARPS; w++) top = fmaxf(top, part[w][0]);
+  if (top == -INFINITY) top = 0.f;
+#pragma unroll
+  for (int w = 0; w < PJ_WARPS; w++) L = fmaf(ex2(part[w][0] - top), part[w][1], L);
   for (int d = threadIdx.x; d < a.D; d += PJ_WARPS * 32) {
     float A = 0.f;
 #pragma unroll
-    for (int w = 0; w < PJ_WARPS; w++) A += part[w][d];
-    static_cast<T *>(a.out)[((long long)head.x * a.NH + kh * a.G + h0 + h) * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
+    for (int w = 0; w < PJ_WARPS; w++) A = fmaf(ex2(part[w][0] - top), part[w][4 + d], A);
+    out[d] = from_f32<T>(L == 0.f ? 0.f : A / L);
   }
 }
 
@@ -998,13 +1066,18 @@ Cut cut_of(const lb200_paged_attn_args *p) {
   c.HEADS = size == 4 ? (c.hpg <= 1 ? 1 : c.hpg <= 2 ? 2 : c.hpg <= 4 ? 4 : c.hpg <= 8 ? 8 : 16) : (c.hpg <= 8 ? 8 : 16);
   long long keys = (long long)p->W * p->page_size;
   if (p->window > 0 && p->window < keys) keys = p->window;
-  const long long blocks = (keys + (size == 4 ? 7 : 15)) / (size == 4 ? 8 : 16), slots = (long long)split_ctas(size, c.DP, c.HEADS) * sm_count();
+  const long long blocks = (keys + (size == 4 ? 7 : 15)) / (size == 4 ? 8 : 16);
+  if ((blocks + UNIT) * p->B > 0x7fffffffll) {  // (the schedule counts a unit's blocks over all sequences in 32 bits)
+    c.streamed = false;
+    return c;
+  }
+  const long long slots = (long long)split_ctas(size, c.DP, c.HEADS) * sm_count();
   const long long n_units = (long long)p->B * p->KH * c.groups;
   for (c.ks = 1; c.ks < 8 && n_units * (c.ks + 1) <= slots && blocks > c.ks * PA_WARPS;) c.ks++;
   if (n_units * c.ks <= slots && blocks <= (long long)c.ks * PA_WARPS * CLUSTER_BLOCKS) return c;
   c.ks = 0;
   const double most_work = (double)p->B * p->KH * c.groups * (double)(blocks + UNIT) / PA_WARPS;  // CTAs' worth, were every sequence as long as the table
-  c.ctas = (int)(slots < PJ_MAX ? slots : PJ_MAX);
+  c.ctas = (int)slots;
   if (most_work < c.ctas) c.ctas = most_work < 1 ? 1 : (int)most_work;
   c.joined = blocks > 1 && c.ctas > 1;
   if (c.joined) {
@@ -1051,7 +1124,9 @@ int launch_split(const SplitArgs &s, const Cut &c, cudaStream_t st) {
   if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
   if (int rc = launched("paged_decode_attn")) return rc;
   if (!c.joined) return 0;
-  e = launch_early(paged_join_kernel<typename P::T>, dim3((unsigned)c.ctas, (unsigned)c.hpg), dim3(PJ_WARPS * 32), st, s, c.HEADS);
+  const dim3 grid((unsigned)((c.ctas + PJ_WARPS - 1) / PJ_WARPS), (unsigned)c.hpg), block(PJ_WARPS * 32);
+  if constexpr (P::DP <= 128) e = launch_early(paged_join_kernel<typename P::T, 1>, grid, block, st, s, c.HEADS, c.ctas);
+  else e = launch_early(paged_join_kernel<typename P::T, 2>, grid, block, st, s, c.HEADS, c.ctas);
   if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
   return launched("paged_decode_attn (join)");
 }
