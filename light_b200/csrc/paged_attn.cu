@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 //     without a key are filled with zeros: a weight of 0 times what lies there must not be NaN.
 //   * Pieces of a unit that was cut are joined in their order, first those of a CTA's warps at its end, in shared memory; what goes on
 //     over CTAs goes to scratch, at most two pieces a CTA, and a second launch joins those: no atomics, the same bits every time.
-constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 8;
+constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 4, CLUSTER_WIDE = 8;
 
 struct SplitArgs {
   PagedArgs p;
@@ -916,21 +916,26 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_clus
   const uint32_t base = umma::smem_u32(mine);
   for (int i = lo + tid; i < hi; i += PA_THREADS) {
     const int h = i / a.D, d = i - h * a.D;
-    float m[8], l[8], v[8], top = -INFINITY, L = 0.f, A = 0.f;
+    float top = -INFINITY, L = 0.f, A = 0.f;
+    for (int r0 = 0; r0 < ks; r0 += 8) {
+      float m[8], l[8], v[8], mx = top;
 #pragma unroll
-    for (int r = 0; r < 8; r++) {  // all remote loads at once
-      const uint32_t row = umma::map_to_rank(base, (uint32_t)(r < ks ? r : 0)) + (uint32_t)(h * P::PR) * 4u;
-      m[r] = r < ks ? umma::ld_cluster_f32(row) : -INFINITY, l[r] = umma::ld_cluster_f32(row + 4u), v[r] = umma::ld_cluster_f32(row + 16u + (uint32_t)d * 4u);
-    }
-#pragma unroll
-    for (int r = 0; r < 8; r++) top = fmaxf(top, m[r]);
-    if (top == -INFINITY) top = 0.f;
-#pragma unroll
-    for (int r = 0; r < 8; r++)
-      if (r < ks) {
-        const float e = ex2(m[r] - top);
-        L = fmaf(e, l[r], L), A = fmaf(e, v[r], A);
+      for (int r = 0; r < 8; r++) {  // all remote loads at once
+        const uint32_t row = umma::map_to_rank(base, (uint32_t)(r0 + r < ks ? r0 + r : 0)) + (uint32_t)(h * P::PR) * 4u;
+        m[r] = umma::ld_cluster_f32(row), l[r] = umma::ld_cluster_f32(row + 4u), v[r] = umma::ld_cluster_f32(row + 16u + (uint32_t)d * 4u);
       }
+#pragma unroll
+      for (int r = 0; r < 8; r++)
+        if (r0 + r < ks) mx = fmaxf(mx, m[r]);
+      const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(top - use);
+      top = mx, L *= corr, A *= corr;
+#pragma unroll
+      for (int r = 0; r < 8; r++)
+        if (r0 + r < ks) {
+          const float e = ex2(m[r] - use);
+          L = fmaf(e, l[r], L), A = fmaf(e, v[r], A);
+        }
+    }
     out[i] = from_f32<T>(L == 0.f ? 0.f : A / L);
   }
   umma::cluster_sync();  // nobody leaves while a peer still reads its part
@@ -1074,6 +1079,7 @@ Cut cut_of(const lb200_paged_attn_args *p) {
   const long long slots = (long long)split_ctas(size, c.DP, c.HEADS) * sm_count();
   const long long n_units = (long long)p->B * p->KH * c.groups;
   for (c.ks = 1; c.ks < 8 && n_units * (c.ks + 1) <= slots && blocks > c.ks * PA_WARPS;) c.ks++;
+  if (c.ks == 8 && n_units <= CLUSTER_WIDE && blocks > 8 * PA_WARPS) c.ks = 16;
   if (n_units * c.ks <= slots && blocks <= (long long)c.ks * PA_WARPS * CLUSTER_BLOCKS) return c;
   c.ks = 0;
   const double most_work = (double)p->B * p->KH * c.groups * (double)(blocks + UNIT) / PA_WARPS;  // CTAs' worth, were every sequence as long as the table
@@ -1092,7 +1098,10 @@ template <typename P>
 int launch_cluster(const SplitArgs &s, const Cut &c, cudaStream_t st) {
   auto kern = paged_attn_cluster_kernel<P>;
   static DeviceOnce once;
-  cudaError_t e = once.ensure([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<P>::SMEM); });
+  cudaError_t e = once.ensure([&] {
+    const cudaError_t f = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<P>::SMEM);
+  });
   if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(s.p.B * s.p.KH * s.groups * c.ks)), cfg.blockDim = dim3(PA_THREADS), cfg.dynamicSmemBytes = SplitCfg<P>::SMEM, cfg.stream = st;

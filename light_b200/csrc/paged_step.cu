@@ -311,14 +311,18 @@ __global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) 
   }
 }
 
-// Rows that can be cut into chunks of CB bytes.  A warp takes a token (or, of few tokens, some of a token's heads); lg lanes take a head, two chunks
-// each, chosen so that the pairs of the rotation are in one lane: chunk c and the one R / 2 elements on, or any two where the pairs are
-// neighbours.  So a head is read and written once, in whole sectors, its mean square is log2(lg) shuffles, and an angle's sine and cosine
-// stay in registers for all heads of the token.  Bound by the memory: 2 (NH + 2 KH) D elements per token.
+// Rows that can be cut into chunks of CB bytes.  A warp takes a token (or, of few tokens, some of a token's heads), lg lanes a head, two chunks each,
+// chosen so that the pairs of the rotation are in one lane: chunk c and the one R / 2 elements on, or any two where the pairs are neighbours.  So
+// a head is read and written once, in whole sectors, its mean square is log2(lg) shuffles, and an angle's sine and cosine, times the weights,
+// stay in registers for all heads of the token: with f, g the lane's chunks and r = rsqrt(mean square + eps)
+//   f' = r (f (w_f cos) - g (w_g sin)),  g' = r (f (w_f sin) + g (w_g cos)),
+// two elements to an instruction (f32x2).  Bound by the memory, 2 (NH + 2 KH) D elements per token, with half as many instructions again as
+// the issue slots that takes: hence the pairs, and a pass each for queries, keys and values without a choice inside.
 constexpr int RC_WARPS = 4, RC_AHEAD = 2;  // heads of a lane that are on their way together
 
 struct Chunks {
   int lg, split, first, count;  // lanes per head, warps per token; chunks that a lane's second lies behind its first; chunks per head
+  float over_d;                 // 1 / D
 };
 
 template <int CB>
@@ -345,47 +349,69 @@ __device__ __forceinline__ void st_raw(void *p, const Raw<CB> &r) {
   else if constexpr (CB == 8) *static_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
   else *static_cast<uint32_t *>(p) = r.w[0];
 }
+// two f32 in a 64-bit register
+__device__ __forceinline__ uint64_t two(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ float lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 template <typename T, int CB>
-__device__ __forceinline__ void unpack(const Raw<CB> &r, float (&f)[CB / sizeof(T)]) {
+__device__ __forceinline__ void unpack(const Raw<CB> &r, uint64_t (&f)[CB / sizeof(T) / 2]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < CB / 4; i++) {
-    if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(r.w[i]);
-    else {
+    for (int i = 0; i < CB / 8; i++) f[i] = (uint64_t)r.w[2 * i + 1] << 32 | r.w[2 * i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < CB / 4; i++) {
       const T *h = reinterpret_cast<const T *>(&r.w[i]);
-      f[2 * i] = to_f32(h[0]), f[2 * i + 1] = to_f32(h[1]);
+      f[i] = two(to_f32(h[0]), to_f32(h[1]));
     }
   }
 }
+__device__ __forceinline__ uint32_t rounded(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t rounded(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
 template <typename T, int CB>
-__device__ __forceinline__ Raw<CB> packed(const float (&f)[CB / sizeof(T)]) {
+__device__ __forceinline__ Raw<CB> packed(const uint64_t (&f)[CB / sizeof(T) / 2]) {
   Raw<CB> r;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < CB / 4; i++) {
-    if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(f[i]);
-    else {
-      T *h = reinterpret_cast<T *>(&r.w[i]);
-      h[0] = from_f32<T>(f[2 * i]), h[1] = from_f32<T>(f[2 * i + 1]);
-    }
+    for (int i = 0; i < CB / 8; i++) r.w[2 * i] = (uint32_t)f[i], r.w[2 * i + 1] = (uint32_t)(f[i] >> 32);
+  } else {
+#pragma unroll
+    for (int i = 0; i < CB / 4; i++) r.w[i] = rounded(lo(f[i]), hi(f[i]), T());
   }
   return r;
 }
 
-template <typename T, int CB>
+template <typename T, int CB, bool BETWEEN>
 __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(RotateArgs a, Chunks ch) {
-  constexpr int E = CB / (int)sizeof(T);
+  constexpr int E = CB / (int)sizeof(T), V = E / 2;
   __shared__ float2 trig[RC_WARPS][RT_MAX_D / 2];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.R >> 1;
-  const long long id = (long long)blockIdx.x * RC_WARPS + warp, t = id / ch.split;
+  const long long id = (long long)blockIdx.x * RC_WARPS + warp, t = ch.split == 1 ? id : id / ch.split;
   if (t >= a.T) return;
-  const int part = (int)(id - t * ch.split), gl = lane & (ch.lg - 1), per = 32 / ch.lg;
+  const int part = (int)(id - t * ch.split), gl = lane & (ch.lg - 1), per = 32 / ch.lg, hl = lane / ch.lg;
   // this lane's chunks, -1 for none
   int c0, c1;
-  bool turns;  // half layout: the lane's two chunks are pairs
-  if (a.interleaved) {
-    turns = false, c0 = gl < ch.count ? gl : -1, c1 = gl < ch.first && gl + ch.first < ch.count ? gl + ch.first : -1;
-    if (gl >= ch.first) c0 = -1;
+  bool turns = false;  // BETWEEN false: the lane's two chunks are pairs
+  if constexpr (BETWEEN) {
+    c0 = gl < ch.first ? gl : -1, c1 = gl < ch.first && gl + ch.first < ch.count ? gl + ch.first : -1;
   } else {
     turns = gl < ch.first;
     c0 = turns ? gl : 2 * ch.first + 2 * (gl - ch.first), c1 = turns ? gl + ch.first : c0 + 1;
@@ -403,98 +429,141 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     }
     if (slot >= 0) page = (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
   }
-  const int heads = a.slots ? (slot >= 0 ? a.NH + 2 * a.KH : a.NH) : a.NH + a.KH;
-  const T *q = static_cast<const T *>(a.q) + t * a.q_s[0], *k = static_cast<const T *>(a.k) + t * a.k_s[0], *v = static_cast<const T *>(a.v) + t * a.v_s[0];
-  const int h0 = part * per + lane / ch.lg, step = ch.split * per;
-  auto fetch = [&](int h, Raw<CB> &x, Raw<CB> &y) {
-    if (h >= heads) return;
-    const T *p = h < a.NH ? q + h * a.q_s[1] : h < a.NH + a.KH ? k + (h - a.NH) * a.k_s[1] : v + (h - a.NH - a.KH) * a.v_s[1];
+  // rounds of `per` heads: queries, keys, values; this warp's are part, part + split, ..
+  const int rq = (a.NH + per - 1) / per, rk = (a.KH + per - 1) / per;
+  const int rounds = a.slots ? (slot >= 0 ? rq + 2 * rk : rq) : rq + rk;
+  struct Side {  // of one of the three: where this lane's head of round 0 comes from and goes to, elements from a round to the next
+    const T *from;
+    T *to;
+    long long step_from, step_to;
+    int heads;
+  };
+  auto side_of = [&](int kind) {
+    Side d;
+    const long long *st = kind == 0 ? a.q_s : kind == 1 ? a.k_s : a.v_s;
+    d.from = static_cast<const T *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + t * st[0] + hl * st[1], d.step_from = per * st[1];
+    d.heads = kind == 0 ? a.NH : a.KH;
+    if (kind == 0) d.to = static_cast<T *>(a.q_out) + (t * a.NH + hl) * a.D, d.step_to = (long long)per * a.D;
+    else if (!a.slots) d.to = static_cast<T *>(a.k_out) + (t * a.KH + hl) * a.D, d.step_to = (long long)per * a.D;
+    else {
+      const long long *cs = kind == 1 ? a.ks : a.vs;
+      d.to = static_cast<T *>(kind == 1 ? a.k_out : a.v_out) + page * cs[0] + hl * cs[1] + row * cs[2], d.step_to = per * cs[1];
+    }
+    return d;
+  };
+  auto kind_of = [&](int r) { return r < rq ? 0 : r < rq + rk ? 1 : 2; };
+  auto base_of = [&](int kind) { return kind == 0 ? 0 : kind == 1 ? rq : rq + rk; };
+  auto fetch = [&](const Side &d, int r, Raw<CB> &x, Raw<CB> &y) {
+    if (r * per + hl >= d.heads) return;
+    const T *p = d.from + r * d.step_from;
     if (c0 >= 0) x = ld_raw<CB>(p + c0 * E);
     if (c1 >= 0) y = ld_raw<CB>(p + c1 * E);
   };
   Raw<CB> x[RC_AHEAD], y[RC_AHEAD];
 #pragma unroll
-  for (int i = 0; i < RC_AHEAD; i++) x[i] = Raw<CB>{}, y[i] = Raw<CB>{}, fetch(h0 + i * step, x[i], y[i]);
+  for (int i = 0; i < RC_AHEAD; i++) x[i] = Raw<CB>{}, y[i] = Raw<CB>{};
+  int r = part, kind = kind_of(r);
+  Side d = side_of(kind);
+  // the first rounds are on their way while the angles are worked out
+  auto ahead = [&](int kind) {
+#pragma unroll
+    for (int i = 0; i < RC_AHEAD; i++) {
+      const int n = r + i * ch.split;
+      if (n < rounds && kind_of(n) == kind) fetch(d, n - base_of(kind), x[i], y[i]);
+    }
+  };
+  if (r < rounds) ahead(kind);
   for (int i = lane; i < half; i += 32) {
     const float2 cs = cos_sin(pos, a.inv_freq[i]);
     trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
   }
   __syncwarp();
-  float2 cs[E];
-  unsigned turned = 0;  // interleaved: bit j: pair j of the first chunk turns; E / 2 + j: of the second
+  while (r < rounds) {
+    // ---- the rounds of one kind
+    const int base = base_of(kind), end = min(rounds, kind == 0 ? rq : kind == 1 ? rq + rk : rounds);
+    const T *const w = static_cast<const T *>(kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr);
+    auto put = [&](int n, const Raw<CB> &u, const Raw<CB> &z) {
+      if ((n - base) * per + hl >= d.heads) return;
+      T *const to = d.to + (n - base) * d.step_to;
+      if (c0 >= 0) st_raw<CB>(to + c0 * E, u);
+      if (c1 >= 0) st_raw<CB>(to + c1 * E, z);
+    };
+    if (kind == 2) {
+      for (; r < end; r += RC_AHEAD * ch.split) {
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    int i = c0 * E + e;
-    bool on = turns;
-    if (a.interleaved) {
-      const int c = e < E / 2 ? c0 : c1;
-      i = c * (E / 2) + e % (E > 1 ? E / 2 : 1), on = c >= 0 && i < half;
-      turned |= (unsigned)on << e;
+        for (int i = 0; i < RC_AHEAD; i++) {
+          const int n = r + i * ch.split;
+          if (n < end) {
+            put(n, x[i], y[i]);
+            if (n + RC_AHEAD * ch.split < end) fetch(d, n + RC_AHEAD * ch.split - base, x[i], y[i]);
+          }
+        }
+      }
+      return;  // (the last kind)
     }
-    cs[e] = on ? trig[warp][i] : make_float2(1.f, 0.f);
-  }
-  Raw<CB> wq0{}, wq1{}, wk0{}, wk1{};
-  if (a.qw) {
-    const T *w = static_cast<const T *>(a.qw);
-    if (c0 >= 0) wq0 = ld_raw<CB>(w + c0 * E);
-    if (c1 >= 0) wq1 = ld_raw<CB>(w + c1 * E);
-  }
-  if (a.kw) {
-    const T *w = static_cast<const T *>(a.kw);
-    if (c0 >= 0) wk0 = ld_raw<CB>(w + c0 * E);
-    if (c1 >= 0) wk1 = ld_raw<CB>(w + c1 * E);
-  }
-  for (int base = part * per; base < heads; base += RC_AHEAD * step) {
+    // what f and g are multiplied by: f' = f ff + g gf, g' = f fg + g gg (halves); per chunk x' = x ff + swapped x gf (neighbours: chunk g has fg, gg)
+    uint64_t ff[V], gf[V], fg[V], gg[V];
+    unsigned turned = 0;  // BETWEEN: bit j: pair j of the first chunk turns; V + j: of the second
+    {
+      Raw<CB> w0{}, w1{};
+      uint64_t wf[V], wg[V];
+      if (w && c0 >= 0) w0 = ld_raw<CB>(w + c0 * E);
+      if (w && c1 >= 0) w1 = ld_raw<CB>(w + c1 * E);
+      unpack<T, CB>(w0, wf), unpack<T, CB>(w1, wg);
 #pragma unroll
-    for (int i = 0; i < RC_AHEAD; i++) {
-      const int h = base + lane / ch.lg + i * step;
-      const bool is_q = h < a.NH, is_v = h >= a.NH + a.KH;
-      const void *w = is_q ? a.qw : a.kw;
-      float f[E], g[E];
-      unpack<T, CB>(x[i], f), unpack<T, CB>(y[i], g);
-      float ss = 0.f;
+      for (int j = 0; j < V; j++) {
+        if (!w) wf[j] = wg[j] = two(1.f, 1.f);
+        if constexpr (BETWEEN) {
+          const int i0 = c0 * V + j, i1 = c1 * V + j;
+          const bool on0 = c0 >= 0 && i0 < half, on1 = c1 >= 0 && i1 < half;
+          const float2 p = on0 ? trig[warp][i0] : make_float2(1.f, 0.f), q = on1 ? trig[warp][i1] : make_float2(1.f, 0.f);
+          turned |= (unsigned)on0 << j | (unsigned)on1 << (V + j);
+          ff[j] = mul2(wf[j], two(p.x, p.x)), gf[j] = two(-hi(wf[j]) * p.y, lo(wf[j]) * p.y);
+          gg[j] = mul2(wg[j], two(q.x, q.x)), fg[j] = two(-hi(wg[j]) * q.y, lo(wg[j]) * q.y);
+        } else {
+          const float2 p = turns ? trig[warp][c0 * E + 2 * j] : make_float2(1.f, 0.f), q = turns ? trig[warp][c0 * E + 2 * j + 1] : make_float2(1.f, 0.f);
+          ff[j] = mul2(wf[j], two(p.x, q.x)), gf[j] = mul2(wg[j], two(-p.y, -q.y)), fg[j] = mul2(wf[j], two(p.y, q.y)), gg[j] = mul2(wg[j], two(p.x, q.x));
+        }
+      }
+    }
+    for (; r < end; r += RC_AHEAD * ch.split) {
 #pragma unroll
-      for (int e = 0; e < E; e++) ss = fmaf(f[e], f[e], ss);
-#pragma unroll
-      for (int e = 0; e < E; e++) ss = fmaf(g[e], g[e], ss);
-      if (a.qw || a.kw)
-        for (int o = ch.lg >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      Raw<CB> u = x[i], z = y[i];
-      if (!is_v) {
+      for (int i = 0; i < RC_AHEAD; i++) {
+        const int n = r + i * ch.split;
+        if (n >= end) break;
+        uint64_t f[V], g[V];
+        unpack<T, CB>(x[i], f), unpack<T, CB>(y[i], g);
+        if (n + RC_AHEAD * ch.split < end) fetch(d, n + RC_AHEAD * ch.split - base, x[i], y[i]);
         if (w) {
-          const float inv = rsqrtf(ss / (float)a.D + a.eps);
-          float wf[E], wg[E];
-          unpack<T, CB>(is_q ? wq0 : wk0, wf), unpack<T, CB>(is_q ? wq1 : wk1, wg);
+          uint64_t s0 = mul2(f[0], f[0]), s1 = mul2(g[0], g[0]);
 #pragma unroll
-          for (int e = 0; e < E; e++) f[e] = f[e] * inv * wf[e], g[e] = g[e] * inv * wg[e];
+          for (int j = 1; j < V; j++) s0 = fma2(f[j], f[j], s0), s1 = fma2(g[j], g[j], s1);
+          float ss = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
+          for (int o = ch.lg >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(ss * ch.over_d + a.eps);
+          const uint64_t inv2 = two(inv, inv);
+#pragma unroll
+          for (int j = 0; j < V; j++) f[j] = mul2(f[j], inv2), g[j] = mul2(g[j], inv2);
         }
-        if (a.interleaved) {
+        uint64_t u[V], z[V];
 #pragma unroll
-          for (int e = 0; e + 1 < E; e += 2) {
-            const float2 p = cs[e / 2], r = cs[E / 2 + e / 2];
-            const float f0 = f[e] * p.x - f[e + 1] * p.y, f1 = f[e] * p.y + f[e + 1] * p.x, g0 = g[e] * r.x - g[e + 1] * r.y, g1 = g[e] * r.y + g[e + 1] * r.x;
-            if (turned >> (e / 2) & 1) f[e] = f0, f[e + 1] = f1;
-            if (turned >> (E / 2 + e / 2) & 1) g[e] = g0, g[e + 1] = g1;
-          }
-        } else if (turns) {
-#pragma unroll
-          for (int e = 0; e < E; e++) {
-            const float f0 = f[e] * cs[e].x - g[e] * cs[e].y, g0 = f[e] * cs[e].y + g[e] * cs[e].x;
-            f[e] = f0, g[e] = g0;
+        for (int j = 0; j < V; j++) {
+          if constexpr (BETWEEN) {
+            u[j] = mul2(f[j], ff[j]), z[j] = mul2(g[j], gg[j]);
+            if (turned >> j & 1) u[j] = fma2(two(hi(f[j]), lo(f[j])), gf[j], u[j]);
+            if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[j]), lo(g[j])), fg[j], z[j]);
+          } else {
+            u[j] = mul2(f[j], ff[j]), z[j] = mul2(g[j], gg[j]);
+            if (turns) u[j] = fma2(g[j], gf[j], u[j]), z[j] = fma2(f[j], fg[j], z[j]);
           }
         }
-        u = packed<T, CB>(f), z = packed<T, CB>(g);
+        put(n, packed<T, CB>(u), packed<T, CB>(z));
       }
-      if (h < heads) {
-        const int kh = is_v ? h - a.NH - a.KH : h - a.NH;
-        T *to = is_q   ? static_cast<T *>(a.q_out) + (t * a.NH + h) * a.D
-                : is_v ? static_cast<T *>(a.v_out) + page * a.vs[0] + kh * a.vs[1] + row * a.vs[2]
-                       : static_cast<T *>(a.k_out) + (a.slots ? page * a.ks[0] + kh * a.ks[1] + row * a.ks[2] : (t * a.KH + kh) * a.D);
-        if (c0 >= 0) st_raw<CB>(to + c0 * E, u);
-        if (c1 >= 0) st_raw<CB>(to + c1 * E, z);
-      }
-      fetch(h + RC_AHEAD * step, x[i], y[i]);
     }
+    // the next kind's first rounds
+    r = base_of(++kind);
+    r += (part - r % ch.split + ch.split) % ch.split;
+    if (r < rounds) d = side_of(kind), ahead(kind);
   }
 }
 
@@ -550,11 +619,16 @@ int qk_norm_rope_check(const lb200_qk_norm_rope_args *p) {
   return 0;
 }
 
+template <typename T, int CB>
+static cudaError_t launch_as(const RotateArgs &a, const Chunks &ch, unsigned ctas, cudaStream_t st) {
+  return a.interleaved ? launch_early(qk_norm_rope_chunks_kernel<T, CB, true>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch)
+                       : launch_early(qk_norm_rope_chunks_kernel<T, CB, false>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch);
+}
 template <typename T>
 static cudaError_t launch_cb(const RotateArgs &a, const Chunks &ch, int cb, unsigned ctas, cudaStream_t st) {
-  return cb == 16  ? launch_early(qk_norm_rope_chunks_kernel<T, 16>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch)
-         : cb == 8 ? launch_early(qk_norm_rope_chunks_kernel<T, 8>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch)
-                   : launch_early(qk_norm_rope_chunks_kernel<T, 4>, dim3(ctas), dim3(RC_WARPS * 32), st, a, ch);
+  if constexpr (sizeof(T) == 2)
+    if (cb == 4) return launch_as<T, 4>(a, ch, ctas, st);
+  return cb == 16 ? launch_as<T, 16>(a, ch, ctas, st) : launch_as<T, 8>(a, ch, ctas, st);
 }
 static int launch_chunks(const RotateArgs &a, const Chunks &ch, int cb, int dtype, unsigned ctas, cudaStream_t st) {
   const cudaError_t e = dtype == LB200_F32    ? launch_cb<float>(a, ch, cb, ctas, st)
@@ -584,16 +658,16 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
   }
   if (!p->interleaved) off |= (uint64_t)(p->rotary / 2) * size;
   int cb = off & 15 ? off & 7 ? off & 3 ? 0 : 4 : 8 : 16;
-  if (p->interleaved && cb < 2 * size) cb = 0;
+  if (cb < 2 * size) cb = 0;
   if (cb) {
     Chunks ch{};
-    ch.count = p->D * size / cb;
+    ch.count = p->D * size / cb, ch.over_d = 1.f / (float)p->D;
     ch.first = p->interleaved ? (ch.count + 1) / 2 : p->rotary / 2 * size / cb;
     const int lanes = p->interleaved ? ch.first : ch.first + (ch.count - 2 * ch.first + 1) / 2;
     for (ch.lg = 1; ch.lg < lanes;) ch.lg *= 2;
     if (ch.lg <= 32) {
       // warps per token: until there are eight for every SM, each with a round of heads or more
-      const int heads = p->NH + p->KH * (p->slots ? 2 : 1), rounds = (heads * ch.lg + 31) / 32;
+      const int per = 32 / ch.lg, rounds = (p->NH + per - 1) / per + (p->KH + per - 1) / per * (p->slots ? 2 : 1);
       for (ch.split = 1; ch.split < rounds && p->T * ch.split < 8ll * sm_count();) ch.split++;
       const long long ctas = (p->T * ch.split + RC_WARPS - 1) / RC_WARPS;
       if (ctas <= 0x7fffffffll) return launch_chunks(a, ch, cb, p->dtype, (unsigned)ctas, st);
