@@ -318,10 +318,11 @@ __global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) 
 //   f' = r (f (w_f cos) - g (w_g sin)),  g' = r (f (w_f sin) + g (w_g cos)),
 // two elements to an instruction (f32x2).  Bound by the memory, 2 (NH + 2 KH) D elements per token, with half as many instructions again as
 // the issue slots that takes: hence the pairs, and a pass each for queries, keys and values without a choice inside.
-constexpr int RC_WARPS = 4, RC_AHEAD = 2;  // heads of a lane that are on their way together
+constexpr int RC_WARPS = 4, RC_AHEAD = 6;  // rounds of heads that are on their way together
 
 struct Chunks {
   int lg, split, first, count;  // lanes per head, warps per token; chunks that a lane's second lies behind its first; chunks per head
+  int q_parts, k_parts;         // of several warps per token, those of the queries, and of the keys and of the values
   float over_d;                 // 1 / D
 };
 
@@ -333,13 +334,13 @@ template <int CB>
 __device__ __forceinline__ Raw<CB> ld_raw(const void *p) {
   Raw<CB> r;
   if constexpr (CB == 16) {
-    const uint4 v = __ldcs(static_cast<const uint4 *>(p));
+    const uint4 v = *static_cast<const uint4 *>(p);
     r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
   } else if constexpr (CB == 8) {
-    const uint2 v = __ldcs(static_cast<const uint2 *>(p));
+    const uint2 v = *static_cast<const uint2 *>(p);
     r.w[0] = v.x, r.w[1] = v.y;
   } else {
-    r.w[0] = __ldcs(static_cast<const uint32_t *>(p));
+    r.w[0] = *static_cast<const uint32_t *>(p);
   }
   return r;
 }
@@ -348,6 +349,25 @@ __device__ __forceinline__ void st_raw(void *p, const Raw<CB> &r) {
   if constexpr (CB == 16) *static_cast<uint4 *>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
   else if constexpr (CB == 8) *static_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
   else *static_cast<uint32_t *>(p) = r.w[0];
+}
+template <int CB>
+__device__ __forceinline__ void cp_chunk(uint32_t dst, const void *src) {
+  if constexpr (CB == 16) cp_async16(dst, src);
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(CB) : "memory");
+}
+template <int CB>
+__device__ __forceinline__ Raw<CB> lds_raw(uint32_t addr) {
+  Raw<CB> r;
+  if constexpr (CB == 16) {
+    const uint4 v = lds128(addr);
+    r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+  } else if constexpr (CB == 8) {
+    const uint2 v = lds64(addr);
+    r.w[0] = v.x, r.w[1] = v.y;
+  } else {
+    r.w[0] = lds32(addr);
+  }
+  return r;
 }
 // two f32 in a 64-bit register
 __device__ __forceinline__ uint64_t two(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
@@ -400,13 +420,20 @@ __device__ __forceinline__ Raw<CB> packed(const uint64_t (&f)[CB / sizeof(T) / 2
 template <typename T, int CB, bool BETWEEN>
 __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(RotateArgs a, Chunks ch) {
   constexpr int E = CB / (int)sizeof(T), V = E / 2;
+  __shared__ __align__(16) unsigned char ring[RC_WARPS][RC_AHEAD][2][32][CB];
   __shared__ float2 trig[RC_WARPS][RT_MAX_D / 2];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.R >> 1;
   const long long id = (long long)blockIdx.x * RC_WARPS + warp, t = ch.split == 1 ? id : id / ch.split;
   if (t >= a.T) return;
-  const int part = (int)(id - t * ch.split), gl = lane & (ch.lg - 1), per = 32 / ch.lg, hl = lane / ch.lg;
+  const int gl = lane & (ch.lg - 1), per = 32 / ch.lg, hl = lane / ch.lg;
+  // the kinds (queries, keys, values) of this warp and its part of their heads: all of a token, or with several warps per token one kind
+  int part = (int)(id - t * ch.split), parts = 1, kind = 0;
+  if (ch.split > 1) {
+    kind = part < ch.q_parts ? 0 : part < ch.q_parts + ch.k_parts ? 1 : 2, parts = kind == 0 ? ch.q_parts : ch.k_parts;
+    part -= kind == 0 ? 0 : kind == 1 ? ch.q_parts : ch.q_parts + ch.k_parts;
+  }
   // this lane's chunks, -1 for none
   int c0, c1;
   bool turns = false;  // BETWEEN false: the lane's two chunks are pairs
@@ -427,80 +454,82 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
       if (lane == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
       slot = -1;
     }
-    if (slot >= 0) page = (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
+    if (slot >= 0) page = a.rows <= 0x7fffffffll ? a.page.div((int)slot) : (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
   }
-  // rounds of `per` heads: queries, keys, values; this warp's are part, part + split, ..
-  const int rq = (a.NH + per - 1) / per, rk = (a.KH + per - 1) / per;
-  const int rounds = a.slots ? (slot >= 0 ? rq + 2 * rk : rq) : rq + rk;
-  struct Side {  // of one of the three: where this lane's head of round 0 comes from and goes to, elements from a round to the next
-    const T *from;
-    T *to;
-    long long step_from, step_to;
-    int heads;
+  // Rounds of `per` heads of a kind, this warp has every parts-th: where this lane's head of the next of them lies, elements from one to the next, and
+  // the heads from this lane's on (it has one while left > 0).
+  struct Walk {
+    T *at;
+    long long step;
+    int left;
   };
-  auto side_of = [&](int kind) {
-    Side d;
+  const int hop = per * parts, h0 = part * per + hl;
+  auto source = [&](int kind) {
     const long long *st = kind == 0 ? a.q_s : kind == 1 ? a.k_s : a.v_s;
-    d.from = static_cast<const T *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + t * st[0] + hl * st[1], d.step_from = per * st[1];
-    d.heads = kind == 0 ? a.NH : a.KH;
-    if (kind == 0) d.to = static_cast<T *>(a.q_out) + (t * a.NH + hl) * a.D, d.step_to = (long long)per * a.D;
-    else if (!a.slots) d.to = static_cast<T *>(a.k_out) + (t * a.KH + hl) * a.D, d.step_to = (long long)per * a.D;
-    else {
-      const long long *cs = kind == 1 ? a.ks : a.vs;
-      d.to = static_cast<T *>(kind == 1 ? a.k_out : a.v_out) + page * cs[0] + hl * cs[1] + row * cs[2], d.step_to = per * cs[1];
-    }
-    return d;
+    return Walk{static_cast<T *>(const_cast<void *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v)) + t * st[0] + h0 * st[1], hop * st[1], (kind == 0 ? a.NH : a.KH) - h0};
   };
-  auto kind_of = [&](int r) { return r < rq ? 0 : r < rq + rk ? 1 : 2; };
-  auto base_of = [&](int kind) { return kind == 0 ? 0 : kind == 1 ? rq : rq + rk; };
-  auto fetch = [&](const Side &d, int r, Raw<CB> &x, Raw<CB> &y) {
-    if (r * per + hl >= d.heads) return;
-    const T *p = d.from + r * d.step_from;
-    if (c0 >= 0) x = ld_raw<CB>(p + c0 * E);
-    if (c1 >= 0) y = ld_raw<CB>(p + c1 * E);
+  auto target = [&](int kind) {
+    const int left = (kind == 0 ? a.NH : a.KH) - h0;
+    if (kind == 0) return Walk{static_cast<T *>(a.q_out) + (t * a.NH + h0) * a.D, (long long)hop * a.D, left};
+    if (!a.slots) return Walk{static_cast<T *>(a.k_out) + (t * a.KH + h0) * a.D, (long long)hop * a.D, left};
+    const long long *cs = kind == 1 ? a.ks : a.vs;
+    return Walk{static_cast<T *>(kind == 1 ? a.k_out : a.v_out) + page * cs[0] + h0 * cs[1] + row * cs[2], hop * cs[1], left};
   };
-  Raw<CB> x[RC_AHEAD], y[RC_AHEAD];
-#pragma unroll
-  for (int i = 0; i < RC_AHEAD; i++) x[i] = Raw<CB>{}, y[i] = Raw<CB>{};
-  int r = part, kind = kind_of(r);
-  Side d = side_of(kind);
-  // the first rounds are on their way while the angles are worked out
-  auto ahead = [&](int kind) {
-#pragma unroll
-    for (int i = 0; i < RC_AHEAD; i++) {
-      const int n = r + i * ch.split;
-      if (n < rounds && kind_of(n) == kind) fetch(d, n - base_of(kind), x[i], y[i]);
-    }
-  };
-  if (r < rounds) ahead(kind);
-  for (int i = lane; i < half; i += 32) {
-    const float2 cs = cos_sin(pos, a.inv_freq[i]);
-    trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
-  }
-  __syncwarp();
-  while (r < rounds) {
-    // ---- the rounds of one kind
-    const int base = base_of(kind), end = min(rounds, kind == 0 ? rq : kind == 1 ? rq + rk : rounds);
-    const T *const w = static_cast<const T *>(kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr);
-    auto put = [&](int n, const Raw<CB> &u, const Raw<CB> &z) {
-      if ((n - base) * per + hl >= d.heads) return;
-      T *const to = d.to + (n - base) * d.step_to;
-      if (c0 >= 0) st_raw<CB>(to + c0 * E, u);
-      if (c1 >= 0) st_raw<CB>(to + c1 * E, z);
-    };
-    if (kind == 2) {
-      for (; r < end; r += RC_AHEAD * ch.split) {
-#pragma unroll
-        for (int i = 0; i < RC_AHEAD; i++) {
-          const int n = r + i * ch.split;
-          if (n < end) {
-            put(n, x[i], y[i]);
-            if (n + RC_AHEAD * ch.split < end) fetch(d, n + RC_AHEAD * ch.split - base, x[i], y[i]);
-          }
-        }
+  const int kinds = min(a.slots ? (slot >= 0 ? 3 : 1) : 2, ch.split > 1 ? kind + 1 : 3);
+  if (kind >= kinds) return;
+  // a ring of rounds in shared memory: every lane copies and reads its own chunks, so nobody waits for anybody
+  const uint32_t mine = umma::smem_u32(ring[warp]) + lane * CB;
+  int far_kind = kind, slot_far = 0, slot_now = 0;
+  Walk far = source(kind);
+  auto fetch = [&]() {  // the next round, if there is one
+    if (far_kind < kinds) {
+      if (far.left > 0) {
+        const uint32_t dst = mine + slot_far * (64 * CB);
+        if (c0 >= 0) cp_chunk<CB>(dst, far.at + c0 * E);
+        if (c1 >= 0) cp_chunk<CB>(dst + 32 * CB, far.at + c1 * E);
       }
-      return;  // (the last kind)
+      far.at += far.step, far.left -= hop;
+      if (far.left + hl <= 0 && ++far_kind < kinds) far = source(far_kind);  // (the same for the whole warp)
     }
+    cp_async_commit();
+    slot_far = slot_far + 1 == RC_AHEAD ? 0 : slot_far + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < RC_AHEAD; i++) fetch();  // on their way while the angles are worked out
+  if (kind < 2) {
+    for (int i = lane; i < half; i += 32) {
+      const float2 cs = cos_sin(pos, a.inv_freq[i]);
+      trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
+    }
+    __syncwarp();
+  }
+  Walk to;
+  auto take = [&](Raw<CB> &x, Raw<CB> &y) {
+    cp_async_wait<RC_AHEAD - 1>();
+    x = lds_raw<CB>(mine + slot_now * (64 * CB)), y = lds_raw<CB>(mine + slot_now * (64 * CB) + 32 * CB);
+    slot_now = slot_now + 1 == RC_AHEAD ? 0 : slot_now + 1;
+  };
+  auto put = [&](const Raw<CB> &u, const Raw<CB> &z) {
+    if (to.left > 0) {
+      if (c0 >= 0) st_raw<CB>(to.at + c0 * E, u);
+      if (c1 >= 0) st_raw<CB>(to.at + c1 * E, z);
+    }
+    to.at += to.step, to.left -= hop;
+  };
+#pragma unroll 1
+  for (; kind < kinds; kind++) {
+    to = target(kind);
+    const T *const w = static_cast<const T *>(kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr);
+    if (kind == 2) {
+      while (to.left + hl > 0) {
+        Raw<CB> x, y;
+        take(x, y);
+        put(x, y);
+        fetch();
+      }
+      return;
+    }
+    if (to.left + hl <= 0) continue;
     // what f and g are multiplied by: f' = f ff + g gf, g' = f fg + g gg (halves); per chunk x' = x ff + swapped x gf (neighbours: chunk g has fg, gg)
     uint64_t ff[V], gf[V], fg[V], gg[V];
     unsigned turned = 0;  // BETWEEN: bit j: pair j of the first chunk turns; V + j: of the second
@@ -526,44 +555,45 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
         }
       }
     }
-    for (; r < end; r += RC_AHEAD * ch.split) {
-#pragma unroll
-      for (int i = 0; i < RC_AHEAD; i++) {
-        const int n = r + i * ch.split;
-        if (n >= end) break;
-        uint64_t f[V], g[V];
-        unpack<T, CB>(x[i], f), unpack<T, CB>(y[i], g);
-        if (n + RC_AHEAD * ch.split < end) fetch(d, n + RC_AHEAD * ch.split - base, x[i], y[i]);
-        if (w) {
-          uint64_t s0 = mul2(f[0], f[0]), s1 = mul2(g[0], g[0]);
-#pragma unroll
-          for (int j = 1; j < V; j++) s0 = fma2(f[j], f[j], s0), s1 = fma2(g[j], g[j], s1);
-          float ss = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
-          for (int o = ch.lg >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float inv = rsqrtf(ss * ch.over_d + a.eps);
-          const uint64_t inv2 = two(inv, inv);
-#pragma unroll
-          for (int j = 0; j < V; j++) f[j] = mul2(f[j], inv2), g[j] = mul2(g[j], inv2);
-        }
-        uint64_t u[V], z[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          if constexpr (BETWEEN) {
-            u[j] = mul2(f[j], ff[j]), z[j] = mul2(g[j], gg[j]);
-            if (turned >> j & 1) u[j] = fma2(two(hi(f[j]), lo(f[j])), gf[j], u[j]);
-            if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[j]), lo(g[j])), fg[j], z[j]);
-          } else {
-            u[j] = mul2(f[j], ff[j]), z[j] = mul2(g[j], gg[j]);
-            if (turns) u[j] = fma2(g[j], gf[j], u[j]), z[j] = fma2(f[j], fg[j], z[j]);
-          }
-        }
-        put(n, packed<T, CB>(u), packed<T, CB>(z));
+#pragma unroll 2
+    while (to.left + hl > 0) {
+      uint64_t f[V], g[V];
+      {
+        Raw<CB> x, y;
+        take(x, y);
+        unpack<T, CB>(x, f), unpack<T, CB>(y, g);
       }
+      if (w) {
+        if (c0 < 0)
+#pragma unroll
+          for (int j = 0; j < V; j++) f[j] = 0;
+        if (c1 < 0)
+#pragma unroll
+          for (int j = 0; j < V; j++) g[j] = 0;
+        uint64_t s0 = mul2(f[0], f[0]), s1 = mul2(g[0], g[0]);
+#pragma unroll
+        for (int j = 1; j < V; j++) s0 = fma2(f[j], f[j], s0), s1 = fma2(g[j], g[j], s1);
+        float ss = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
+        for (int o = ch.lg >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(ss * ch.over_d + a.eps);
+        const uint64_t inv2 = two(inv, inv);
+#pragma unroll
+        for (int j = 0; j < V; j++) f[j] = mul2(f[j], inv2), g[j] = mul2(g[j], inv2);
+      }
+      uint64_t u[V], z[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        u[j] = mul2(f[j], ff[j]), z[j] = mul2(g[j], gg[j]);
+        if constexpr (BETWEEN) {
+          if (turned >> j & 1) u[j] = fma2(two(hi(f[j]), lo(f[j])), gf[j], u[j]);
+          if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[j]), lo(g[j])), fg[j], z[j]);
+        } else if (turns) {
+          u[j] = fma2(g[j], gf[j], u[j]), z[j] = fma2(f[j], fg[j], z[j]);
+        }
+      }
+      put(packed<T, CB>(u), packed<T, CB>(z));
+      fetch();
     }
-    // the next kind's first rounds
-    r = base_of(++kind);
-    r += (part - r % ch.split + ch.split) % ch.split;
-    if (r < rounds) d = side_of(kind), ahead(kind);
   }
 }
 
@@ -666,9 +696,15 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
     const int lanes = p->interleaved ? ch.first : ch.first + (ch.count - 2 * ch.first + 1) / 2;
     for (ch.lg = 1; ch.lg < lanes;) ch.lg *= 2;
     if (ch.lg <= 32) {
-      // warps per token: until there are eight for every SM, each with a round of heads or more
-      const int per = 32 / ch.lg, rounds = (p->NH + per - 1) / per + (p->KH + per - 1) / per * (p->slots ? 2 : 1);
-      for (ch.split = 1; ch.split < rounds && p->T * ch.split < 8ll * sm_count();) ch.split++;
+      // Warps per token: one that has its angles for all heads, or, of fewer tokens than four for every SM, more with as many rounds of one kind
+      // each, until there are eight for every SM.
+      const int per = 32 / ch.lg, rq = (p->NH + per - 1) / per, rk = (p->KH + per - 1) / per, kinds = p->slots ? 3 : 2;
+      ch.split = 1, ch.q_parts = ch.k_parts = 0;
+      if (p->T < 4ll * sm_count())
+        for (int rounds = rk; rounds >= 1 && p->T * (ch.split > 1 ? ch.split : 0) < 8ll * sm_count(); rounds = rounds == 1 ? 0 : (rounds + 1) / 2) {
+          ch.q_parts = (rq + rounds - 1) / rounds, ch.k_parts = (rk + rounds - 1) / rounds;
+          ch.split = ch.q_parts + (kinds - 1) * ch.k_parts;
+        }
       const long long ctas = (p->T * ch.split + RC_WARPS - 1) / RC_WARPS;
       if (ctas <= 0x7fffffffll) return launch_chunks(a, ch, cb, p->dtype, (unsigned)ctas, st);
     }
