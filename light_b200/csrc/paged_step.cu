@@ -322,7 +322,7 @@ constexpr int RC_WARPS = 4, RC_AHEAD = 6;  // rounds of heads that are on their 
 
 struct Chunks {
   int lg, split, first, count;  // lanes per head, warps per token; chunks that a lane's second lies behind its first; chunks per head
-  int q_parts, k_parts;         // of several warps per token, those of the queries, and of the keys and of the values
+  int q_parts, k_parts;         // where a warp takes heads of one kind: warps of the queries, and of the keys and of the values
   float over_d;                 // 1 / D
 };
 
@@ -428,9 +428,10 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
   const long long id = (long long)blockIdx.x * RC_WARPS + warp, t = ch.split == 1 ? id : id / ch.split;
   if (t >= a.T) return;
   const int gl = lane & (ch.lg - 1), per = 32 / ch.lg, hl = lane / ch.lg;
-  // the kinds (queries, keys, values) of this warp and its part of their heads: all of a token, or with several warps per token one kind
-  int part = (int)(id - t * ch.split), parts = 1, kind = 0;
-  if (ch.split > 1) {
+  // the kinds (queries, keys, values) of this warp and its part of their heads: every kind, or with many warps per token one
+  int part = (int)(id - t * ch.split), parts = ch.split, kind = 0;
+  const bool one_kind = ch.q_parts > 0;
+  if (one_kind) {
     kind = part < ch.q_parts ? 0 : part < ch.q_parts + ch.k_parts ? 1 : 2, parts = kind == 0 ? ch.q_parts : ch.k_parts;
     part -= kind == 0 ? 0 : kind == 1 ? ch.q_parts : ch.q_parts + ch.k_parts;
   }
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     const long long *cs = kind == 1 ? a.ks : a.vs;
     return Walk{static_cast<T *>(kind == 1 ? a.k_out : a.v_out) + page * cs[0] + h0 * cs[1] + row * cs[2], hop * cs[1], left};
   };
-  const int kinds = min(a.slots ? (slot >= 0 ? 3 : 1) : 2, ch.split > 1 ? kind + 1 : 3);
+  const int kinds = min(a.slots ? (slot >= 0 ? 3 : 1) : 2, one_kind ? kind + 1 : 3);
   if (kind >= kinds) return;
   // a ring of rounds in shared memory: every lane copies and reads its own chunks, so nobody waits for anybody
   const uint32_t mine = umma::smem_u32(ring[warp]) + lane * CB;
@@ -555,44 +556,57 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
         }
       }
     }
-#pragma unroll 2
     while (to.left + hl > 0) {
-      uint64_t f[V], g[V];
-      {
-        Raw<CB> x, y;
-        take(x, y);
-        unpack<T, CB>(x, f), unpack<T, CB>(y, g);
+      // two rounds side by side, if the kind has two more: a round alone is a chain of some 400 cycles
+      const bool both = to.left + hl > hop;
+      uint64_t f[2][V], g[2][V];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        Raw<CB> x{}, y{};
+        if (i == 0 || both) take(x, y);
+        unpack<T, CB>(x, f[i]), unpack<T, CB>(y, g[i]);
       }
       if (w) {
-        if (c0 < 0)
+        float ss[2];
 #pragma unroll
-          for (int j = 0; j < V; j++) f[j] = 0;
-        if (c1 < 0)
+        for (int i = 0; i < 2; i++) {
 #pragma unroll
-          for (int j = 0; j < V; j++) g[j] = 0;
-        uint64_t s0 = mul2(f[0], f[0]), s1 = mul2(g[0], g[0]);
+          for (int j = 0; j < V; j++) f[i][j] = c0 < 0 ? 0 : f[i][j], g[i][j] = c1 < 0 ? 0 : g[i][j];  // (no chunk: the ring holds anything there)
+          uint64_t s0 = mul2(f[i][0], f[i][0]), s1 = mul2(g[i][0], g[i][0]);
 #pragma unroll
-        for (int j = 1; j < V; j++) s0 = fma2(f[j], f[j], s0), s1 = fma2(g[j], g[j], s1);
-        float ss = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
-        for (int o = ch.lg >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss * ch.over_d + a.eps);
-        const uint64_t inv2 = two(inv, inv);
+          for (int j = 1; j < V; j++) s0 = fma2(f[i][j], f[i][j], s0), s1 = fma2(g[i][j], g[i][j], s1);
+          ss[i] = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
+        }
+        for (int o = ch.lg >> 1; o > 0; o >>= 1) {
+          const float p = __shfl_xor_sync(0xffffffffu, ss[0], o), q = __shfl_xor_sync(0xffffffffu, ss[1], o);
+          ss[0] += p, ss[1] += q;
+        }
 #pragma unroll
-        for (int j = 0; j < V; j++) f[j] = mul2(f[j], inv2), g[j] = mul2(g[j], inv2);
-      }
-      uint64_t u[V], z[V];
+        for (int i = 0; i < 2; i++) {
+          const float inv = rsqrtf(ss[i] * ch.over_d + a.eps);
+          const uint64_t inv2 = two(inv, inv);
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        u[j] = mul2(f[j], ff[j]), z[j] = mul2(g[j], gg[j]);
-        if constexpr (BETWEEN) {
-          if (turned >> j & 1) u[j] = fma2(two(hi(f[j]), lo(f[j])), gf[j], u[j]);
-          if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[j]), lo(g[j])), fg[j], z[j]);
-        } else if (turns) {
-          u[j] = fma2(g[j], gf[j], u[j]), z[j] = fma2(f[j], fg[j], z[j]);
+          for (int j = 0; j < V; j++) f[i][j] = mul2(f[i][j], inv2), g[i][j] = mul2(g[i][j], inv2);
         }
       }
-      put(packed<T, CB>(u), packed<T, CB>(z));
-      fetch();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        uint64_t u[V], z[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          u[j] = mul2(f[i][j], ff[j]), z[j] = mul2(g[i][j], gg[j]);
+          if constexpr (BETWEEN) {
+            if (turned >> j & 1) u[j] = fma2(two(hi(f[i][j]), lo(f[i][j])), gf[j], u[j]);
+            if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[i][j]), lo(g[i][j])), fg[j], z[j]);
+          } else if (turns) {
+            u[j] = fma2(g[i][j], gf[j], u[j]), z[j] = fma2(f[i][j], fg[j], z[j]);
+          }
+        }
+        if (i == 0 || both) {
+          put(packed<T, CB>(u), packed<T, CB>(z));
+          fetch();
+        }
+      }
     }
   }
 }
@@ -696,12 +710,12 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
     const int lanes = p->interleaved ? ch.first : ch.first + (ch.count - 2 * ch.first + 1) / 2;
     for (ch.lg = 1; ch.lg < lanes;) ch.lg *= 2;
     if (ch.lg <= 32) {
-      // Warps per token: one that has its angles for all heads, or, of fewer tokens than four for every SM, more with as many rounds of one kind
-      // each, until there are eight for every SM.
+      // Warps per token: one that has its angles for all heads; two, of fewer than twelve tokens for every SM (1037 tokens of 48 F32 heads: 13.2 ->
+      // 9.7 us); of fewer than four, as many as have one to four rounds of one kind each, until there are eight for every SM.
       const int per = 32 / ch.lg, rq = (p->NH + per - 1) / per, rk = (p->KH + per - 1) / per, kinds = p->slots ? 3 : 2;
-      ch.split = 1, ch.q_parts = ch.k_parts = 0;
+      ch.split = p->T < 12ll * sm_count() ? 2 : 1, ch.q_parts = ch.k_parts = 0;
       if (p->T < 4ll * sm_count())
-        for (int rounds = rk; rounds >= 1 && p->T * (ch.split > 1 ? ch.split : 0) < 8ll * sm_count(); rounds = rounds == 1 ? 0 : (rounds + 1) / 2) {
+        for (int rounds = rk; rounds >= 1 && p->T * (ch.q_parts ? ch.split : 0) < 8ll * sm_count(); rounds = rounds == 1 ? 0 : (rounds + 1) / 2) {
           ch.q_parts = (rq + rounds - 1) / rounds, ch.k_parts = (rk + rounds - 1) / rounds;
           ch.split = ch.q_parts + (kinds - 1) * ch.k_parts;
         }
