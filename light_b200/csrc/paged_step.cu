@@ -14,9 +14,10 @@ __device__ unsigned int g_step_status = 0;
 // the stack does not hold gets none, and as first_b never falls, none after it that needs any.  Token i of the batch belongs to the
 // request with starts_b <= i < starts_{b + 1}: a binary search in shared memory.
 //
-// Two dependent reads (the lengths; then the stack or the table) and the stores bound it; the work is one cluster's: every CTA of it scans
-// the lengths for itself, and the barrier between the scan and the stores lets lengths and counter be updated in place.
-constexpr int PG_THREADS = 1024, PG_MAX_B = 8192;
+// Two dependent reads (the lengths; then the stack or the table) and the stores bound it: latency.  Every CTA scans the lengths for itself and
+// stores its share.  Where lengths and counter are updated in place the CTAs are one cluster, with its barrier between the scan and the
+// stores; else any number of them.
+constexpr int PG_THREADS = 1024, PG_MAX_B = LB200_PAGED_MAX_REQUESTS, PG_AHEAD = 4;  // entries of a thread that are on their way together
 
 struct PagesArgs {
   int *table;
@@ -48,13 +49,16 @@ __device__ __forceinline__ Two block_scan(Two v, Two &total) {
   __syncthreads();  // (part may still be read from the call before)
   if (lane == 31) part[warp] = x;
   __syncthreads();
-  Two before = {0, 0}, all = {0, 0};
-  for (int w = 0; w < (int)blockDim.x / 32; w++) {
-    if (w < warp) before.a += part[w].a, before.b += part[w].b;
-    all.a += part[w].a, all.b += part[w].b;
+  Two w = lane < (int)blockDim.x / 32 ? part[lane] : Two{0, 0};  // the warps' sums, summed by every warp
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, w.a, o), b = __shfl_up_sync(0xffffffffu, w.b, o);
+    if (lane >= o) w.a += a, w.b += b;
   }
-  total = all;
-  return {before.a + x.a - v.a, before.b + x.b - v.b};
+  total = {__shfl_sync(0xffffffffu, w.a, 31), __shfl_sync(0xffffffffu, w.b, 31)};
+  const int upto = max(warp - 1, 0);
+  const Two before = {__shfl_sync(0xffffffffu, w.a, upto), __shfl_sync(0xffffffffu, w.b, upto)};
+  return {(warp ? before.a : 0) + x.a - v.a, (warp ? before.b : 0) + x.b - v.b};
 }
 
 // the b with at[b] <= i < at[b + 1], for at[0] = 0 <= i < at[n]
@@ -70,107 +74,123 @@ __device__ __forceinline__ int owner_of(const int *at, int n, int i) {
 
 __device__ __forceinline__ int saturated(long long v) { return (int)(v < 0x7fffffffll ? v : 0x7fffffffll); }
 
-__global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, int ctas) {
+// all CTAs have read what the stores may overwrite
+__device__ __forceinline__ void pages_barrier(bool cluster) {
+  if (cluster) umma::cluster_sync();
+  else __syncthreads();
+}
+
+__global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, bool cluster) {
   extern __shared__ int sm[];
+  __shared__ int cut;
   int *starts = sm, *first = sm + a.B + 1, *len = first + a.B + 1;  // len: -1 - n for a request that gets nothing
   pdl_launch_dependents();
   pdl_wait();
-  const int rank = blockIdx.x, tid = threadIdx.x;
+  const int rank = blockIdx.x, tid = threadIdx.x, P = a.page.d;
   const int free_now = a.free_count[0], avail = min(max(free_now, 0), a.capacity);
   bool odd = free_now != avail;
+  if (tid == 0) cut = 0x7fffffff;
+  auto held_of = [&](int n) {
+    const int q = a.page.div(n);
+    return q + (q * P < n);
+  };
   Two carry = {0, 0};
-  long long taken = 0;
   for (int base = 0; base < a.B; base += blockDim.x) {
     const int b = base + tid;
-    long long n = 0, m = 0, more = 0;
+    int n = 0, m = 0, more = 0;
+    bool fits = false;
     if (b < a.B) {
-      const int n0 = a.lens[b], m0 = a.new_lens[b];
-      odd |= n0 < 0 || m0 < 0;
-      n = max(n0, 0), m = max(m0, 0);
+      n = a.lens[b], m = a.new_lens[b];
+      odd |= n < 0 || m < 0;
+      n = max(n, 0), m = max(m, 0), fits = (long long)n + m <= (long long)a.W * P;
+      if (fits) more = held_of(n + m) - held_of(n);
     }
-    Two total, at = block_scan({m, 0}, total);
-    const long long from = carry.a + at.a;
-    const bool fits = n + m <= (long long)a.W * a.page.d && from + m <= a.tokens;
-    if (b < a.B && fits) {
-      const int held = a.page.div((int)n + 0) + (a.page.div((int)n) * a.page.d < (int)n), want = a.page.div((int)(n + m)) + (a.page.div((int)(n + m)) * a.page.d < (int)(n + m));
-      more = want - held;
-    }
-    Two total2, at2 = block_scan({more, 0}, total2);
-    const long long f = carry.b + at2.a;
-    const bool given = fits && (more == 0 || f + more <= avail);
+    // (A request whose rows pass `tokens` counts in the sums: so do all after it, of which none can have a token, or so a page.)
+    Two total, at = block_scan({m, more}, total);
     if (b < a.B) {
-      starts[b] = saturated(from), first[b] = saturated(f), len[b] = given ? (int)n : -1 - (int)n;
+      const long long from = carry.a + at.a, f = carry.b + at.b;
+      const bool given = fits && from + m <= a.tokens && (more == 0 || f + more <= avail);
+      starts[b] = saturated(from), first[b] = saturated(f), len[b] = given ? n : -1 - n;
       odd |= !given;
+      if (!given && more > 0) atomicMin(&cut, saturated(f));  // (a minimum: no order)
     }
-    carry.a += total.a, carry.b += total2.a;
+    carry.a += total.a, carry.b += total.b;
   }
   if (tid == 0) starts[a.B] = saturated(carry.a), first[a.B] = saturated(carry.b);
-  __syncthreads();
-  // pages taken: those of the requests before the first that does not get its own
-  int cut = saturated(carry.b);
-  for (int b = tid; b < a.B; b += blockDim.x)
-    if (len[b] < 0 && first[b + 1] > first[b]) cut = min(cut, first[b]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) cut = min(cut, __shfl_xor_sync(0xffffffffu, cut, o));
-  __shared__ int least;
-  if (tid == 0) least = 0x7fffffff;
-  __syncthreads();
-  if ((tid & 31) == 0) atomicMin(&least, cut);
-  if (ctas > 1) umma::cluster_sync();  // every CTA has read the lengths and the counter
-  else __syncthreads();
-  taken = least;
+  pages_barrier(cluster);
+  const int taken = min(cut, first[a.B]);  // pages: those of the requests before the first that does not get its own
   if (odd && rank == 0) atomicOr(&g_step_status, (unsigned)PAGED_REFUSED);
 
-  const int gid = rank * blockDim.x + tid, threads = ctas * blockDim.x;
+  const int gid = rank * blockDim.x + tid, threads = gridDim.x * blockDim.x;
   for (int b = gid; b < a.B; b += threads) {
     const int l = len[b], m = starts[b + 1] - starts[b];
     a.lens_out[b] = l < 0 ? -1 - l : l + m;
     a.granted[b] = l < 0 ? 0 : m;
     a.starts[b] = starts[b];
   }
-  if (gid == 0) a.starts[a.B] = starts[a.B], a.count_out[0] = avail - (int)taken;
-  auto held_of = [&](int b) {
-    const int n = len[b] < 0 ? -1 - len[b] : len[b], q = a.page.div(n);
-    return q + (q * a.page.d < n);
-  };
-  for (int p = gid; p < (int)taken; p += threads) {
-    const int b = owner_of(first, a.B, p);
-    a.table[(long long)b * a.table_stride + held_of(b) + (p - first[b])] = a.free_pages[avail - 1 - p];
-  }
+  if (gid == 0) a.starts[a.B] = starts[a.B], a.count_out[0] = avail - taken;
   const int given_rows = starts[a.B];
-  for (long long i = gid; i < a.tokens; i += threads) {
-    long long pos = 0, slot = -1;
-    if (i < given_rows) {
-      const int b = owner_of(starts, a.B, (int)i), l = len[b];
-      pos = (long long)(l < 0 ? -1 - l : l) + (int)i - starts[b];
-      if (l >= 0) {
-        const int w = a.page.div((int)pos), x = w - held_of(b);
-        const int pg = x >= 0 ? a.free_pages[avail - 1 - first[b] - x] : a.table[(long long)b * a.table_stride + w];
-        if (pg >= 0) slot = (long long)pg * a.page.d + ((int)pos - w * a.page.d);
+  for (long long i0 = gid; i0 < a.tokens; i0 += PG_AHEAD * (long long)threads) {
+    int pg[PG_AHEAD], in[PG_AHEAD];
+    long long pos[PG_AHEAD];
+#pragma unroll
+    for (int j = 0; j < PG_AHEAD; j++) {
+      const long long i = i0 + j * (long long)threads;
+      pg[j] = -1, pos[j] = 0, in[j] = 0;
+      if (i < given_rows && i < a.tokens) {
+        const int b = owner_of(starts, a.B, (int)i), l = len[b], n = l < 0 ? -1 - l : l;
+        pos[j] = (long long)n + ((int)i - starts[b]);
+        if (l >= 0) {
+          const int w = a.page.div((int)pos[j]), x = w - held_of(n);
+          in[j] = (int)pos[j] - w * P;
+          pg[j] = x >= 0 ? a.free_pages[avail - 1 - first[b] - x] : a.table[(long long)b * a.table_stride + w];
+        }
       }
     }
-    a.positions[i] = pos, a.slots[i] = slot;
+#pragma unroll
+    for (int j = 0; j < PG_AHEAD; j++) {
+      const long long i = i0 + j * (long long)threads;
+      if (i < a.tokens) a.positions[i] = pos[j], a.slots[i] = pg[j] >= 0 ? (long long)pg[j] * P + in[j] : -1;
+    }
+  }
+  for (int p0 = gid; p0 < taken; p0 += PG_AHEAD * threads) {  // (after the tokens: their first pages are not among these)
+    int pg[PG_AHEAD];
+#pragma unroll
+    for (int j = 0; j < PG_AHEAD; j++)
+      if (p0 + j * threads < taken) pg[j] = a.free_pages[avail - 1 - (p0 + j * threads)];
+#pragma unroll
+    for (int j = 0; j < PG_AHEAD; j++) {
+      const int p = p0 + j * threads;
+      if (p < taken) {
+        const int b = owner_of(first, a.B, p), l = len[b];
+        a.table[(long long)b * a.table_stride + held_of(l < 0 ? -1 - l : l) + (p - first[b])] = pg[j];
+      }
+    }
   }
 }
 
 // The pages of the requests marked done, in order, on top of the stack.
-__global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, int ctas) {
+__global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, bool cluster) {
   extern __shared__ int sm[];
-  int *first = sm;
+  int *first = sm, *keep = sm + a.B + 1;
   pdl_launch_dependents();
   pdl_wait();
   const int rank = blockIdx.x, tid = threadIdx.x;
   const int free_now = a.free_count[0], avail = min(max(free_now, 0), a.capacity);
   bool odd = free_now != avail;
   long long carry = 0;
-  // a request's length and mark are read and written by the same threads: position b % threads of every CTA reads, one of them writes after the barrier
   for (int base = 0; base < a.B; base += blockDim.x) {
     const int b = base + tid;
-    long long held = 0;
-    if (b < a.B && a.done[b]) {
-      const int n = a.lens[b], q = a.page.div(max(n, 0));
-      odd |= n < 0;
-      held = min(q + (q * a.page.d < n), a.W);
+    int held = 0;
+    if (b < a.B) {
+      const int n = a.lens[b];
+      const bool done = a.done[b];
+      keep[b] = done ? 0 : n;
+      if (done) {
+        const int q = a.page.div(max(n, 0));
+        odd |= n < 0;
+        held = min(q + (q * a.page.d < n), a.W);
+      }
     }
     Two total, at = block_scan({held, 0}, total);
     if (b < a.B) first[b] = saturated(carry + at.a);
@@ -179,42 +199,54 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, 
   if (tid == 0) first[a.B] = saturated(carry);
   const int total = (int)min(carry, (long long)(a.capacity - avail));
   odd |= total < carry;
-  constexpr int OWN = (PG_MAX_B + PG_THREADS - 1) / PG_THREADS;
-  int keep[OWN];
-#pragma unroll
-  for (int i = 0; i < OWN; i++) {
-    const int b = (i * ctas + rank) * (int)blockDim.x + tid;
-    keep[i] = b < a.B ? (a.done[b] ? 0 : a.lens[b]) : 0;
-  }
-  if (ctas > 1) umma::cluster_sync();
-  else __syncthreads();
+  pages_barrier(cluster);
   if (odd && rank == 0) atomicOr(&g_step_status, (unsigned)PAGED_REFUSED);
-  const int gid = rank * blockDim.x + tid, threads = ctas * blockDim.x;
-#pragma unroll
-  for (int i = 0; i < OWN; i++) {
-    const int b = (i * ctas + rank) * (int)blockDim.x + tid;
-    if (b < a.B) a.lens_out[b] = keep[i];
-  }
+  const int gid = rank * blockDim.x + tid, threads = gridDim.x * blockDim.x;
+  for (int b = gid; b < a.B; b += threads) a.lens_out[b] = keep[b];
   if (gid == 0) a.count_out[0] = avail + total;
-  for (int p = gid; p < total; p += threads) {
-    const int b = owner_of(first, a.B, p);
-    a.free_pages[avail + p] = a.table[(long long)b * a.table_stride + (p - first[b])];
+  for (long long p0 = gid; p0 < total; p0 += PG_AHEAD * (long long)threads) {
+    int pg[PG_AHEAD];
+#pragma unroll
+    for (int j = 0; j < PG_AHEAD; j++) {
+      const long long p = p0 + j * (long long)threads;
+      if (p < total) {
+        const int b = owner_of(first, a.B, (int)p);
+        pg[j] = a.table[(long long)b * a.table_stride + ((int)p - first[b])];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PG_AHEAD; j++) {
+      const long long p = p0 + j * (long long)threads;
+      if (p < total) a.free_pages[avail + p] = pg[j];
+    }
   }
 }
 
-int launch_pages(void (*kern)(PagesArgs, int), const PagesArgs &a, size_t smem, bool many, cudaStream_t st, DeviceOnce &once, const char *what) {
-  cudaError_t e = once.ensure([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (PG_MAX_B * 3 + 2) * 4); });
+// `work`: entries at most, beside the requests
+int launch_pages(void (*kern)(PagesArgs, bool), const PagesArgs &a, size_t smem, long long work, cudaStream_t st, DeviceOnce &once, const char *what) {
+  cudaError_t e = once.ensure([&] {
+    const cudaError_t f = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (PG_MAX_B * 3 + 2) * 4);
+  });
   if (e != cudaSuccess) return fail((int)e, "light_b200: %s: %s", what, cudaGetErrorString(e));
-  const int ctas = many ? 8 : 1;
+  // as many threads as there are requests or entries, and CTAs where that is more than one's, up to what one cluster or the GPU holds
+  const bool inplace = a.lens_out == a.lens || a.count_out == a.free_count;
+  const long long want = work > a.B ? work : a.B;
+  const int threads = want >= PG_THREADS ? PG_THREADS : (int)((want + 31) / 32 * 32 < 128 ? 128 : (want + 31) / 32 * 32);
+  long long ctas = (work + 2 * PG_THREADS - 1) / (2 * PG_THREADS), most = inplace ? 16 : sm_count();
+  ctas = ctas < 1 ? 1 : ctas > most ? most : ctas;
+  if (inplace)
+    while (ctas & (ctas - 1)) ctas &= ctas - 1;  // (a power of two)
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3(PG_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = (unsigned)ctas, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
-  cfg.attrs = at, cfg.numAttrs = many ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, a, ctas);
+  const bool cluster = inplace && ctas > 1;
+  cfg.attrs = at, cfg.numAttrs = cluster ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, a, cluster);
   if (e != cudaSuccess) return fail((int)e, "light_b200: %s: %s", what, cudaGetErrorString(e));
   return launched(what);
 }
@@ -639,12 +671,13 @@ static PagesArgs pages_args(const lb200_paged_pages *p) {
 
 int paged_advance(const lb200_paged_pages *p, cudaStream_t st) {
   static DeviceOnce once;
-  return launch_pages(paged_advance_kernel, pages_args(p), (size_t)(3 * p->B + 2) * 4, p->tokens > 4096, st, once, "paged_advance");
+  return launch_pages(paged_advance_kernel, pages_args(p), (size_t)(3 * p->B + 2) * 4, p->tokens, st, once, "paged_advance");
 }
 
 int paged_release(const lb200_paged_pages *p, cudaStream_t st) {
   static DeviceOnce once;
-  return launch_pages(paged_release_kernel, pages_args(p), (size_t)(p->B + 1) * 4, true, st, once, "paged_release");
+  const long long pages = (long long)p->B * p->W;
+  return launch_pages(paged_release_kernel, pages_args(p), (size_t)(2 * p->B + 1) * 4, pages < p->capacity ? pages : p->capacity, st, once, "paged_release");
 }
 
 int qk_norm_rope_check(const lb200_qk_norm_rope_args *p) {
