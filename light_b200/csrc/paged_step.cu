@@ -537,8 +537,7 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     __syncwarp();
   }
   Walk to;
-  auto take = [&](Raw<CB> &x, Raw<CB> &y) {
-    cp_async_wait<RC_AHEAD - 1>();
+  auto take = [&](Raw<CB> &x, Raw<CB> &y) {  // (its copies have been waited for)
     x = lds_raw<CB>(mine + slot_now * (64 * CB)), y = lds_raw<CB>(mine + slot_now * (64 * CB) + 32 * CB);
     slot_now = slot_now + 1 == RC_AHEAD ? 0 : slot_now + 1;
   };
@@ -556,6 +555,7 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     if (kind == 2) {
       while (to.left + hl > 0) {
         Raw<CB> x, y;
+        cp_async_wait<RC_AHEAD - 1>();
         take(x, y);
         put(x, y);
         fetch();
@@ -591,6 +591,8 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     while (to.left + hl > 0) {
       // two rounds side by side, if the kind has two more: a round alone is a chain of some 400 cycles
       const bool both = to.left + hl > hop;
+      if (both) cp_async_wait<RC_AHEAD - 2>();
+      else cp_async_wait<RC_AHEAD - 1>();
       uint64_t f[2][V], g[2][V];
 #pragma unroll
       for (int i = 0; i < 2; i++) {

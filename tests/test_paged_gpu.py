@@ -257,6 +257,32 @@ def test_rotation_sizes(cuda, dtype, T, NH, KH):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,NH,KH,D", [(700, 32, 8, 128), (2000, 24, 8, 128), (5000, 32, 8, 128), (4000, 28, 4, 80), (3000, 16, 2, 256)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_of_prompts_from_cold_memory(cuda, dtype, T, NH, KH, D, interleaved):
+    """Many rounds of heads per warp, all of them from memory: what arrives late must be waited for."""
+    g = torch.Generator(cuda).manual_seed(T)
+    qkv = torch.randn((T, (NH + 2 * KH) * D), generator=g, device=cuda).to(dtype)
+    q, k, v = (x.unflatten(1, (-1, D)) for x in qkv.split((NH * D, KH * D, KH * D), 1))
+    w = (1 + 0.2 * torch.randn(D, generator=g, device=cuda)).to(dtype)
+    freq, _ = ops.RoPEFrequencies(D, 500000.0)
+    positions = torch.arange(T, device=cuda)
+    pages = T // 16 + 1
+    kc, vc = (torch.zeros((pages, KH, 16, D), dtype=dtype, device=cuda) for _ in range(2))
+    slots = torch.randperm(pages * 16, generator=g, device=cuda)[:T].contiguous()
+    flush = torch.zeros(1 << 26, device=cuda)
+    for _ in range(3):
+        flush.add_(1)
+        got, _ = ops.QKNormRoPE(q, k, positions, freq, q_weight=w, k_weight=w, interleaved=interleaved, v=v, k_cache=kc, v_cache=vc, slots=slots)
+        want, bound = paged_plain.rotated(q, w, 1e-6, positions, freq, interleaved, 1.0)
+        assert bool(((got.double() - want).abs() <= bound).all())
+        want, bound = paged_plain.rotated(k, w, 1e-6, positions, freq, interleaved, 1.0)
+        assert bool(((kc[slots // 16, :, slots % 16].double() - want).abs() <= bound).all())
+        assert torch.equal(vc[slots // 16, :, slots % 16], v)
+        kc.zero_(), vc.zero_()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rotation_odd_addresses_and_orders(cuda, dtype):
     """Heads off 16 bytes, elements apart, one key for all tokens, weights in the middle of a tensor; a zero row stays zero."""
     g = torch.Generator(cuda).manual_seed(5)
