@@ -67,8 +67,10 @@ static int bind(int device) {
 struct OnDevice {
   int before = -1, rc;
   explicit OnDevice(int device) {
-    if (cudaGetDevice(&before) != cudaSuccess || before == device) before = -1;
-    rc = bind(device);
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    const bool here = before >= 0 && before == device;
+    if (here) before = -1;
+    rc = here && device < 64 && g_ready[device] ? 0 : bind(device);
   }
   ~OnDevice() {
     if (before >= 0) cudaSetDevice(before);

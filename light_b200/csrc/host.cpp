@@ -309,6 +309,13 @@ PyObject *moe_gemm(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
 }
 
 // ---- many sequences over one paged cache
+// A contiguous tensor in the memory of `whole`, `at` bytes in (outputs that come together, from one allocation).
+at::Tensor piece(const at::Tensor &whole, int64_t at, at::IntArrayRef sizes, at::ScalarType dt) {
+  auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(dt));
+  t->set_sizes_contiguous(sizes);
+  t->set_storage_offset(at / (int64_t)c10::elementSize(dt));
+  return at::Tensor(std::move(t));
+}
 bool i32_of(const at::Tensor &t, int dev, int64_t n) {  // a contiguous I32 tensor of n elements
   return t.is_cuda() && t.scalar_type() == at::kInt && t.is_contiguous() && t.get_device() == dev && t.numel() == n;
 }
@@ -351,9 +358,11 @@ PyObject *paged_advance(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const int64_t B = t.t->size(0), W = t.t->size(1), cap = f.t->numel();
   NEED(i32_of(*l.t, dev, B) && i32_of(*n.t, dev, B) && i32_of(*c.t, dev, 1) && f.t->dim() == 1 && cap > 0 && cap < (1ll << 31) && i32_of(*f.t, dev, cap));
   NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31) && tokens >= 0);
-  const auto i32 = l.t->options(), i64 = i32.dtype(at::kLong);
-  at::Tensor pos = at::empty({tokens}, i64), slots = at::empty({tokens}, i64), starts = at::empty({B + 1}, i32), granted = at::empty({B}, i32);
-  at::Tensor lens = inplace ? *l.t : at::empty({B}, i32), count = inplace ? *c.t : at::empty({1}, i32);
+  const at::Tensor whole = at::empty({16 * tokens + 4 * (3 * B + 2)}, l.t->options().dtype(at::kByte));
+  const int64_t ints = 16 * tokens;
+  at::Tensor pos = piece(whole, 0, {tokens}, at::kLong), slots = piece(whole, 8 * tokens, {tokens}, at::kLong);
+  at::Tensor starts = piece(whole, ints, {B + 1}, at::kInt), granted = piece(whole, ints + 4 * (B + 1), {B}, at::kInt);
+  at::Tensor lens = inplace ? *l.t : piece(whole, ints + 4 * (2 * B + 1), {B}, at::kInt), count = inplace ? *c.t : piece(whole, ints + 4 * (3 * B + 1), {1}, at::kInt);
   lb200_paged_pages p{};
   p.block_table = t.t->data_ptr<int>(), p.lens = l.t->const_data_ptr<int>(), p.new_lens = n.t->const_data_ptr<int>(), p.free_pages = f.t->data_ptr<int>();
   p.free_count = c.t->const_data_ptr<int>(), p.lens_out = lens.data_ptr<int>(), p.granted = granted.data_ptr<int>(), p.starts = starts.data_ptr<int>();
@@ -378,7 +387,11 @@ PyObject *paged_release(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   NEED(i32_of(*l.t, dev, B) && i32_of(*c.t, dev, 1) && f.t->dim() == 1 && cap > 0 && cap < (1ll << 31) && i32_of(*f.t, dev, cap) && d.t->is_cuda() && d.t->is_contiguous() &&
        d.t->scalar_type() == at::kBool && d.t->numel() == B && d.t->get_device() == dev);
   NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31));
-  at::Tensor lens = inplace ? *l.t : at::empty({B}, l.t->options()), count = inplace ? *c.t : at::empty({1}, l.t->options());
+  at::Tensor lens = *l.t, count = *c.t;
+  if (!inplace) {
+    const at::Tensor whole = at::empty({B + 1}, l.t->options());
+    lens = piece(whole, 0, {B}, at::kInt), count = piece(whole, 4 * B, {1}, at::kInt);
+  }
   lb200_paged_pages p{};
   p.block_table = t.t->data_ptr<int>(), p.lens = l.t->const_data_ptr<int>(), p.done = (const uint8_t *)d.t->const_data_ptr(), p.free_pages = f.t->data_ptr<int>();
   p.free_count = c.t->const_data_ptr<int>(), p.lens_out = lens.data_ptr<int>(), p.free_count_out = count.data_ptr<int>();

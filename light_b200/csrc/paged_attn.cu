@@ -303,7 +303,7 @@ struct MmaBlock {
   }
 };
 
-// f32: a block of 8 keys, f32 products.  For the scores a lane has a key and a quarter of its chunks (the queries are broadcasts from shared
+// f32: a block of 8 keys, f32 products, two to an instruction (f32x2).  For the scores a lane has a key and a quarter of its chunks (the queries are broadcasts from shared
 // memory); the four lanes of a key hand each other halves of their heads until each has its own complete.  The weights go through
 // shared memory, and for the values a lane owns chunks of dims (of 64 dims: and every other key).
 template <int DP_, int GH>
@@ -311,8 +311,9 @@ struct F32Block {
   using T = float;
   static constexpr int DP = DP_, KB = 8, HEADS = GH, ROWB = DP * 4, PR = DP + 4;
   static constexpr int OWN = GH < 4 ? 1 : GH / 4, NC = DP < 128 ? 1 : DP / 128, SPLIT = DP < 128 ? 128 / DP : 1;  // heads of a lane; chunks; keys side by side
-  static constexpr int QS = GH * DP * 4, PS = (KB * GH * 4 + GH * 4 + 15) / 16 * 16, EXTRA = QS + PS;  // of a warp: queries | weights, corrections
-  float acc[GH][NC][4], m[OWN], l[OWN];
+  static constexpr int QS = GH * DP * 4, PS = (KB * GH * 8 + GH * 4 + 15) / 16 * 16, EXTRA = QS + PS;  // of a warp: queries | weights (twice each), corrections
+  uint64_t acc[GH][NC][2];
+  float m[OWN], l[OWN];
 
   __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *extra) {
     const PagedArgs &a = s.p;
@@ -330,9 +331,7 @@ struct F32Block {
 #pragma unroll
     for (int h = 0; h < GH; h++)
 #pragma unroll
-      for (int i = 0; i < NC; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[h][i][e] = 0.f;
+      for (int i = 0; i < NC; i++) acc[h][i][0] = acc[h][i][1] = 0;
   }
 
   __device__ __forceinline__ static int first_head(int lane) { return GH >= 4 ? (lane & 2 ? GH / 2 : 0) + (lane & 1 ? GH / 4 : 0) : GH == 2 ? lane >> 1 & 1 : 0; }
@@ -340,23 +339,27 @@ struct F32Block {
   __device__ __forceinline__ void block(const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *extra) {
     const int lane = threadIdx.x & 31, key = lane >> 2, qd = lane & 3;
     const float *qs = reinterpret_cast<const float *>(extra);
-    float *ps = reinterpret_cast<float *>(extra + QS), *cs = ps + KB * GH;
-    float d[GH];
+    float2 *ps = reinterpret_cast<float2 *>(extra + QS);
+    float *cs = reinterpret_cast<float *>(ps + KB * GH);
+    uint64_t d2[GH];
 #pragma unroll
-    for (int h = 0; h < GH; h++) d[h] = 0.f;
+    for (int h = 0; h < GH; h++) d2[h] = 0;
     const uint32_t krow = kbase + key * ROWB;
     const int turn = spread(key);
 #pragma unroll
     for (int i = 0; i < DP / 16; i++) {
       const int c = qd + 4 * i;
       const uint4 w = lds128(krow + ((c ^ turn) << 4));
-      const float4 k = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+      const uint64_t k0 = (uint64_t)w.y << 32 | w.x, k1 = (uint64_t)w.w << 32 | w.z;
 #pragma unroll
       for (int h = 0; h < GH; h++) {
-        const float4 q = *reinterpret_cast<const float4 *>(qs + h * DP + 4 * c);
-        d[h] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, d[h]))));
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(qs + h * DP + 4 * c);
+        d2[h] = fma2(q.x, k0, fma2(q.y, k1, d2[h]));
       }
     }
+    float d[GH];
+#pragma unroll
+    for (int h = 0; h < GH; h++) d[h] = lo(d2[h]) + hi(d2[h]);
     int cnt = GH;
 #pragma unroll
     for (int x = 2; x >= 1; x >>= 1) {
@@ -386,51 +389,55 @@ struct F32Block {
       const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(m[i] - use), p = ex2(s - use);
       same = same && mx == m[i];
       m[i] = mx, l[i] = fmaf(l[i], corr, p);
-      ps[key * GH + h0 + i] = p;
+      ps[key * GH + h0 + i] = make_float2(p, p);
       if (key == 0) cs[h0 + i] = corr;
     }
     __syncwarp();
     if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
       for (int h = 0; h < GH; h++) {
-        const float c = cs[h];
+        const uint64_t c = two(cs[h], cs[h]);
 #pragma unroll
-        for (int i = 0; i < NC; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[h][i][e] *= c;
+        for (int i = 0; i < NC; i++) acc[h][i][0] = mul2(acc[h][i][0], c), acc[h][i][1] = mul2(acc[h][i][1], c);
       }
     }
     constexpr int LANES = 32 / SPLIT;  // of a row
 #pragma unroll
     for (int k0 = 0; k0 < KB; k0 += SPLIT) {
       const int k = k0 + lane / LANES;
-      float p[GH];
-      if constexpr (GH >= 4) {
+      uint64_t p[GH];
+      if constexpr (GH >= 2) {
 #pragma unroll
-        for (int h = 0; h < GH; h += 4) {
-          const float4 x = *reinterpret_cast<const float4 *>(ps + k * GH + h);
-          p[h] = x.x, p[h + 1] = x.y, p[h + 2] = x.z, p[h + 3] = x.w;
+        for (int h = 0; h < GH; h += 2) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(ps + k * GH + h);
+          p[h] = x.x, p[h + 1] = x.y;
         }
       } else {
-#pragma unroll
-        for (int h = 0; h < GH; h++) p[h] = ps[k * GH + h];
+        p[0] = *reinterpret_cast<const uint64_t *>(ps + k);
       }
 #pragma unroll
       for (int i = 0; i < NC; i++) {
         const int c = lane % LANES + 32 * i;
         const uint4 w = lds128(kbase + (KB + k) * ROWB + ((c ^ spread(k)) << 4));
-        const float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
+        const uint64_t v0 = (uint64_t)w.y << 32 | w.x, v1 = (uint64_t)w.w << 32 | w.z;
 #pragma unroll
-        for (int h = 0; h < GH; h++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[h][i][e] = fmaf(p[h], v[e], acc[h][i][e]);
+        for (int h = 0; h < GH; h++) acc[h][i][0] = fma2(p[h], v0, acc[h][i][0]), acc[h][i][1] = fma2(p[h], v1, acc[h][i][1]);
       }
     }
+  }
+  // the four dims of a chunk, of all lanes that have some of its keys
+  __device__ __forceinline__ float4 dims(int h, int i) const {
+    float v[4] = {lo(acc[h][i][0]), hi(acc[h][i][0]), lo(acc[h][i][1]), hi(acc[h][i][1])};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+      for (int x = 32 / SPLIT; x < 32; x <<= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], x);
+    return make_float4(v[0], v[1], v[2], v[3]);
   }
 
   __device__ __forceinline__ void write(float *out, int count, int D, unsigned char *extra) {
     const int lane = threadIdx.x & 31, h0 = first_head(lane);
-    float *cs = reinterpret_cast<float *>(extra + QS) + KB * GH;
+    float *cs = reinterpret_cast<float *>(extra + QS) + 2 * KB * GH;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < OWN; i++) {
@@ -446,14 +453,10 @@ struct F32Block {
       const float sum = cs[h], inv = 1.f / sum;
 #pragma unroll
       for (int i = 0; i < NC; i++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-          for (int x = LANES; x < 32; x <<= 1) acc[h][i][e] += __shfl_xor_sync(0xffffffffu, acc[h][i][e], x);
+        const float4 v = dims(h, i);
         const int c = lane % LANES + 32 * i;
         if (lane < LANES && c * 4 < D && h < count)
-          *reinterpret_cast<float4 *>(out + h * D + 4 * c) =
-              sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc[h][i][0] * inv, acc[h][i][1] * inv, acc[h][i][2] * inv, acc[h][i][3] * inv);
+          *reinterpret_cast<float4 *>(out + h * D + 4 * c) = sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       }
     }
   }
@@ -472,19 +475,16 @@ struct F32Block {
     for (int h = 0; h < GH; h++)
 #pragma unroll
       for (int i = 0; i < NC; i++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-          for (int x = LANES; x < 32; x <<= 1) acc[h][i][e] += __shfl_xor_sync(0xffffffffu, acc[h][i][e], x);
+        const float4 v = dims(h, i);
         const int c = lane % LANES + 32 * i;
-        if (lane < LANES && c * 4 < D) *reinterpret_cast<float4 *>(part + h * PR + 4 + 4 * c) = make_float4(acc[h][i][0], acc[h][i][1], acc[h][i][2], acc[h][i][3]);
+        if (lane < LANES && c * 4 < D) *reinterpret_cast<float4 *>(part + h * PR + 4 + 4 * c) = v;
       }
   }
 };
 
 // shared memory of a CTA with rings of `stages` blocks, and how many CTAs of two blocks or more fit on an SM (three at most: registers)
 constexpr int split_smem(int size, int DP, int HEADS, int stages) {
-  const int rows = size == 2 ? 16 : 8, extra = size == 2 ? 0 : HEADS * DP * 4 + (rows * HEADS * 4 + HEADS * 4 + 15) / 16 * 16;
+  const int rows = size == 2 ? 16 : 8, extra = size == 2 ? 0 : HEADS * DP * 4 + (rows * HEADS * 8 + HEADS * 4 + 15) / 16 * 16;
   return PA_WARPS * (stages * 2 * rows * DP * size + HEADS * (DP + 4) * 4 + extra);
 }
 constexpr int split_room(int ctas) { return 228 * 1024 / ctas - 1024 - 512; }  // beside what is static

@@ -401,20 +401,6 @@ __device__ __forceinline__ Raw<CB> lds_raw(uint32_t addr) {
   }
   return r;
 }
-// two f32 in a 64-bit register
-__device__ __forceinline__ uint64_t two(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
-__device__ __forceinline__ float lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 template <typename T, int CB>
 __device__ __forceinline__ void unpack(const Raw<CB> &r, uint64_t (&f)[CB / sizeof(T) / 2]) {
   if constexpr (sizeof(T) == 4) {
