@@ -303,95 +303,101 @@ struct MmaBlock {
   }
 };
 
-// f32: a block of 8 keys, f32 products, two to an instruction (f32x2).  For the scores a lane has a key and a quarter of its chunks (the queries are broadcasts from shared
-// memory); the four lanes of a key hand each other halves of their heads until each has its own complete.  The weights go through
-// shared memory, and for the values a lane owns chunks of dims (of 64 dims: and every other key).
+// f32: a block of 8 keys, f32 products, two to an instruction (f32x2).
+//   Scores: sixteen lanes take a key, two keys at a time; a lane has DP / 64 chunks of all query heads in registers (from shared memory, as
+//   broadcasts, they cost four cycles of it each, half of all it does) and multiplies four keys' with them.  The 4 GH partial sums are
+//   exchanged until every lane has one score complete (two of 8 heads): at each step it hands half of them to its partner and keeps the other half.
+//   Value i = 4 h + t (head h, key 2 t + lane / 16) ends in the lanes with lane % 16 = i (8 heads: i / 2; fewer than 4: several lanes).
+//   Values: the weights go through shared memory, twice each, as the f32x2 products want them; SPLIT keys at a time, a lane owns NC chunks of dims.
 template <int DP_, int GH>
 struct F32Block {
   using T = float;
   static constexpr int DP = DP_, KB = 8, HEADS = GH, ROWB = DP * 4, PR = DP + 4;
-  static constexpr int OWN = GH < 4 ? 1 : GH / 4, NC = DP < 128 ? 1 : DP / 128, SPLIT = DP < 128 ? 128 / DP : 1;  // heads of a lane; chunks; keys side by side
-  static constexpr int QS = GH * DP * 4, PS = (KB * GH * 8 + GH * 4 + 15) / 16 * 16, EXTRA = QS + PS;  // of a warp: queries | weights (twice each), corrections
-  uint64_t acc[GH][NC][2];
-  float m[OWN], l[OWN];
+  static constexpr int QC = DP / 64, NV = 4 * GH, OWN = NV > 16 ? NV / 16 : 1, SAME = NV < 16 ? 16 / NV : 1;  // chunks of a query; sums; scores of a lane, lanes of a score
+  static constexpr int SPLIT = GH > 4 ? (DP == 64 ? 2 : 1) : DP == 64 ? 4 : DP == 128 ? 2 : 1, LANES = 32 / SPLIT, NC = DP / 4 / LANES;
+  static constexpr int EXTRA = KB * GH * 8 + (GH * 4 + 15) / 16 * 16;  // of a warp: weights, corrections or sums
+  uint64_t q[GH][QC][2], acc[GH][NC][2];
+  float m, l;  // of this lane's head
 
-  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *extra) {
+  __device__ __forceinline__ static int head_of(int lane) { return (lane & 15) * OWN / SAME / 4; }
+  __device__ __forceinline__ static int t_of(int lane, int i) { return ((lane & 15) * OWN / SAME + i) & 3; }
+
+  __device__ __forceinline__ void begin(const SplitArgs &s, int b, int kh, int h0, int count, unsigned char *) {
     const PagedArgs &a = s.p;
-    float4 *qs = reinterpret_cast<float4 *>(extra);
-    __syncwarp();  // (the unit before is done with them)
-#pragma unroll 1
-    for (int i = threadIdx.x & 31; i < GH * DP / 4; i += 32) {
-      const int h = i / (DP / 4), c = i % (DP / 4);
-      qs[i] = h < count && 4 * c < a.D ? *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + b * a.q_s[0] + (kh * a.G + h0 + h) * a.q_s[1] + 4 * c)
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __syncwarp();
+    const int lane = threadIdx.x & 31;
+    const float *from = static_cast<const float *>(a.q) + b * a.q_s[0] + (kh * a.G + h0) * a.q_s[1];
 #pragma unroll
-    for (int i = 0; i < OWN; i++) m[i] = -INFINITY, l[i] = 0.f;
+    for (int h = 0; h < GH; h++)
+#pragma unroll
+      for (int i = 0; i < QC; i++) {
+        const int c = (lane & 15) + 16 * i;
+        q[h][i][0] = q[h][i][1] = 0;
+        if (h < count && 4 * c < a.D) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(from + h * a.q_s[1] + 4 * c);
+          q[h][i][0] = v.x, q[h][i][1] = v.y;
+        }
+      }
+    m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int h = 0; h < GH; h++)
 #pragma unroll
       for (int i = 0; i < NC; i++) acc[h][i][0] = acc[h][i][1] = 0;
   }
 
-  __device__ __forceinline__ static int first_head(int lane) { return GH >= 4 ? (lane & 2 ? GH / 2 : 0) + (lane & 1 ? GH / 4 : 0) : GH == 2 ? lane >> 1 & 1 : 0; }
-
   __device__ __forceinline__ void block(const Scorer &score, uint32_t kbase, uint32_t valid, unsigned char *extra) {
-    const int lane = threadIdx.x & 31, key = lane >> 2, qd = lane & 3;
-    const float *qs = reinterpret_cast<const float *>(extra);
-    float2 *ps = reinterpret_cast<float2 *>(extra + QS);
+    const int lane = threadIdx.x & 31, sub = lane >> 4;
+    float2 *ps = reinterpret_cast<float2 *>(extra);
     float *cs = reinterpret_cast<float *>(ps + KB * GH);
-    uint64_t d2[GH];
+    float v[NV];
 #pragma unroll
-    for (int h = 0; h < GH; h++) d2[h] = 0;
-    const uint32_t krow = kbase + key * ROWB;
-    const int turn = spread(key);
+    for (int t = 0; t < 4; t++) {
+      uint64_t d[GH];
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) {
-      const int c = qd + 4 * i;
-      const uint4 w = lds128(krow + ((c ^ turn) << 4));
-      const uint64_t k0 = (uint64_t)w.y << 32 | w.x, k1 = (uint64_t)w.w << 32 | w.z;
+      for (int h = 0; h < GH; h++) d[h] = 0;
+      const int key = 2 * t + sub;
 #pragma unroll
-      for (int h = 0; h < GH; h++) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(qs + h * DP + 4 * c);
-        d2[h] = fma2(q.x, k0, fma2(q.y, k1, d2[h]));
+      for (int i = 0; i < QC; i++) {
+        const uint4 w = lds128(kbase + key * ROWB + ((((lane & 15) + 16 * i) ^ spread(key)) << 4));
+        const uint64_t k0 = (uint64_t)w.y << 32 | w.x, k1 = (uint64_t)w.w << 32 | w.z;
+#pragma unroll
+        for (int h = 0; h < GH; h++) d[h] = fma2(q[h][i][0], k0, fma2(q[h][i][1], k1, d[h]));
       }
+#pragma unroll
+      for (int h = 0; h < GH; h++) v[4 * h + t] = lo(d[h]) + hi(d[h]);
     }
-    float d[GH];
+    int cnt = NV;
 #pragma unroll
-    for (int h = 0; h < GH; h++) d[h] = lo(d2[h]) + hi(d2[h]);
-    int cnt = GH;
-#pragma unroll
-    for (int x = 2; x >= 1; x >>= 1) {
-      if (cnt > 1) {
+    for (int x = 8; x >= 1; x >>= 1) {
+      if (cnt > OWN) {
         const int half = cnt / 2;
         const bool up = lane & x;
 #pragma unroll
-        for (int i = 0; i < GH / 2; i++)
+        for (int i = 0; i < NV / 2; i++)
           if (i < half) {
-            const float send = up ? d[i] : d[i + half], keep = up ? d[i + half] : d[i];
-            d[i] = keep + __shfl_xor_sync(0xffffffffu, send, x);
+            const float send = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, x);
           }
         cnt = half;
       } else {
-        d[0] += __shfl_xor_sync(0xffffffffu, d[0], x);
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], x);
       }
     }
-    const int h0 = first_head(lane);
-    bool same = true;
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < OWN; i++) v[i] = valid >> (2 * t_of(lane, i) + sub) & 1 ? score(v[i]) : -INFINITY, mx = fmaxf(mx, v[i]);
+#pragma unroll
+    for (int x = 1; x < 4 / OWN; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x * SAME));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+    const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(m - use);
+    const bool same = mx == m;
+    m = mx, l *= corr;
 #pragma unroll
     for (int i = 0; i < OWN; i++) {
-      const float s = valid >> key & 1 ? score(d[i]) : -INFINITY;
-      float mx = s;
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      mx = fmaxf(mx, m[i]);
-      const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(m[i] - use), p = ex2(s - use);
-      same = same && mx == m[i];
-      m[i] = mx, l[i] = fmaf(l[i], corr, p);
-      ps[key * GH + h0 + i] = make_float2(p, p);
-      if (key == 0) cs[h0 + i] = corr;
+      const float p = ex2(v[i] - use);
+      l += p;
+      ps[(2 * t_of(lane, i) + sub) * GH + head_of(lane)] = make_float2(p, p);
     }
+    cs[head_of(lane)] = corr;  // (the same from all lanes of a head)
     __syncwarp();
     if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
@@ -401,7 +407,6 @@ struct F32Block {
         for (int i = 0; i < NC; i++) acc[h][i][0] = mul2(acc[h][i][0], c), acc[h][i][1] = mul2(acc[h][i][1], c);
       }
     }
-    constexpr int LANES = 32 / SPLIT;  // of a row
 #pragma unroll
     for (int k0 = 0; k0 < KB; k0 += SPLIT) {
       const int k = k0 + lane / LANES;
@@ -417,44 +422,44 @@ struct F32Block {
       }
 #pragma unroll
       for (int i = 0; i < NC; i++) {
-        const int c = lane % LANES + 32 * i;
-        const uint4 w = lds128(kbase + (KB + k) * ROWB + ((c ^ spread(k)) << 4));
+        const uint4 w = lds128(kbase + (KB + k) * ROWB + (((lane % LANES + LANES * i) ^ spread(k)) << 4));
         const uint64_t v0 = (uint64_t)w.y << 32 | w.x, v1 = (uint64_t)w.w << 32 | w.z;
 #pragma unroll
         for (int h = 0; h < GH; h++) acc[h][i][0] = fma2(p[h], v0, acc[h][i][0]), acc[h][i][1] = fma2(p[h], v1, acc[h][i][1]);
       }
     }
   }
+
   // the four dims of a chunk, of all lanes that have some of its keys
   __device__ __forceinline__ float4 dims(int h, int i) const {
     float v[4] = {lo(acc[h][i][0]), hi(acc[h][i][0]), lo(acc[h][i][1]), hi(acc[h][i][1])};
 #pragma unroll
     for (int e = 0; e < 4; e++)
 #pragma unroll
-      for (int x = 32 / SPLIT; x < 32; x <<= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], x);
+      for (int x = LANES; x < 32; x <<= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], x);
     return make_float4(v[0], v[1], v[2], v[3]);
+  }
+  __device__ __forceinline__ float sum_of() const {  // over the keys of all lanes of this lane's head
+    float sum = l;
+#pragma unroll
+    for (int x = 1; x < 4 / OWN; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x * SAME);
+    return sum + __shfl_xor_sync(0xffffffffu, sum, 16);
   }
 
   __device__ __forceinline__ void write(float *out, int count, int D, unsigned char *extra) {
-    const int lane = threadIdx.x & 31, h0 = first_head(lane);
-    float *cs = reinterpret_cast<float *>(extra + QS) + 2 * KB * GH;
+    const int lane = threadIdx.x & 31;
+    float *cs = reinterpret_cast<float *>(extra) + 2 * KB * GH;
+    const float mine = sum_of();
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < OWN; i++) {
-      float sum = l[i];
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (lane < 4) cs[h0 + i] = sum;
-    }
+    cs[head_of(lane)] = mine;
     __syncwarp();
-    constexpr int LANES = 32 / SPLIT;
 #pragma unroll
     for (int h = 0; h < GH; h++) {
       const float sum = cs[h], inv = 1.f / sum;
 #pragma unroll
       for (int i = 0; i < NC; i++) {
         const float4 v = dims(h, i);
-        const int c = lane % LANES + 32 * i;
+        const int c = lane % LANES + LANES * i;
         if (lane < LANES && c * 4 < D && h < count)
           *reinterpret_cast<float4 *>(out + h * D + 4 * c) = sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       }
@@ -462,21 +467,15 @@ struct F32Block {
   }
 
   __device__ __forceinline__ void store(float *part, int D) {
-    const int lane = threadIdx.x & 31, h0 = first_head(lane);
-#pragma unroll
-    for (int i = 0; i < OWN; i++) {
-      float sum = l[i];
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (lane < 4) part[(h0 + i) * PR] = m[i], part[(h0 + i) * PR + 1] = sum;
-    }
-    constexpr int LANES = 32 / SPLIT;
+    const int lane = threadIdx.x & 31;
+    const float mine = sum_of();
+    part[head_of(lane) * PR] = m, part[head_of(lane) * PR + 1] = mine;  // (the same from all lanes of a head)
 #pragma unroll
     for (int h = 0; h < GH; h++)
 #pragma unroll
       for (int i = 0; i < NC; i++) {
         const float4 v = dims(h, i);
-        const int c = lane % LANES + 32 * i;
+        const int c = lane % LANES + LANES * i;
         if (lane < LANES && c * 4 < D) *reinterpret_cast<float4 *>(part + h * PR + 4 + 4 * c) = v;
       }
   }
@@ -484,7 +483,7 @@ struct F32Block {
 
 // shared memory of a CTA with rings of `stages` blocks, and how many CTAs of two blocks or more fit on an SM (three at most: registers)
 constexpr int split_smem(int size, int DP, int HEADS, int stages) {
-  const int rows = size == 2 ? 16 : 8, extra = size == 2 ? 0 : HEADS * DP * 4 + (rows * HEADS * 8 + HEADS * 4 + 15) / 16 * 16;
+  const int rows = size == 2 ? 16 : 8, extra = size == 2 ? 0 : rows * HEADS * 8 + (HEADS * 4 + 15) / 16 * 16;
   return PA_WARPS * (stages * 2 * rows * DP * size + HEADS * (DP + 4) * 4 + extra);
 }
 constexpr int split_room(int ctas) { return 228 * 1024 / ctas - 1024 - 512; }  // beside what is static
@@ -1066,9 +1065,9 @@ Cut cut_of(const lb200_paged_attn_args *p) {
   c.streamed = p->D % 16 == 0 && !(off & 15) && (far[0] > far[1] ? far[0] : far[1]) / c.unit <= 0xffffffffull;
   if (!c.streamed) return c;
   c.DP = p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256;
-  const int most = size == 4 && c.DP == 256 ? 8 : 16;  // heads per unit: what shared memory and registers hold
+  const int most = size == 2 ? 16 : c.DP == 256 ? 4 : 8;  // heads per unit: what the registers hold
   c.groups = (G + most - 1) / most, c.hpg = (G + c.groups - 1) / c.groups, c.groups = (G + c.hpg - 1) / c.hpg;
-  c.HEADS = size == 4 ? (c.hpg <= 1 ? 1 : c.hpg <= 2 ? 2 : c.hpg <= 4 ? 4 : c.hpg <= 8 ? 8 : 16) : (c.hpg <= 8 ? 8 : 16);
+  c.HEADS = size == 4 ? (c.hpg <= 1 ? 1 : c.hpg <= 2 ? 2 : c.hpg <= 4 ? 4 : 8) : (c.hpg <= 8 ? 8 : 16);
   long long keys = (long long)p->W * p->page_size;
   if (p->window > 0 && p->window < keys) keys = p->window;
   const long long blocks = (keys + (size == 4 ? 7 : 15)) / (size == 4 ? 8 : 16);
@@ -1148,9 +1147,8 @@ int launch_dtype(const SplitArgs &s, const Cut &c, int dtype, cudaStream_t st) {
     case 1: return launch_split<F32Block<DP, 1>>(s, c, st);
     case 2: return launch_split<F32Block<DP, 2>>(s, c, st);
     case 4: return launch_split<F32Block<DP, 4>>(s, c, st);
-    case 8: return launch_split<F32Block<DP, 8>>(s, c, st);
   }
-  if constexpr (DP < 256) return launch_split<F32Block<DP, 16>>(s, c, st);
+  if constexpr (DP < 256) return launch_split<F32Block<DP, 8>>(s, c, st);
   return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: %d heads per unit", c.HEADS);
 
 }
