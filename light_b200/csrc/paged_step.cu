@@ -255,7 +255,7 @@ int launch_pages(void (*kern)(PagesArgs, bool), const PagesArgs &a, size_t smem,
 // y = x rsqrt(mean x^2 + eps) w over the D elements of a head (no weight: y = x), then the first R of them in pairs (a, b):
 //   (a cos t - b sin t, a sin t + b cos t) factor,   t = position * inv_freq[i],   pair i = (i, i + R / 2) or (2 i, 2 i + 1).
 // f32 from the operand to the one rounding at the end; t in f64 (200000 positions far, an f32 angle is off by 0.01), reduced there to
-// [-pi, pi] for the f32 functions.  The angles are the same for every head of a token, so a CTA takes a token and computes each once.
+// half a turn for the f32 functions.  The angles are the same for every head of a token, so a CTA takes a token and computes each once.
 struct RotateArgs {
   const void *q, *k, *v, *qw, *kw;
   void *q_out, *k_out, *v_out;            // k_out: dense, or the cache's keys with slots
@@ -270,10 +270,9 @@ struct RotateArgs {
 };
 
 __device__ __forceinline__ float2 cos_sin(long long pos, double freq) {
-  const double t = (double)pos * freq;
-  const double r = fma(-6.283185307179586476925, rint(t * 0.15915494309189533577), t);
+  const double t = (double)pos * freq * 0.15915494309189533577;  // in turns: 10^6 radians keep 2^-35 of one
   float s, c;
-  sincosf((float)r, &s, &c);
+  sincospif(2.f * (float)(t - rint(t)), &s, &c);
   return make_float2(c, s);
 }
 
@@ -350,7 +349,7 @@ __global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) 
 //   f' = r (f (w_f cos) - g (w_g sin)),  g' = r (f (w_f sin) + g (w_g cos)),
 // two elements to an instruction (f32x2).  Bound by the memory, 2 (NH + 2 KH) D elements per token, with half as many instructions again as
 // the issue slots that takes: hence the pairs, and a pass each for queries, keys and values without a choice inside.
-constexpr int RC_WARPS = 4, RC_AHEAD = 6;  // rounds of heads that are on their way together
+constexpr int RC_WARPS = 4, RC_AHEAD = 6, RC_SLOTS = 32;  // rounds of heads that are on their way together; warps on an SM
 
 struct Chunks {
   int lg, split, first, count;  // lanes per head, warps per token; chunks that a lane's second lies behind its first; chunks per head
@@ -443,15 +442,15 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.R >> 1;
-  const long long id = (long long)blockIdx.x * RC_WARPS + warp, t = ch.split == 1 ? id : id / ch.split;
+  const long long id = (long long)blockIdx.x * RC_WARPS + warp, stride = (long long)gridDim.x * RC_WARPS / ch.split;  // (the host makes it whole)
+  long long t = ch.split == 1 ? id : id / ch.split;
   if (t >= a.T) return;
   const int gl = lane & (ch.lg - 1), per = 32 / ch.lg, hl = lane / ch.lg;
   // the kinds (queries, keys, values) of this warp and its part of their heads: every kind, or with many warps per token one
-  int part = (int)(id - t * ch.split), parts = ch.split, kind = 0;
-  const bool one_kind = ch.q_parts > 0;
-  if (one_kind) {
-    kind = part < ch.q_parts ? 0 : part < ch.q_parts + ch.k_parts ? 1 : 2, parts = kind == 0 ? ch.q_parts : ch.k_parts;
-    part -= kind == 0 ? 0 : kind == 1 ? ch.q_parts : ch.q_parts + ch.k_parts;
+  int part = (int)(id - t * ch.split), parts = ch.split, kind0 = 0, kinds = a.slots ? 3 : 2;
+  if (ch.q_parts > 0) {
+    kind0 = part < ch.q_parts ? 0 : part < ch.q_parts + ch.k_parts ? 1 : 2, kinds = kind0 + 1, parts = kind0 == 0 ? ch.q_parts : ch.k_parts;
+    part -= kind0 == 0 ? 0 : kind0 == 1 ? ch.q_parts : ch.q_parts + ch.k_parts;
   }
   // this lane's chunks, -1 for none
   int c0, c1;
@@ -464,17 +463,6 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     if (c0 >= ch.count) c0 = -1;
     if (c1 >= ch.count) c1 = -1;
   }
-  const long long pos = a.positions[t];
-  long long slot = -1;
-  int page = 0, row = 0;
-  if (a.slots) {
-    slot = a.slots[t];
-    if (slot >= a.rows) {
-      if (lane == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
-      slot = -1;
-    }
-    if (slot >= 0) page = a.rows <= 0x7fffffffll ? a.page.div((int)slot) : (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
-  }
   // Rounds of `per` heads of a kind, this warp has every parts-th: where this lane's head of the next of them lies, elements from one to the next, and
   // the heads from this lane's on (it has one while left > 0).
   struct Walk {
@@ -483,62 +471,81 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
     int left;
   };
   const int hop = per * parts, h0 = part * per + hl;
-  auto source = [&](int kind) {
+  auto source = [&](int kind, long long t) {
     const long long *st = kind == 0 ? a.q_s : kind == 1 ? a.k_s : a.v_s;
     return Walk{static_cast<T *>(const_cast<void *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v)) + t * st[0] + h0 * st[1], hop * st[1], (kind == 0 ? a.NH : a.KH) - h0};
   };
-  auto target = [&](int kind) {
+  auto target = [&](int kind, int page, int row) {
     const int left = (kind == 0 ? a.NH : a.KH) - h0;
     if (kind == 0) return Walk{static_cast<T *>(a.q_out) + (t * a.NH + h0) * a.D, (long long)hop * a.D, left};
     if (!a.slots) return Walk{static_cast<T *>(a.k_out) + (t * a.KH + h0) * a.D, (long long)hop * a.D, left};
     const long long *cs = kind == 1 ? a.ks : a.vs;
     return Walk{static_cast<T *>(kind == 1 ? a.k_out : a.v_out) + page * cs[0] + h0 * cs[1] + row * cs[2], hop * cs[1], left};
   };
-  const int kinds = min(a.slots ? (slot >= 0 ? 3 : 1) : 2, one_kind ? kind + 1 : 3);
-  if (kind >= kinds) return;
-  // a ring of rounds in shared memory: every lane copies and reads its own chunks, so nobody waits for anybody
+  // a ring of rounds in shared memory, those of the next token behind this one's: every lane copies and reads its own chunks, so nobody waits for anybody
   const uint32_t mine = umma::smem_u32(ring[warp]) + lane * CB;
-  int far_kind = kind, slot_far = 0, slot_now = 0;
-  Walk far = source(kind);
+  for (int i = 0; i < RC_AHEAD; i++) {  // no chunk: zeros, in the mean square
+    if (c0 < 0) *reinterpret_cast<Raw<CB> *>(ring[warp][i][0][lane]) = Raw<CB>{};
+    if (c1 < 0) *reinterpret_cast<Raw<CB> *>(ring[warp][i][1][lane]) = Raw<CB>{};
+  }
+  int far_kind = kind0, slot_far = 0, slot_now = 0;
+  long long far_t = t;
+  Walk far = source(kind0, t);
   auto fetch = [&]() {  // the next round, if there is one
-    if (far_kind < kinds) {
+    if (far_t < a.T) {
       if (far.left > 0) {
         const uint32_t dst = mine + slot_far * (64 * CB);
         if (c0 >= 0) cp_chunk<CB>(dst, far.at + c0 * E);
         if (c1 >= 0) cp_chunk<CB>(dst + 32 * CB, far.at + c1 * E);
       }
       far.at += far.step, far.left -= hop;
-      if (far.left + hl <= 0 && ++far_kind < kinds) far = source(far_kind);  // (the same for the whole warp)
+      while (far.left + hl <= 0 && far_t < a.T) {  // (the same for the whole warp)
+        if (++far_kind == kinds) far_kind = kind0, far_t += stride;
+        if (far_t < a.T) far = source(far_kind, far_t);
+      }
     }
     cp_async_commit();
     slot_far = slot_far + 1 == RC_AHEAD ? 0 : slot_far + 1;
   };
+  long long pos = a.positions[t], slot = a.slots ? a.slots[t] : 0;
 #pragma unroll
   for (int i = 0; i < RC_AHEAD; i++) fetch();  // on their way while the angles are worked out
-  if (kind < 2) {
-    for (int i = lane; i < half; i += 32) {
-      const float2 cs = cos_sin(pos, a.inv_freq[i]);
-      trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
-    }
-    __syncwarp();
-  }
   Walk to;
   auto take = [&](Raw<CB> &x, Raw<CB> &y) {  // (its copies have been waited for)
     x = lds_raw<CB>(mine + slot_now * (64 * CB)), y = lds_raw<CB>(mine + slot_now * (64 * CB) + 32 * CB);
     slot_now = slot_now + 1 == RC_AHEAD ? 0 : slot_now + 1;
   };
+  bool kept = true;
   auto put = [&](const Raw<CB> &u, const Raw<CB> &z) {
-    if (to.left > 0) {
+    if (to.left > 0 && kept) {
       if (c0 >= 0) st_raw<CB>(to.at + c0 * E, u);
       if (c1 >= 0) st_raw<CB>(to.at + c1 * E, z);
     }
     to.at += to.step, to.left -= hop;
   };
 #pragma unroll 1
-  for (; kind < kinds; kind++) {
-    to = target(kind);
+  for (; t < a.T; t += stride) {
+  int page = 0, row = 0;
+  if (slot >= a.rows && a.slots) {
+    if (lane == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
+    slot = -1;
+  }
+  if (slot >= 0 && a.slots) page = a.rows <= 0x7fffffffll ? a.page.div((int)slot) : (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
+  if (kind0 < 2) {
+    __syncwarp();  // (the token before is done with its angles)
+    for (int i = lane; i < half; i += 32) {
+      const float2 cs = cos_sin(pos, a.inv_freq[i]);
+      trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
+    }
+    __syncwarp();
+  }
+  const bool placed = slot >= 0;
+  if (t + stride < a.T) pos = a.positions[t + stride], slot = a.slots ? a.slots[t + stride] : 0;
+#pragma unroll 1
+  for (int kind = kind0; kind < kinds; kind++) {
+    to = target(kind, page, row), kept = kind == 0 || placed;
     const T *const w = static_cast<const T *>(kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr);
-    if (kind == 2) {
+    if (kind == 2 || !kept) {  // copied as they are, or passed over
       while (to.left + hl > 0) {
         Raw<CB> x, y;
         cp_async_wait<RC_AHEAD - 1>();
@@ -546,7 +553,7 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
         put(x, y);
         fetch();
       }
-      return;
+      continue;
     }
     if (to.left + hl <= 0) continue;
     // what f and g are multiplied by: f' = f ff + g gf, g' = f fg + g gg (halves); per chunk x' = x ff + swapped x gf (neighbours: chunk g has fg, gg)
@@ -590,8 +597,6 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
         float ss[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-#pragma unroll
-          for (int j = 0; j < V; j++) f[i][j] = c0 < 0 ? 0 : f[i][j], g[i][j] = c1 < 0 ? 0 : g[i][j];  // (no chunk: the ring holds anything there)
           uint64_t s0 = mul2(f[i][0], f[i][0]), s1 = mul2(g[i][0], g[i][0]);
 #pragma unroll
           for (int j = 1; j < V; j++) s0 = fma2(f[i][j], f[i][j], s0), s1 = fma2(g[i][j], g[i][j], s1);
@@ -628,6 +633,7 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
         }
       }
     }
+  }
   }
 }
 
@@ -740,8 +746,11 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
           ch.q_parts = (rq + rounds - 1) / rounds, ch.k_parts = (rk + rounds - 1) / rounds;
           ch.split = ch.q_parts + (kinds - 1) * ch.k_parts;
         }
-      const long long ctas = (p->T * ch.split + RC_WARPS - 1) / RC_WARPS;
-      if (ctas <= 0x7fffffffll) return launch_chunks(a, ch, cb, p->dtype, (unsigned)ctas, st);
+      // a warp takes a token after the other, where all of them together have more than RC_SLOTS warps for every SM
+      long long ctas = (p->T * ch.split + RC_WARPS - 1) / RC_WARPS;
+      if (ch.split == 1 && ctas > (long long)RC_SLOTS / RC_WARPS * sm_count()) ctas = (long long)RC_SLOTS / RC_WARPS * sm_count();
+      if (ch.split > 1) ctas = (ctas + ch.split - 1) / ch.split * ch.split;  // (a whole number of tokens at a time)
+      return launch_chunks(a, ch, cb, p->dtype, (unsigned)ctas, st);
     }
   }
   cudaError_t e;
