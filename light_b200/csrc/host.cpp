@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -309,6 +310,10 @@ PyObject *moe_gemm(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
 }
 
 // ---- many sequences over one paged cache
+// An output: uninitialised memory of this stream's part of the caching allocator, asked for without torch's dispatcher (half a microsecond of five).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, int dev) {
+  return at::detail::empty_cuda(sizes, dt, at::Device(at::kCUDA, (c10::DeviceIndex)dev), std::nullopt);
+}
 // A contiguous tensor in the memory of `whole`, `at` bytes in (outputs that come together, from one allocation).
 at::Tensor piece(const at::Tensor &whole, int64_t at, at::IntArrayRef sizes, at::ScalarType dt) {
   auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(dt));
@@ -358,7 +363,7 @@ PyObject *paged_advance(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const int64_t B = t.t->size(0), W = t.t->size(1), cap = f.t->numel();
   NEED(i32_of(*l.t, dev, B) && i32_of(*n.t, dev, B) && i32_of(*c.t, dev, 1) && f.t->dim() == 1 && cap > 0 && cap < (1ll << 31) && i32_of(*f.t, dev, cap));
   NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31) && tokens >= 0);
-  const at::Tensor whole = at::empty({16 * tokens + 4 * (3 * B + 2)}, l.t->options().dtype(at::kByte));
+  const at::Tensor whole = fresh({16 * tokens + 4 * (3 * B + 2)}, at::kByte, dev);
   const int64_t ints = 16 * tokens;
   at::Tensor pos = piece(whole, 0, {tokens}, at::kLong), slots = piece(whole, 8 * tokens, {tokens}, at::kLong);
   at::Tensor starts = piece(whole, ints, {B + 1}, at::kInt), granted = piece(whole, ints + 4 * (B + 1), {B}, at::kInt);
@@ -389,7 +394,7 @@ PyObject *paged_release(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31));
   at::Tensor lens = *l.t, count = *c.t;
   if (!inplace) {
-    const at::Tensor whole = at::empty({B + 1}, l.t->options());
+    const at::Tensor whole = fresh({B + 1}, at::kInt, dev);
     lens = piece(whole, 0, {B}, at::kInt), count = piece(whole, 4 * B, {1}, at::kInt);
   }
   lb200_paged_pages p{};
@@ -429,8 +434,8 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     for (int i = 0; i < 2; i++) p.v_stride[i] = v.t->stride(i);
     p.pages = kc.t->size(0), p.page_size = (int)kc.t->size(2);
   }
-  at::Tensor q_out = at::empty({T, NH, D}, q.t->options()), k_out;
-  if (!cached) k_out = at::empty({T, KH, D}, q.t->options()), p.k_out = k_out.data_ptr(), p.page_size = 1;
+  at::Tensor q_out = fresh({T, NH, D}, dt, dev), k_out;
+  if (!cached) k_out = fresh({T, KH, D}, dt, dev), p.k_out = k_out.data_ptr(), p.page_size = 1;
   p.q = q.t->const_data_ptr(), p.k = k.t->const_data_ptr(), p.q_weight = w[0].t ? w[0].t->const_data_ptr() : nullptr, p.k_weight = w[1].t ? w[1].t->const_data_ptr() : nullptr;
   p.positions = pos.t->const_data_ptr<int64_t>(), p.inv_freq = freq.t->const_data_ptr<double>(), p.q_out = q_out.data_ptr();
   for (int i = 0; i < 2; i++) p.q_stride[i] = q.t->stride(i), p.k_stride[i] = k.t->stride(i);
@@ -456,7 +461,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const int64_t B = q.t->size(0), NH = q.t->size(1), D = q.t->size(2), KH = k.t->size(1), stride = table_of(*t.t);
   NEED(act_of(*q.t) >= 0 && B > 0 && D > 0 && KH > 0 && NH % KH == 0 && heads_of(*q.t, B, D, dt, dev) && cache_of(*k.t, *v.t, KH, D, dt, dev, false));
   NEED(stride > 0 && t.t->size(0) == B && t.t->size(1) < (1ll << 31) && t.t->get_device() == dev && l.t->dim() == 1 && i32_of(*l.t, dev, B) && k.t->size(2) < (1ll << 31));
-  at::Tensor out = at::empty({B, NH, D}, q.t->options()), own;
+  at::Tensor out = fresh({B, NH, D}, dt, dev), own;
   lb200_paged_attn_args p{};
   p.q = q.t->const_data_ptr(), p.k = k.t->const_data_ptr(), p.v = v.t->const_data_ptr(), p.block_table = t.t->const_data_ptr<int>(), p.lens = l.t->const_data_ptr<int>();
   p.out = out.data_ptr();
@@ -465,7 +470,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   p.table_stride = stride, p.pages = k.t->size(0), p.dtype = act_of(*q.t), p.B = (int)B, p.NH = (int)NH, p.KH = (int)KH, p.D = (int)D, p.page_size = (int)k.t->size(2);
   p.W = (int)t.t->size(1), p.window = (int)window, p.scale = (float)PyFloat_AsDouble(a[5]), p.softcap = (float)PyFloat_AsDouble(a[7]);
   p.scratch_bytes = light_b200_paged_attn_scratch_bytes(&p, dev);
-  if (p.scratch_bytes) own = at::empty({(int64_t)p.scratch_bytes}, q.t->options().dtype(at::kByte)), p.scratch = own.data_ptr();
+  if (p.scratch_bytes) own = fresh({(int64_t)p.scratch_bytes}, at::kByte, dev), p.scratch = own.data_ptr();
   return give(light_b200_paged_decode_attn(&p, dev, stream_of(dev)), out);
 }
 
