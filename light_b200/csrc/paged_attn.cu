@@ -547,7 +547,7 @@ struct Row {
   bool valid;
 };
 
-template <typename P>
+template <typename P, int S>
 struct Feeder {
   using C = SplitCfg<P>;
   using T = typename P::T;
@@ -562,15 +562,16 @@ struct Feeder {
     const int lane = threadIdx.x & 31;
     k0 = static_cast<const char *>(s.p.k) + lane % LANES * 16, v0 = static_cast<const char *>(s.p.v) + lane % LANES * 16;
     if (s.p.D < P::DP) {  // chunks past the head: nothing is copied there, and the products run over them
-      for (int i = lane; i < C::RING / 16; i += 32) reinterpret_cast<uint4 *>(ring_)[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = lane; i < S * C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(ring_)[i] = make_uint4(0u, 0u, 0u, 0u);
       __syncwarp();
     }
   }
-  __device__ __forceinline__ Row peek(const Cursor &c) const {  // (lanes from KB on repeat)
+  __device__ __forceinline__ Row peek(const Cursor &c) const { return peek(c, c.j0, c.n); }
+  __device__ __forceinline__ Row peek(const Cursor &c, int j0, int n) const {  // (lanes from KB on repeat)
     const PagedArgs &a = s.p;
     Row r;
-    const int j = c.j0 + c.block * P::KB + (threadIdx.x & (P::KB - 1)), w = a.page.div(j);
-    r.valid = j < c.n, r.row = j - w * a.page.d, r.kh = c.kh;
+    const int j = j0 + c.block * P::KB + (threadIdx.x & (P::KB - 1)), w = a.page.div(j);
+    r.valid = j < n, r.row = j - w * a.page.d, r.kh = c.kh;
     r.pg = r.valid ? a.table[c.b * a.table_stride + w] : -1;
     return r;
   }
@@ -620,7 +621,6 @@ struct Feeder {
   }
   // the run's first S - 1 blocks on their way, and the next one's page
   __device__ __forceinline__ Row fill(Cursor &far, int hop) {
-    constexpr int S = C::S;
     Row first[S - 1], next;
     int have = 0;
 #pragma unroll
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
   float *const part = reinterpret_cast<float *>(smem + PA_WARPS * C::RING + warp * C::PART);
   if (now.left > 0) {
     Cursor far = now;  // what is fetched, ahead of what is folded
-    Feeder<P> feed(s, ring, masks[warp]);
+    Feeder<P, S> feed(s, ring, masks[warp]);
     Row next = feed.fill(far, hop);
     const Scorer score(a.scale, a.softcap);
     P state;
@@ -843,101 +843,141 @@ __global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_kern
       for (int i = tid; i < a.NH * a.D; i += PA_THREADS) static_cast<T *>(a.out)[(long long)b * a.NH * a.D + i] = from_f32<T>(0.f);
 }
 
-// Few units of few blocks: a cluster of up to eight CTAs takes a unit, its warps the blocks in turn, and the parts meet in the CTAs' shared memory:
-// one launch, no scratch, no schedule to work out, which is what counts when there is little to read.
+// Few units of few blocks: a cluster of up to sixteen CTAs takes a unit, its warps the blocks in turn: one launch, no scratch, no schedule to work
+// out, which is what counts when there is little to read.  What bounds it is a chain of latencies, so:
+//   * the queries, the length and (without a window) the page of a warp's first block are asked for together;
+//   * the output is dealt to the CTAs in slices, and each CTA pushes its part of every slice into the shared memory of the one that has it, before
+//     the one barrier: what is read after it is at home, and nobody has to stay for others to read from.  (1024 keys by 16 CTAs: 5.35 us with
+//     the parts pulled and a barrier at the end, 5.1 us; 32 units by 8: 6.9, 6.4.)
+constexpr int CL_MAX = 16;
+
 template <typename P>
-__global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_cluster_kernel(SplitArgs s, int ks) {
+struct ClusterCfg {
   using C = SplitCfg<P>;
+  static constexpr int PARTS = PA_WARPS * (C::PART + P::EXTRA), TAKE = P::HEADS * P::DP * 4 + CL_MAX * (16 + P::HEADS * 8);  // parts of the slice, maxima and sums
+  static constexpr int stages(int n) { return n > 2 && PA_WARPS * n * C::STAGE + PARTS + TAKE > split_room(C::CTAS) ? stages(n - 1) : n; }
+  static constexpr int S = stages(C::S), RING = S * C::STAGE, SMEM = PA_WARPS * RING + PARTS + TAKE;
+  static_assert(SMEM <= split_room(C::CTAS), "");
+};
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};\n" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, const float (&v)[4]) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+}
+
+// `slice`: chunks of four dims of a CTA's slice of the unit's heads
+template <typename P>
+__global__ void __launch_bounds__(PA_THREADS, SplitCfg<P>::CTAS) paged_attn_cluster_kernel(SplitArgs s, int ks, FastDiv slice) {
+  using C = ClusterCfg<P>;
   using T = typename P::T;
-  constexpr int KB = P::KB, S = C::S;
+  constexpr int KB = P::KB, S = C::S, PART = SplitCfg<P>::PART;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t masks[PA_WARPS][S];
   pdl_launch_dependents();
   pdl_wait();
   const PagedArgs &a = s.p;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, units = a.KH * s.groups, rank = blockIdx.x % ks, b = blockIdx.x / ks / units;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, units = a.KH * s.groups, rank = blockIdx.x % ks, unit = blockIdx.x / ks, b = unit / units;
+  const int hop = ks * PA_WARPS;
+  unsigned char *const ring = smem + warp * C::RING, *const extra = smem + PA_WARPS * (C::RING + PART) + warp * P::EXTRA;
+  float *const part = reinterpret_cast<float *>(smem + PA_WARPS * C::RING + warp * PART);
   Cursor far;
-  far.at<KB>(a, b);
-  far.unit(blockIdx.x / ks - b * units, s.groups), far.block = rank * PA_WARPS + warp;
-  const int hop = ks * PA_WARPS, blocks = far.blocks;
-  far.left = blocks - far.block;
+  far.b = b, far.unit(unit - b * units, s.groups), far.block = rank * PA_WARPS + warp;
   const int kh = far.kh, h0 = far.hg * s.hpg, count = min(s.hpg, a.G - h0);
+  P state;
+  Feeder<P, S> feed(s, ring, masks[warp]);
+  state.begin(s, b, kh, h0, count, extra);
+  Row next;
+  const bool early = a.window == 0;
+  if (early) next = feed.peek(far, 0, a.W * a.page.d);
+  far.at<KB>(a, b);
+  const int blocks = far.blocks;
+  int left = far.left = blocks - far.block;
   T *const out = static_cast<T *>(a.out) + ((long long)b * a.NH + kh * a.G + h0) * a.D;
   if (tid == 0 && rank == 0 && kh == 0 && far.hg == 0 && a.lens[b] != far.n) atomicOr(&g_attn_status, (unsigned)PAGED_LENGTH);
   if (blocks == 0) {  // (the whole cluster)
     for (int i = rank * PA_THREADS + tid; i < count * a.D; i += ks * PA_THREADS) out[i] = from_f32<T>(0.f);
     return;
   }
-  unsigned char *const ring = smem + warp * C::RING, *const extra = smem + PA_WARPS * (C::RING + C::PART) + warp * P::EXTRA;
-  float *const part = reinterpret_cast<float *>(smem + PA_WARPS * C::RING + warp * C::PART);
-  P state;
-  {
-    Feeder<P> feed(s, ring, masks[warp]);
-    int left = far.left;
-    Row next = feed.fill(far, hop);
-    state.begin(s, b, kh, h0, count, extra);
-    const Scorer score(a.scale, a.softcap);
-    int slot = 0, fill = S - 1;
-    for (; left > 0; left -= hop) {
-      cp_async_wait<S - 2>();
-      __syncwarp();
-      feed.more(far, next, hop, fill);
-      state.block(score, feed.ring + slot * C::STAGE, masks[warp][slot], extra);
-      slot = slot + 1 == S ? 0 : slot + 1, fill = fill + 1 == S ? 0 : fill + 1;
+  if (ks > 1) umma::cluster_arrive();  // this CTA runs: others may write into its memory
+  if (early) next.valid = (rank * PA_WARPS + warp) * KB + (lane & (KB - 1)) < far.n;
+  else if (left > 0) next = feed.peek(far);
+  // S blocks on their way to begin with; a slot is filled again as soon as it has been folded
+#pragma unroll
+  for (int i = 0; i < S; i++) {
+    if (far.left > 0) {
+      feed.issue(next, i);
+      far.next<KB>(s, hop);
+      if (far.left > 0) next = feed.peek(far);
     }
-    cp_async_wait<0>();
-    if (feed.odd) atomicOr(&g_attn_status, feed.odd);
+    cp_async_commit();
   }
+  const Scorer score(a.scale, a.softcap);
+  for (int slot = 0; left > 0; left -= hop) {
+    cp_async_wait<S - 1>();
+    __syncwarp();
+    state.block(score, feed.ring + slot * SplitCfg<P>::STAGE, masks[warp][slot], extra);
+    __syncwarp();
+    if (left > hop) feed.more(far, next, hop, slot);
+    slot = slot + 1 == S ? 0 : slot + 1;
+  }
+  if (feed.odd) atomicOr(&g_attn_status, feed.odd);
   state.store(part, a.D);
   __syncthreads();
   const float *const parts = reinterpret_cast<const float *>(smem + PA_WARPS * C::RING);
-  float *const mine = reinterpret_cast<float *>(smem);  // [HEADS][PR] of this CTA, over its drained rings
+  // what the CTAs push here: of each its part of this slice, then of each its maxima and sums
+  const uint32_t take = umma::smem_u32(smem + PA_WARPS * C::RING + C::PARTS);
+  const uint32_t take_ml = take + (uint32_t)ks * slice.d * 16u;
+  if (ks > 1) umma::cluster_wait();
   for (int h = warp; h < count; h += PA_WARPS) {
     const float *row = parts + h * P::PR;
+    float2 ml[PA_WARPS];
     float top = -INFINITY, L = 0.f, e[PA_WARPS];
 #pragma unroll
-    for (int w = 0; w < PA_WARPS; w++) top = fmaxf(top, row[w * P::HEADS * P::PR]);
+    for (int w = 0; w < PA_WARPS; w++) ml[w] = *reinterpret_cast<const float2 *>(row + w * P::HEADS * P::PR), top = fmaxf(top, ml[w].x);
     const float use = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int w = 0; w < PA_WARPS; w++) e[w] = ex2(row[w * P::HEADS * P::PR] - use), L = fmaf(e[w], row[w * P::HEADS * P::PR + 1], L);
-    if (ks > 1 && lane == 0) mine[h * P::PR] = top, mine[h * P::PR + 1] = L;
-    for (int d = lane; d < a.D; d += 32) {
-      float A = 0.f;
+    for (int w = 0; w < PA_WARPS; w++) e[w] = ex2(ml[w].x - use), L = fmaf(e[w], ml[w].y, L);
+    if (ks > 1 && lane < ks) st_cluster(umma::map_to_rank(take_ml, (uint32_t)lane) + (uint32_t)(rank * P::HEADS + h) * 8u, make_float2(top, L));
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; w++) A = fmaf(e[w], row[w * P::HEADS * P::PR + 4 + d], A);
-      if (ks > 1) mine[h * P::PR + 4 + d] = A;
-      else out[h * a.D + d] = from_f32<T>(L == 0.f ? 0.f : A / L);
-    }
+    for (int d = 4 * lane; d < P::DP; d += 128)
+      if (d < a.D) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; w++) {
+          const float4 x = *reinterpret_cast<const float4 *>(row + w * P::HEADS * P::PR + 4 + d);
+          v[0] = fmaf(e[w], x.x, v[0]), v[1] = fmaf(e[w], x.y, v[1]), v[2] = fmaf(e[w], x.z, v[2]), v[3] = fmaf(e[w], x.w, v[3]);
+        }
+        if (ks == 1) {
+          store4(out + h * a.D + d, v, L);
+        } else {
+          const int c = (h * a.D + d) >> 2, to = slice.div(c);
+          st_cluster(umma::map_to_rank(take, (uint32_t)to) + (uint32_t)(rank * slice.d + c - to * slice.d) * 16u, v);
+        }
+      }
   }
   if (ks == 1) return;
-  umma::cluster_sync();
-  const int all = count * a.D, lo = all * rank / ks, hi = all * (rank + 1) / ks;
-  const uint32_t base = umma::smem_u32(mine);
-  for (int i = lo + tid; i < hi; i += PA_THREADS) {
-    const int h = i / a.D, d = i - h * a.D;
-    float top = -INFINITY, L = 0.f, A = 0.f;
-    for (int r0 = 0; r0 < ks; r0 += 8) {
-      float m[8], l[8], v[8], mx = top;
-#pragma unroll
-      for (int r = 0; r < 8; r++) {  // all remote loads at once
-        const uint32_t row = umma::map_to_rank(base, (uint32_t)(r0 + r < ks ? r0 + r : 0)) + (uint32_t)(h * P::PR) * 4u;
-        m[r] = umma::ld_cluster_f32(row), l[r] = umma::ld_cluster_f32(row + 4u), v[r] = umma::ld_cluster_f32(row + 16u + (uint32_t)d * 4u);
-      }
-#pragma unroll
-      for (int r = 0; r < 8; r++)
-        if (r0 + r < ks) mx = fmaxf(mx, m[r]);
-      const float use = mx == -INFINITY ? 0.f : mx, corr = ex2(top - use);
-      top = mx, L *= corr, A *= corr;
-#pragma unroll
-      for (int r = 0; r < 8; r++)
-        if (r0 + r < ks) {
-          const float e = ex2(m[r] - use);
-          L = fmaf(e, l[r], L), A = fmaf(e, v[r], A);
-        }
+  umma::cluster_arrive();
+  umma::cluster_wait();
+  for (int c = tid; c < slice.d; c += PA_THREADS) {
+    const int i = 4 * (rank * slice.d + c), h = i / a.D;
+    if (h >= count) break;
+    const float2 *ml = reinterpret_cast<const float2 *>(smem + PA_WARPS * C::RING + C::PARTS + ks * slice.d * 16) + h;
+    const float4 *v = reinterpret_cast<const float4 *>(smem + PA_WARPS * C::RING + C::PARTS) + c;
+    float top = -INFINITY, L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int r = 0; r < ks; r++) top = fmaxf(top, ml[r * P::HEADS].x);
+    if (top == -INFINITY) top = 0.f;
+#pragma unroll 4
+    for (int r = 0; r < ks; r++) {
+      const float2 x = ml[r * P::HEADS];
+      const float4 y = v[r * slice.d];
+      const float e = ex2(x.x - top);
+      L = fmaf(e, x.y, L), A[0] = fmaf(e, y.x, A[0]), A[1] = fmaf(e, y.y, A[1]), A[2] = fmaf(e, y.z, A[2]), A[3] = fmaf(e, y.w, A[3]);
     }
-    out[i] = from_f32<T>(L == 0.f ? 0.f : A / L);
+    store4(out + i, A, L);
   }
-  umma::cluster_sync();  // nobody leaves while a peer still reads its part
 }
 
 // The pieces of a unit that was cut, in order: piece 0 is the second of the CTA where it begins, piece i the first of the i-th CTA after it.
@@ -1099,18 +1139,18 @@ int launch_cluster(const SplitArgs &s, const Cut &c, cudaStream_t st) {
   static DeviceOnce once;
   cudaError_t e = once.ensure([&] {
     const cudaError_t f = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return f != cudaSuccess ? f : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<P>::SMEM);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ClusterCfg<P>::SMEM);
   });
   if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(s.p.B * s.p.KH * s.groups * c.ks)), cfg.blockDim = dim3(PA_THREADS), cfg.dynamicSmemBytes = SplitCfg<P>::SMEM, cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(s.p.B * s.p.KH * s.groups * c.ks)), cfg.blockDim = dim3(PA_THREADS), cfg.dynamicSmemBytes = ClusterCfg<P>::SMEM, cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = (unsigned)c.ks, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
   cfg.attrs = at, cfg.numAttrs = c.ks > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, s, c.ks);
+  e = cudaLaunchKernelEx(&cfg, kern, s, c.ks, FastDiv((c.hpg * s.p.D / 4 + c.ks - 1) / c.ks));
   if (e != cudaSuccess) return fail((int)e, "light_b200: paged_decode_attn: %s", cudaGetErrorString(e));
   return launched("paged_decode_attn");
 }
