@@ -460,6 +460,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const auto dt = q.t->scalar_type();
   const int64_t B = q.t->size(0), NH = q.t->size(1), D = q.t->size(2), KH = k.t->size(1), stride = table_of(*t.t);
   NEED(act_of(*q.t) >= 0 && B > 0 && D > 0 && KH > 0 && NH % KH == 0 && heads_of(*q.t, B, D, dt, dev) && cache_of(*k.t, *v.t, KH, D, dt, dev, false));
+  const int64_t step = q.t->element_size();
+  NEED(!(((uintptr_t)q.t->const_data_ptr() | (uintptr_t)(B > 1 ? q.t->stride(0) * step : 0) | (uintptr_t)(NH > 1 ? q.t->stride(1) * step : 0)) & 15));
   NEED(stride > 0 && t.t->size(0) == B && t.t->size(1) < (1ll << 31) && t.t->get_device() == dev && l.t->dim() == 1 && i32_of(*l.t, dev, B) && k.t->size(2) < (1ll << 31));
   at::Tensor out = fresh({B, NH, D}, dt, dev), own;
   lb200_paged_attn_args p{};

@@ -1121,6 +1121,9 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"ops.PagedDecodeAttention: window {window}, softcap {softcap}")
     W = block_table.shape[1]
     qh, lc = _head_rows(q), lens.contiguous()
+    step = q.element_size()
+    if (qh.data_ptr() | (qh.stride(0) * step if B > 1 else 0) | (qh.stride(1) * step if NH > 1 else 0)) & 15:  # the fast kernels read 16 bytes at a time
+        qh = qh.clone(memory_format=torch.contiguous_format)
     table = block_table if block_table.stride(1) == 1 and (B == 1 or block_table.stride(0) >= W) else block_table.contiguous()
     out = torch.empty((B, NH, D), dtype=q.dtype, device=q.device)
     a = _lib.PagedAttnArgs(q=qh.data_ptr(), k=k_cache.data_ptr(), v=v_cache.data_ptr(), block_table=table.data_ptr(), lens=lc.data_ptr(), out=out.data_ptr(),

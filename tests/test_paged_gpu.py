@@ -121,6 +121,9 @@ def test_attention_strided_query_and_shared_cache_tensor(cuda, dtype):
     want = _check(q, k, v, table, lens)
     got = ops.PagedDecodeAttention(wide[:, 2:10], both[:, 0], both[:, 1], tables[:, 1:1 + table.shape[1]], lens, 64 ** -0.5)
     assert torch.equal(got, want)
+    off = torch.zeros((2, 8, 67), dtype=dtype, device=cuda)[..., 1:65]  # heads off 16 bytes
+    off.copy_(q)
+    assert torch.equal(ops.PagedDecodeAttention(off, k, v, table, lens, 64 ** -0.5), want)
     odd = q.transpose(1, 2).contiguous().transpose(1, 2)  # elements of a head apart
     assert torch.equal(ops.PagedDecodeAttention(odd, k, v, table.t().contiguous().t(), lens, 64 ** -0.5), want)
 
@@ -168,6 +171,32 @@ def test_attention_pages_and_lengths_outside(cuda, dtype, D):
     got = _check(q, k, v, table, lens)
     assert bool((got[2] == 0).all()) and bool((got[4] == 0).all())
     assert ops.paged_status(0) & 3 == 3
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_keys_and_values_in_different_orders(cuda, dtype):
+    """Keys a page's head after the other, values a page's row after the other: their rows lie at different distances."""
+    q, k, v, table, lens = _case(cuda, dtype, [200, 16, 333], 3, 4, 80, 16)
+    v = v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    _check(q, k, v, table, lens)
+    _check(q, k, v, table, lens, window=50)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[0, 0, 0], [1], [1] * 300, [5000] + [0] * 200 + [1], [16] * 40 + [3000] * 3 + [17] * 40, [0] * 130 + [700]])
+def test_attention_batches_of_a_kind(cuda, dtype, lens):
+    _check(*_case(cuda, dtype, lens, 2, 4, 64, 16, width=300))  # (a table much wider than the sequences)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_from_cold_memory_is_the_same_every_time(cuda, dtype):
+    r = random.Random(4)
+    case = _case(cuda, dtype, [int(2 ** r.uniform(0, 13)) for _ in range(40)], 4, 4, 128, 16)
+    want = _check(*case)
+    flush = torch.zeros(1 << 26, device=cuda)
+    for _ in range(5):
+        flush.add_(1)
+        assert torch.equal(ops.PagedDecodeAttention(*case, 128 ** -0.5), want)
 
 
 def test_attention_offsets_beyond_32_bits(cuda):
@@ -517,6 +546,21 @@ def test_a_captured_step_is_the_step(cuda, dtype):
         inputs.copy_(x)
         graph.replay()
         assert torch.equal(out, want) and torch.equal(graphed.lens, eager.lens) and torch.equal(graphed.table, eager.table)
+
+
+@pytest.mark.parametrize("n", [300, 6000])
+def test_lengths_that_the_launch_before_writes(cuda, n):
+    """The length and the page of the new token come from the kernel right before the attention."""
+    q, k, v, table, lens = _case(cuda, torch.bfloat16, [n, 40, 7], 2, 4, 128, 16, spare=9, width=2)
+    k.nan_to_num_(0.5), v.nan_to_num_(0.25)
+    free = _t(sorted(set(range(k.shape[0])) - set(table.flatten().tolist())), cuda)
+    count = _t([free.numel()], cuda)
+    one = torch.ones(3, dtype=torch.int32, device=cuda)
+    for _ in range(30):
+        s = ops.PagedAdvance(table, lens, one, free, count, 16, 3, inplace=True)
+        got = ops.PagedDecodeAttention(q, k, v, table, s.lens, 0.1)
+        want, bound = paged_plain.attention(q, k, v, table, lens, 0.1)
+        assert bool(((got.double() - want).abs() <= bound).all())
 
 
 def test_two_streams_at_once(cuda):
