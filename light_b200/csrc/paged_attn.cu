@@ -47,7 +47,9 @@ struct Scorer {
 };
 
 // ------------------------------------------------------------------------------------ any head size, any stride
-// A CTA takes a query head, its four warps every fourth key, a lane every 32nd dim.
+// What the kernels below do not take: head sizes that are not whole 16s, cache rows off 16 bytes, strides whose offsets do not fit 32 bits.  A
+// CTA takes a query head, its four warps every fourth key, a lane every 32nd dim; a chain of a key's latencies bounds it (64 ragged
+// sequences to 8192 keys, 8 KV heads of 128 under 32: 2.96 ms, where the kernel below takes 45 us).
 constexpr int PL_WARPS = 4, PL_MAX_D = 256;
 
 template <typename T>
@@ -113,6 +115,12 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 //     without a key are filled with zeros: a weight of 0 times what lies there must not be NaN.
 //   * Pieces of a unit that was cut are joined in their order, first those of a CTA's warps at its end, in shared memory; what goes on
 //     over CTAs goes to scratch, at most two pieces a CTA, and a second launch joins those: no atomics, the same bits every time.
+// Bound by the memory where sequences are long: one of 131072 keys (537 MB, bf16) 89 us, 6.0 TB/s; eight of 8192 in f32 (537 MB) 90 us.  Of
+// shorter ones by what a launch costs beside its stream: 64 ragged ones (232 MB) 45 us, of which about 6 are the chain of lengths,
+// schedule, pages and first rows (2000 + 1500 + 2000 + 2500 cycles) and 4 the join.
+//   * One wave of CTAs: two, three and four waves of finer runs take 98, 102 and 108 us for the one long sequence, each wave that chain again.
+//   * UNIT 3: 1, 2, 5, 8 give 49.7, 44.5, 45.1, 45.0 us for the 64, and 18.4, 17.6, 20.9, 24.3 for 200 of 300 keys at most (3: 45.2, 18.0).
+//   * All four warps of a CTA on the blocks of one unit in turn, with barriers, took 75 us for the 64: two microseconds a unit.
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 4, CLUSTER_WIDE = 8;
 
 struct SplitArgs {
@@ -124,8 +132,7 @@ struct SplitArgs {
   float *ml, *acc;    // [2 CTAs][HEADS][2], [2 CTAs][HEADS][D]
 };
 
-// 16-byte chunk c of row r of a block lies at chunk c ^ spread(r): eight rows of one chunk on all banks (ldmatrix), two rows of four
-// neighbouring chunks as well (the f32 kernel's lanes)
+// 16-byte chunk c of row r of a block lies at chunk c ^ spread(r): eight rows of one chunk on all banks (ldmatrix)
 __device__ __forceinline__ int spread(int r) { return (r & 1) << 2 | (r >> 1 & 3); }
 
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
@@ -163,6 +170,7 @@ __device__ __forceinline__ uint32_t pack(float &a, float &b, __nv_bfloat16) {
 // bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
 //   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
 //   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
+//   A block of 128 dims is about 400 instructions of a warp, 0.65 us by itself; eight warps of an SM fold 8 KB each in 1.4 us, which is the memory's rate.
 //   P is rounded to the cache's type, as the instruction wants it: 2^-8 (bf16) or 2^-11 of each weight, no more than the output's own rounding;
 //   the sum below the fraction adds the rounded weights, so that they sum to one.
 template <typename T_, int DP_, int NT>
@@ -304,8 +312,9 @@ struct MmaBlock {
 };
 
 // f32: a block of 8 keys, f32 products, two to an instruction (f32x2).
-//   Scores: sixteen lanes take a key, two keys at a time; a lane has DP / 64 chunks of all query heads in registers (from shared memory, as
-//   broadcasts, they cost four cycles of it each, half of all it does) and multiplies four keys' with them.  The 4 GH partial sums are
+//   Scores: sixteen lanes take a key, two keys at a time; a lane has DP / 64 chunks of all query heads in registers and multiplies four keys'
+//   with them.  (Read from shared memory, as broadcasts, they were half of its traffic, 252 wavefronts a block instead of 123: seconds of
+//   calls of eight sequences of 8192 keys, at the clocks that they run at, 101 us each instead of 92.)  The 4 GH partial sums are
 //   exchanged until every lane has one score complete (two of 8 heads): at each step it hands half of them to its partner and keeps the other half.
 //   Value i = 4 h + t (head h, key 2 t + lane / 16) ends in the lanes with lane % 16 = i (8 heads: i / 2; fewer than 4: several lanes).
 //   Values: the weights go through shared memory, twice each, as the f32x2 products want them; SPLIT keys at a time, a lane owns NC chunks of dims.
@@ -1116,9 +1125,12 @@ Cut cut_of(const lb200_paged_attn_args *p) {
     return c;
   }
   const long long slots = (long long)split_ctas(size, c.DP, c.HEADS) * sm_count();
+  // A cluster to a unit where all are resident at once and a warp has CLUSTER_BLOCKS blocks at most.  Up to there it is the faster one whatever
+  // the lengths (bf16, 8 KV heads, us of the split kernel and of this one: 1 x 2048 keys 7.9, 6.2; 4 x 1024 9.2, 6.8; 16 x 512 12.1, 10.6);
+  // with more blocks it gains less on sequences of one length (4 x 4096: 18.7, 16.9) than it loses on others (4 x 8192 ragged: 12.5, 21.2).
   const long long n_units = (long long)p->B * p->KH * c.groups;
   for (c.ks = 1; c.ks < 8 && n_units * (c.ks + 1) <= slots && blocks > c.ks * PA_WARPS;) c.ks++;
-  if (c.ks == 8 && n_units <= CLUSTER_WIDE && blocks > 8 * PA_WARPS) c.ks = 16;
+  if (c.ks == 8 && n_units <= CLUSTER_WIDE && blocks > 8 * PA_WARPS) c.ks = 16;  // (1 x 2048: 7.2 -> 6.2, 1 x 4096: 10.7 -> 8.4)
   if (n_units * c.ks <= slots && blocks <= (long long)c.ks * PA_WARPS * CLUSTER_BLOCKS) return c;
   c.ks = 0;
   const double most_work = (double)p->B * p->KH * c.groups * (double)(blocks + UNIT) / PA_WARPS;  // CTAs' worth, were every sequence as long as the table

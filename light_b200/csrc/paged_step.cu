@@ -14,8 +14,8 @@ __device__ unsigned int g_step_status = 0;
 // the stack does not hold gets none, and as first_b never falls, none after it that needs any.  Token i of the batch belongs to the
 // request with starts_b <= i < starts_{b + 1}: a binary search in shared memory.
 //
-// Two dependent reads (the lengths; then the stack or the table) and the stores bound it: latency.  Every CTA scans the lengths for itself and
-// stores its share.  Where lengths and counter are updated in place the CTAs are one cluster, with its barrier between the scan and the
+// Two dependent reads (the lengths; then the stack or the table) and the stores bound it: latency.  A step of 256 requests 3.5 us, 43000 tokens of
+// 48 prompts 5.3, the return of 900 requests' 95000 pages 5.2.  Every CTA scans the lengths for itself and stores its share.  Where lengths and counter are updated in place the CTAs are one cluster, with its barrier between the scan and the
 // stores; else any number of them.
 constexpr int PG_THREADS = 1024, PG_MAX_B = LB200_PAGED_MAX_REQUESTS, PG_AHEAD = 4;  // entries of a thread that are on their way together
 
@@ -255,7 +255,7 @@ int launch_pages(void (*kern)(PagesArgs, bool), const PagesArgs &a, size_t smem,
 // y = x rsqrt(mean x^2 + eps) w over the D elements of a head (no weight: y = x), then the first R of them in pairs (a, b):
 //   (a cos t - b sin t, a sin t + b cos t) factor,   t = position * inv_freq[i],   pair i = (i, i + R / 2) or (2 i, 2 i + 1).
 // f32 from the operand to the one rounding at the end; t in f64 (200000 positions far, an f32 angle is off by 0.01), reduced there to
-// half a turn for the f32 functions.  The angles are the same for every head of a token, so a CTA takes a token and computes each once.
+// half a turn for the f32 functions.  The angles are the same for every head of a token, so each is computed once.
 struct RotateArgs {
   const void *q, *k, *v, *qw, *kw;
   void *q_out, *k_out, *v_out;            // k_out: dense, or the cache's keys with slots
@@ -278,6 +278,8 @@ __device__ __forceinline__ float2 cos_sin(long long pos, double freq) {
 
 constexpr int RT_THREADS = 256, RT_MAX_D = 256;
 
+// Any addresses: a CTA takes a token, a warp a head, a lane every 32nd element; pairs meet in shared memory.  (8192 tokens of 48 bf16 heads of 128:
+// 157 us, where the kernel below takes 36.5.)
 template <typename T>
 __global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) {
   __shared__ float trig[RT_MAX_D];  // cos, sin of R / 2 angles
@@ -347,8 +349,10 @@ __global__ void __launch_bounds__(RT_THREADS) qk_norm_rope_kernel(RotateArgs a) 
 // a head is read and written once, in whole sectors, its mean square is log2(lg) shuffles, and an angle's sine and cosine, times the weights,
 // stay in registers for all heads of the token: with f, g the lane's chunks and r = rsqrt(mean square + eps)
 //   f' = r (f (w_f cos) - g (w_g sin)),  g' = r (f (w_f sin) + g (w_g cos)),
-// two elements to an instruction (f32x2).  Bound by the memory, 2 (NH + 2 KH) D elements per token, with half as many instructions again as
-// the issue slots that takes: hence the pairs, and a pass each for queries, keys and values without a choice inside.
+// two elements to an instruction (f32x2).  Bound by the memory, 2 (NH + 2 KH) D elements per token, and nearly by the issue slots (2800
+// instructions per token of 48 heads of 128, 1000 of them whatever the head size): 8192 such tokens in bf16 (201 MB) 36.5 us, 5.5 TB/s; 1037 in f32
+// 9.6 us, 5.3 TB/s.  Loads into registers two rounds ahead instead of the ring: 45.7 us; a choice of kind at every head: 69 us; registers
+// for five or six CTAs an SM: 43 and 57 us (spills); 16 or 1000 warps an SM instead of RC_SLOTS: 40.6, 38.4 us.
 constexpr int RC_WARPS = 4, RC_AHEAD = 6, RC_SLOTS = 32;  // rounds of heads that are on their way together; warps on an SM
 
 struct Chunks {
@@ -525,115 +529,115 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
   };
 #pragma unroll 1
   for (; t < a.T; t += stride) {
-  int page = 0, row = 0;
-  if (slot >= a.rows && a.slots) {
-    if (lane == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
-    slot = -1;
-  }
-  if (slot >= 0 && a.slots) page = a.rows <= 0x7fffffffll ? a.page.div((int)slot) : (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
-  if (kind0 < 2) {
-    __syncwarp();  // (the token before is done with its angles)
-    for (int i = lane; i < half; i += 32) {
-      const float2 cs = cos_sin(pos, a.inv_freq[i]);
-      trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
+    int page = 0, row = 0;
+    if (slot >= a.rows && a.slots) {
+      if (lane == 0) atomicOr(&g_step_status, (unsigned)PAGED_SLOT);
+      slot = -1;
     }
-    __syncwarp();
-  }
-  const bool placed = slot >= 0;
-  if (t + stride < a.T) pos = a.positions[t + stride], slot = a.slots ? a.slots[t + stride] : 0;
+    if (slot >= 0 && a.slots) page = a.rows <= 0x7fffffffll ? a.page.div((int)slot) : (int)(slot / a.page.d), row = (int)(slot - (long long)page * a.page.d);
+    if (kind0 < 2) {
+      __syncwarp();  // (the token before is done with its angles)
+      for (int i = lane; i < half; i += 32) {
+        const float2 cs = cos_sin(pos, a.inv_freq[i]);
+        trig[warp][i] = make_float2(cs.x * a.factor, cs.y * a.factor);
+      }
+      __syncwarp();
+    }
+    const bool placed = slot >= 0;
+    if (t + stride < a.T) pos = a.positions[t + stride], slot = a.slots ? a.slots[t + stride] : 0;
 #pragma unroll 1
-  for (int kind = kind0; kind < kinds; kind++) {
-    to = target(kind, page, row), kept = kind == 0 || placed;
-    const T *const w = static_cast<const T *>(kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr);
-    if (kind == 2 || !kept) {  // copied as they are, or passed over
-      while (to.left + hl > 0) {
-        Raw<CB> x, y;
-        cp_async_wait<RC_AHEAD - 1>();
-        take(x, y);
-        put(x, y);
-        fetch();
-      }
-      continue;
-    }
-    if (to.left + hl <= 0) continue;
-    // what f and g are multiplied by: f' = f ff + g gf, g' = f fg + g gg (halves); per chunk x' = x ff + swapped x gf (neighbours: chunk g has fg, gg)
-    uint64_t ff[V], gf[V], fg[V], gg[V];
-    unsigned turned = 0;  // BETWEEN: bit j: pair j of the first chunk turns; V + j: of the second
-    {
-      Raw<CB> w0{}, w1{};
-      uint64_t wf[V], wg[V];
-      if (w && c0 >= 0) w0 = ld_raw<CB>(w + c0 * E);
-      if (w && c1 >= 0) w1 = ld_raw<CB>(w + c1 * E);
-      unpack<T, CB>(w0, wf), unpack<T, CB>(w1, wg);
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        if (!w) wf[j] = wg[j] = two(1.f, 1.f);
-        if constexpr (BETWEEN) {
-          const int i0 = c0 * V + j, i1 = c1 * V + j;
-          const bool on0 = c0 >= 0 && i0 < half, on1 = c1 >= 0 && i1 < half;
-          const float2 p = on0 ? trig[warp][i0] : make_float2(1.f, 0.f), q = on1 ? trig[warp][i1] : make_float2(1.f, 0.f);
-          turned |= (unsigned)on0 << j | (unsigned)on1 << (V + j);
-          ff[j] = mul2(wf[j], two(p.x, p.x)), gf[j] = two(-hi(wf[j]) * p.y, lo(wf[j]) * p.y);
-          gg[j] = mul2(wg[j], two(q.x, q.x)), fg[j] = two(-hi(wg[j]) * q.y, lo(wg[j]) * q.y);
-        } else {
-          const float2 p = turns ? trig[warp][c0 * E + 2 * j] : make_float2(1.f, 0.f), q = turns ? trig[warp][c0 * E + 2 * j + 1] : make_float2(1.f, 0.f);
-          ff[j] = mul2(wf[j], two(p.x, q.x)), gf[j] = mul2(wg[j], two(-p.y, -q.y)), fg[j] = mul2(wf[j], two(p.y, q.y)), gg[j] = mul2(wg[j], two(p.x, q.x));
-        }
-      }
-    }
-    while (to.left + hl > 0) {
-      // two rounds side by side, if the kind has two more: a round alone is a chain of some 400 cycles
-      const bool both = to.left + hl > hop;
-      if (both) cp_async_wait<RC_AHEAD - 2>();
-      else cp_async_wait<RC_AHEAD - 1>();
-      uint64_t f[2][V], g[2][V];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        Raw<CB> x{}, y{};
-        if (i == 0 || both) take(x, y);
-        unpack<T, CB>(x, f[i]), unpack<T, CB>(y, g[i]);
-      }
-      if (w) {
-        float ss[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          uint64_t s0 = mul2(f[i][0], f[i][0]), s1 = mul2(g[i][0], g[i][0]);
-#pragma unroll
-          for (int j = 1; j < V; j++) s0 = fma2(f[i][j], f[i][j], s0), s1 = fma2(g[i][j], g[i][j], s1);
-          ss[i] = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
-        }
-        for (int o = ch.lg >> 1; o > 0; o >>= 1) {
-          const float p = __shfl_xor_sync(0xffffffffu, ss[0], o), q = __shfl_xor_sync(0xffffffffu, ss[1], o);
-          ss[0] += p, ss[1] += q;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const float inv = rsqrtf(ss[i] * ch.over_d + a.eps);
-          const uint64_t inv2 = two(inv, inv);
-#pragma unroll
-          for (int j = 0; j < V; j++) f[i][j] = mul2(f[i][j], inv2), g[i][j] = mul2(g[i][j], inv2);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        uint64_t u[V], z[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          u[j] = mul2(f[i][j], ff[j]), z[j] = mul2(g[i][j], gg[j]);
-          if constexpr (BETWEEN) {
-            if (turned >> j & 1) u[j] = fma2(two(hi(f[i][j]), lo(f[i][j])), gf[j], u[j]);
-            if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[i][j]), lo(g[i][j])), fg[j], z[j]);
-          } else if (turns) {
-            u[j] = fma2(g[i][j], gf[j], u[j]), z[j] = fma2(f[i][j], fg[j], z[j]);
-          }
-        }
-        if (i == 0 || both) {
-          put(packed<T, CB>(u), packed<T, CB>(z));
+    for (int kind = kind0; kind < kinds; kind++) {
+      to = target(kind, page, row), kept = kind == 0 || placed;
+      const T *const w = static_cast<const T *>(kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr);
+      if (kind == 2 || !kept) {  // copied as they are, or passed over
+        while (to.left + hl > 0) {
+          Raw<CB> x, y;
+          cp_async_wait<RC_AHEAD - 1>();
+          take(x, y);
+          put(x, y);
           fetch();
         }
+        continue;
+      }
+      if (to.left + hl <= 0) continue;
+      // what f and g are multiplied by: f' = f ff + g gf, g' = f fg + g gg (halves); per chunk x' = x ff + swapped x gf (neighbours: chunk g has fg, gg)
+      uint64_t ff[V], gf[V], fg[V], gg[V];
+      unsigned turned = 0;  // BETWEEN: bit j: pair j of the first chunk turns; V + j: of the second
+      {
+        Raw<CB> w0{}, w1{};
+        uint64_t wf[V], wg[V];
+        if (w && c0 >= 0) w0 = ld_raw<CB>(w + c0 * E);
+        if (w && c1 >= 0) w1 = ld_raw<CB>(w + c1 * E);
+        unpack<T, CB>(w0, wf), unpack<T, CB>(w1, wg);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          if (!w) wf[j] = wg[j] = two(1.f, 1.f);
+          if constexpr (BETWEEN) {
+            const int i0 = c0 * V + j, i1 = c1 * V + j;
+            const bool on0 = c0 >= 0 && i0 < half, on1 = c1 >= 0 && i1 < half;
+            const float2 p = on0 ? trig[warp][i0] : make_float2(1.f, 0.f), q = on1 ? trig[warp][i1] : make_float2(1.f, 0.f);
+            turned |= (unsigned)on0 << j | (unsigned)on1 << (V + j);
+            ff[j] = mul2(wf[j], two(p.x, p.x)), gf[j] = two(-hi(wf[j]) * p.y, lo(wf[j]) * p.y);
+            gg[j] = mul2(wg[j], two(q.x, q.x)), fg[j] = two(-hi(wg[j]) * q.y, lo(wg[j]) * q.y);
+          } else {
+            const float2 p = turns ? trig[warp][c0 * E + 2 * j] : make_float2(1.f, 0.f), q = turns ? trig[warp][c0 * E + 2 * j + 1] : make_float2(1.f, 0.f);
+            ff[j] = mul2(wf[j], two(p.x, q.x)), gf[j] = mul2(wg[j], two(-p.y, -q.y)), fg[j] = mul2(wf[j], two(p.y, q.y)), gg[j] = mul2(wg[j], two(p.x, q.x));
+          }
+        }
+      }
+      while (to.left + hl > 0) {
+        // two rounds side by side, if the kind has two more: a round alone is a chain of some 400 cycles
+        const bool both = to.left + hl > hop;
+        if (both) cp_async_wait<RC_AHEAD - 2>();
+        else cp_async_wait<RC_AHEAD - 1>();
+        uint64_t f[2][V], g[2][V];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          Raw<CB> x{}, y{};
+          if (i == 0 || both) take(x, y);
+          unpack<T, CB>(x, f[i]), unpack<T, CB>(y, g[i]);
+        }
+        if (w) {
+          float ss[2];
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            uint64_t s0 = mul2(f[i][0], f[i][0]), s1 = mul2(g[i][0], g[i][0]);
+#pragma unroll
+            for (int j = 1; j < V; j++) s0 = fma2(f[i][j], f[i][j], s0), s1 = fma2(g[i][j], g[i][j], s1);
+            ss[i] = (lo(s0) + hi(s0)) + (lo(s1) + hi(s1));
+          }
+          for (int o = ch.lg >> 1; o > 0; o >>= 1) {
+            const float p = __shfl_xor_sync(0xffffffffu, ss[0], o), q = __shfl_xor_sync(0xffffffffu, ss[1], o);
+            ss[0] += p, ss[1] += q;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const float inv = rsqrtf(ss[i] * ch.over_d + a.eps);
+            const uint64_t inv2 = two(inv, inv);
+#pragma unroll
+            for (int j = 0; j < V; j++) f[i][j] = mul2(f[i][j], inv2), g[i][j] = mul2(g[i][j], inv2);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          uint64_t u[V], z[V];
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            u[j] = mul2(f[i][j], ff[j]), z[j] = mul2(g[i][j], gg[j]);
+            if constexpr (BETWEEN) {
+              if (turned >> j & 1) u[j] = fma2(two(hi(f[i][j]), lo(f[i][j])), gf[j], u[j]);
+              if (turned >> (V + j) & 1) z[j] = fma2(two(hi(g[i][j]), lo(g[i][j])), fg[j], z[j]);
+            } else if (turns) {
+              u[j] = fma2(g[i][j], gf[j], u[j]), z[j] = fma2(f[i][j], fg[j], z[j]);
+            }
+          }
+          if (i == 0 || both) {
+            put(packed<T, CB>(u), packed<T, CB>(z));
+            fetch();
+          }
+        }
       }
     }
-  }
   }
 }
 
