@@ -38,12 +38,17 @@ __device__ __forceinline__ float ex2(float x) {  // relative error 2^-22; result
   return y;
 }
 
-// A score in units of log2 e.  tanh z = 1 - 2 / (e^(2 z) + 1): absolute error of a few 2^-24, which is what a score's error counts by.
+// A score in units of log2 e.  tanh z = 1 - 2 / (e^(2 z) + 1), whose absolute error is a few 2^-24: nothing for a z of the order of 1, but scores far
+// below the cap would lose cap 2^-23 of themselves; below 0.35 its Taylor series to z^9 instead (the next term is 2^-22 of z there).
 struct Scorer {
-  float sc, cap;  // without a cap: scale log2 e; with one: 2 log2 e scale / cap, and cap log2 e
-  __device__ Scorer(float scale, float softcap) : sc(softcap > 0.f ? 2.f * LOG2E * scale / softcap : scale * LOG2E), cap(softcap * LOG2E) {}
+  float sc, cap;  // without a cap: scale log2 e; with one: scale / cap, and cap log2 e
+  __device__ Scorer(float scale, float softcap) : sc(softcap > 0.f ? scale / softcap : scale * LOG2E), cap(softcap * LOG2E) {}
   __device__ __forceinline__ float operator()(float dot) const { return cap > 0.f ? capped(dot * sc) : dot * sc; }
-  __device__ __forceinline__ float capped(float x) const { return cap - cap * 2.f * __fdividef(1.f, ex2(x) + 1.f); }
+  __device__ __forceinline__ float capped(float z) const {
+    const float far = 1.f - 2.f * __fdividef(1.f, ex2(z * (2.f * LOG2E)) + 1.f), y = z * z;
+    const float near = z * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    return cap * (fabsf(z) < 0.35f ? near : far);
+  }
 };
 
 // ------------------------------------------------------------------------------------ any head size, any stride

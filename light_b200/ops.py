@@ -938,8 +938,8 @@ def _pages_args(op: str, block_table: torch.Tensor, lens: torch.Tensor, free_pag
     _i32(op, block_table.device, lens=lens, free_pages=free_pages, free_count=free_count)
     if lens.numel() != B or free_pages.dim() != 1 or free_pages.numel() == 0 or free_count.numel() != 1:
         raise ValueError(f"ops.{op}: lens {tuple(lens.shape)}, free_pages {tuple(free_pages.shape)}, free_count {tuple(free_count.shape)} for {B} requests")
-    if page_size < 1:
-        raise ValueError(f"ops.{op}: page size {page_size}")
+    if not 1 <= page_size < 1 << 31 or free_pages.numel() >= 1 << 31:
+        raise ValueError(f"ops.{op}: page size {page_size}, {free_pages.numel()} entries of free_pages")
     return dev, B, _lib.PagedPages(block_table=block_table.data_ptr(), lens=lens.data_ptr(), free_pages=free_pages.data_ptr(), free_count=free_count.data_ptr(),
                                    table_stride=block_table.stride(0) if B > 1 else W, B=B, W=W, page_size=page_size, capacity=free_pages.numel())
 

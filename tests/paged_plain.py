@@ -97,9 +97,9 @@ def attention(q, k_cache, v_cache, table, lens, scale, window=0, softcap=0.0, ro
             p = torch.softmax(s, -1)
             out[b, h * G:(h + 1) * G] = p @ v
             spread = p @ v.abs()
-            # a score: D products summed in f32 (tensor cores cut, they do not round: a whole step each), scaled, capped; its error is p's relative
-            # one, exp2 adds two steps, and rescaling at a new maximum one each time, 64 times at most; the sums over the keys: one step per key
+            # a score: D products summed in f32 (tensor cores cut, they do not round: a whole step each), scaled, capped (a tanh right to 16 steps of its
+            # value, and no larger than the score); its error is p's relative one, exp2 adds two steps, and rescaling at a new maximum one each time, 64 times at most; the sums over the keys: one step per key
             # in the worst order.  Numerator and denominator have them each.
-            e = (D + 8) * 2.0 ** -23 * size + 8 * softcap * 2.0 ** -24 + 70 * 2.0 ** -23 + min(len(j), 4096) * 2.0 ** -24
+            e = (D + 8 + (8 if softcap else 0)) * 2.0 ** -23 * size + 70 * 2.0 ** -23 + min(len(j), 4096) * 2.0 ** -24
             bound[b, h * G:(h + 1) * G] = u * p.matmul(v).abs() + 2 * (u_p + e) * spread + LEAST[q.dtype]
     return out, bound

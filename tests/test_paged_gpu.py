@@ -72,7 +72,7 @@ def test_attention_one_sequence(cuda, dtype, n):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window", [1, 7, 64, 100, 1 << 30])
-@pytest.mark.parametrize("softcap", [0.0, 2.0, 50.0])
+@pytest.mark.parametrize("softcap", [0.0, 0.01, 2.0, 50.0, 1e6])
 def test_attention_window_and_cap(cuda, dtype, window, softcap):
     _check(*_case(cuda, dtype, [300, 5, 0, 64, 65, 1], 2, 5, 128, 24, seed=window % 97), window=window, softcap=softcap)
 
@@ -444,7 +444,7 @@ def test_page_refusals(cuda):
     for call, bad in [(adv, b) for b in (dict(new_lens=i[:1]), dict(new_lens=i.long()), dict(tokens=-1))] + [(rel, b) for b in (dict(done=i), dict(done=(i > 0)[:1]), dict(done=(i > 0).cpu()))] + \
             [(c, b) for c in (adv, rel) for b in (dict(block_table=T.long()), dict(block_table=T.t()), dict(block_table=T[:, :0]), dict(block_table=T[0]), dict(block_table=T[:1].expand(2, 2)),
                                                   dict(lens=i[:1]), dict(lens=i.long()), dict(lens=_t([1, 1, 1, 1], cuda)[::2]), dict(free_pages=f.long()), dict(free_pages=f[:0]),
-                                                  dict(free_count=f), dict(page_size=0), dict(lens=i.cpu()))]:
+                                                  dict(free_count=f), dict(page_size=0), dict(page_size=1 << 32), dict(lens=i.cpu()))]:
         with pytest.raises(ValueError, match="ops.Paged"):
             call(**bad)
     with pytest.raises(_lib.Light200Error, match="at most 8192"):
