@@ -383,7 +383,7 @@ LB200_API int light_b200_decode_attn(const lb200_decode_attn_args *args, int dev
 /* 0, or of the calls so far on this device (synchronises): bit 0: a length outside [0, W page_size] reached the attention (it used the
  * nearest inside); bit 1: a page outside [0, pages) did (its keys counted as absent); bit 2: a slot at or beyond pages * page_size
  * reached qk_norm_rope (nothing was written for it); bit 3: paged_advance left a request without its tokens, or it or
- * paged_release met a negative length or a count outside [0, capacity]. */
+ * paged_release met a negative length or a count outside [0, capacity], or paged_release a length beyond the table (it pushed W pages). */
 LB200_API int light_b200_paged_status(int device);
 
 #define LB200_PAGED_MAX_REQUESTS 8192
@@ -416,7 +416,8 @@ LB200_API int light_b200_paged_release(const lb200_paged_pages *args, int device
  * of them then rotated in pairs by positions[t] * inv_freq[i] and multiplied by factor; pair i is (i, i + rotary / 2), or (2 i, 2 i + 1)
  * with interleaved.  Angles in f64, the rest in f32, rounded once.  (Reference ops.RMSNorm over a head and ops.RoPE, ops/norm.go:69-111,
  * ops/rope.go:30-77, as launches of their own.)
- * With slots: key and value (copied) of token t go to row slots[t] of the cache instead of k_out; a negative slot writes nothing. */
+ * With slots: key and value (copied) of token t go to row slots[t] of the cache instead of k_out; a negative slot writes nothing;
+ * tokens that share a slot leave a mix of their elements. */
 typedef struct lb200_qk_norm_rope_args {
   const void *q, *k, *v;      /* (T, NH, D), (T, KH, D), (T, KH, D): token and head strides below; v with slots only       */
   const void *q_weight, *k_weight; /* (D) at dtype, or NULL each                                                           */
@@ -434,7 +435,7 @@ typedef struct lb200_qk_norm_rope_args {
 LB200_API int light_b200_qk_norm_rope(const lb200_qk_norm_rope_args *args, int device, void *stream);
 
 /* out (B, NH, D) = softmax(s) V over the keys [max(0, lens[b] - window), lens[b]) of sequence b (window 0: all), s = scale q.k, with
- * softcap > 0 softcap * tanh(scale q.k / softcap).  lens[b] counts the new token, whose key and value are in the cache already.  A
+ * softcap (1e-20 to 1e20, or 0 for none) softcap * tanh(scale q.k / softcap).  lens[b] counts the new token, whose key and value are in the cache already.  A
  * sequence without keys, or whose keys all score -inf, gives zeros.  scratch: device memory of light_b200_paged_attn_scratch_bytes or more, 256-byte aligned,
  * uninitialised, which nothing else uses until the call has run; 0 bytes where the call has no use for any. */
 typedef struct lb200_paged_attn_args {

@@ -416,7 +416,7 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const int dev = q.t->get_device();
   const auto dt = q.t->scalar_type();
   const int64_t T = q.t->size(0), NH = q.t->size(1), D = q.t->size(2);
-  NEED(act_of(*q.t) >= 0 && T > 0 && D > 0 && heads_of(*q.t, T, D, dt, dev) && heads_of(*k.t, T, D, dt, dev));
+  NEED(act_of(*q.t) >= 0 && T > 0 && D > 0 && D <= 256 && NH < (1ll << 31) && heads_of(*q.t, T, D, dt, dev) && heads_of(*k.t, T, D, dt, dev) && k.t->size(1) < (1ll << 31));
   const int64_t KH = k.t->size(1), R = 2 * freq.t->numel();
   NEED(pos.t->is_cuda() && pos.t->scalar_type() == at::kLong && pos.t->dim() == 1 && pos.t->size(0) == T && pos.t->is_contiguous() && pos.t->get_device() == dev);
   NEED(cuda_contig(*freq.t) && freq.t->scalar_type() == at::kDouble && freq.t->dim() == 1 && R <= D && freq.t->get_device() == dev);
@@ -427,7 +427,7 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   for (int i = 9; i < 12; i++) NEED((a[i] != Py_None) == cached);
   lb200_qk_norm_rope_args p{};
   if (cached) {
-    NEED(v.ok(a[9]) && kc.ok(a[10]) && vc.ok(a[11]) && sl.ok(a[12]) && heads_of(*v.t, T, D, dt, dev) && v.t->size(1) == KH && cache_of(*kc.t, *vc.t, KH, D, dt, dev, true));
+    NEED(v.ok(a[9]) && kc.ok(a[10]) && vc.ok(a[11]) && sl.ok(a[12]) && heads_of(*v.t, T, D, dt, dev) && v.t->size(1) == KH && cache_of(*kc.t, *vc.t, KH, D, dt, dev, true) && kc.t->size(2) < (1ll << 31));
     NEED(sl.t->is_cuda() && sl.t->scalar_type() == at::kLong && sl.t->dim() == 1 && sl.t->size(0) == T && sl.t->is_contiguous() && sl.t->get_device() == dev);
     p.v = v.t->const_data_ptr(), p.slots = sl.t->const_data_ptr<int64_t>(), p.k_out = kc.t->data_ptr(), p.v_out = vc.t->data_ptr();
     for (int i = 0; i < 3; i++) p.k_cache_stride[i] = kc.t->stride(i), p.v_cache_stride[i] = vc.t->stride(i);
@@ -459,7 +459,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const int dev = q.t->get_device();
   const auto dt = q.t->scalar_type();
   const int64_t B = q.t->size(0), NH = q.t->size(1), D = q.t->size(2), KH = k.t->size(1), stride = table_of(*t.t);
-  NEED(act_of(*q.t) >= 0 && B > 0 && D > 0 && KH > 0 && NH % KH == 0 && heads_of(*q.t, B, D, dt, dev) && cache_of(*k.t, *v.t, KH, D, dt, dev, false));
+  NEED(act_of(*q.t) >= 0 && B > 0 && B < (1ll << 31) && D > 0 && D <= 256 && KH > 0 && NH < (1ll << 31) && NH % KH == 0 && heads_of(*q.t, B, D, dt, dev) && cache_of(*k.t, *v.t, KH, D, dt, dev, false));
   const int64_t step = q.t->element_size();
   NEED(!(((uintptr_t)q.t->const_data_ptr() | (uintptr_t)(B > 1 ? q.t->stride(0) * step : 0) | (uintptr_t)(NH > 1 ? q.t->stride(1) * step : 0)) & 15));
   NEED(stride > 0 && t.t->size(0) == B && t.t->size(1) < (1ll << 31) && t.t->get_device() == dev && l.t->dim() == 1 && i32_of(*l.t, dev, B) && k.t->size(2) < (1ll << 31));

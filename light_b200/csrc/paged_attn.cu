@@ -41,7 +41,7 @@ __device__ __forceinline__ float ex2(float x) {  // relative error 2^-22; result
 // A score in units of log2 e.  tanh z = 1 - 2 / (e^(2 z) + 1), whose absolute error is a few 2^-24: nothing for a z of the order of 1, but scores far
 // below the cap would lose cap 2^-23 of themselves; below 0.35 its Taylor series to z^9 instead (the next term is 2^-22 of z there).
 struct Scorer {
-  float sc, cap;  // without a cap: scale log2 e; with one: scale / cap, and cap log2 e
+  float sc, cap;  // without a cap: scale log2 e; with one, of 1e-20 to 1e20 (neither overflows): scale / cap, and cap log2 e
   __device__ Scorer(float scale, float softcap) : sc(softcap > 0.f ? scale / softcap : scale * LOG2E), cap(softcap * LOG2E) {}
   __device__ __forceinline__ float operator()(float dot) const { return cap > 0.f ? capped(dot * sc) : dot * sc; }
   __device__ __forceinline__ float capped(float z) const {
@@ -1207,7 +1207,6 @@ int launch_dtype(const SplitArgs &s, const Cut &c, int dtype, cudaStream_t st) {
   }
   if constexpr (DP < 256) return launch_split<F32Block<DP, 8>>(s, c, st);
   return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: %d heads per unit", c.HEADS);
-
 }
 
 }  // namespace
@@ -1220,7 +1219,7 @@ int paged_attn_check(const lb200_paged_attn_args *p) {
   if (!p) return fail(LB200_E_NULL, "light_b200: paged_decode_attn: null argument block");
   if (p->dtype != LB200_F32 && p->dtype != LB200_BF16 && p->dtype != LB200_F16) return fail(LB200_E_DTYPE, "light_b200: paged_decode_attn: element type %d", p->dtype);
   if (p->B < 0 || p->NH <= 0 || p->KH <= 0 || p->NH % p->KH || p->D <= 0 || p->D > PL_MAX_D || p->page_size <= 0 || p->W <= 0 || p->pages <= 0 || p->window < 0 ||
-      p->table_stride < p->W || !(p->softcap >= 0.f))
+      p->table_stride < p->W || !(p->softcap == 0.f || (p->softcap >= 1e-20f && p->softcap <= 1e20f)))
     return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: B %d NH %d KH %d D %d (at most %d) page size %d table %d pages %lld window %d softcap %g", p->B, p->NH, p->KH,
                 p->D, PL_MAX_D, p->page_size, p->W, (long long)p->pages, p->window, (double)p->softcap);
   if ((long long)p->W * p->page_size > 0x7ffffc00ll || p->pages > 0x7fffffffll || (long long)p->B * p->NH > 0x7fffffffll)

@@ -15,8 +15,8 @@ __device__ unsigned int g_step_status = 0;
 // request with starts_b <= i < starts_{b + 1}: a binary search in shared memory.
 //
 // Two dependent reads (the lengths; then the stack or the table) and the stores bound it: latency.  A step of 256 requests 3.5 us, 43000 tokens of
-// 48 prompts 5.3, the return of 900 requests' 95000 pages 5.2.  Every CTA scans the lengths for itself and stores its share.  Where lengths and counter are updated in place the CTAs are one cluster, with its barrier between the scan and the
-// stores; else any number of them.
+// 48 prompts 5.3, the return of 900 requests' 95000 pages 5.2.  Every CTA scans the lengths for itself and stores its share.  Where lengths and
+// counter are updated in place the CTAs are one cluster, with its barrier between the scan and the stores; else any number of them.
 constexpr int PG_THREADS = 1024, PG_MAX_B = LB200_PAGED_MAX_REQUESTS, PG_AHEAD = 4;  // entries of a thread that are on their way together
 
 struct PagesArgs {
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, 
       keep[b] = done ? 0 : n;
       if (done) {
         const int q = a.page.div(max(n, 0));
-        odd |= n < 0;
+        odd |= n < 0 || n > a.W * a.page.d;
         held = min(q + (q * a.page.d < n), a.W);
       }
     }

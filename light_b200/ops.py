@@ -938,8 +938,8 @@ def _pages_args(op: str, block_table: torch.Tensor, lens: torch.Tensor, free_pag
     _i32(op, block_table.device, lens=lens, free_pages=free_pages, free_count=free_count)
     if lens.numel() != B or free_pages.dim() != 1 or free_pages.numel() == 0 or free_count.numel() != 1:
         raise ValueError(f"ops.{op}: lens {tuple(lens.shape)}, free_pages {tuple(free_pages.shape)}, free_count {tuple(free_count.shape)} for {B} requests")
-    if not 1 <= page_size < 1 << 31 or free_pages.numel() >= 1 << 31:
-        raise ValueError(f"ops.{op}: page size {page_size}, {free_pages.numel()} entries of free_pages")
+    if not 1 <= page_size < 1 << 31 or max(free_pages.numel(), B, W) >= 1 << 31:
+        raise ValueError(f"ops.{op}: page size {page_size}, {free_pages.numel()} entries of free_pages, block_table {tuple(block_table.shape)}")
     return dev, B, _lib.PagedPages(block_table=block_table.data_ptr(), lens=lens.data_ptr(), free_pages=free_pages.data_ptr(), free_count=free_count.data_ptr(),
                                    table_stride=block_table.stride(0) if B > 1 else W, B=B, W=W, page_size=page_size, capacity=free_pages.numel())
 
@@ -1033,6 +1033,8 @@ def _check_paged_cache(op: str, k_cache: torch.Tensor, v_cache: torch.Tensor, KH
         raise ValueError(f"ops.{op}: want caches (pages, {KH}, page size, {D}), got {tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
     if k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.device != device or v_cache.device != device:
         raise ValueError(f"ops.{op}: caches {k_cache.dtype} on {k_cache.device} / {v_cache.dtype} on {v_cache.device}, want {dtype} on {device}")
+    if max(k_cache.shape) >= 1 << 31:
+        raise ValueError(f"ops.{op}: caches {tuple(k_cache.shape)}: want fewer than 2^31 of each")
     for c in (k_cache, v_cache):
         if D > 1 and c.stride(3) != 1:
             raise ValueError(f"ops.{op}: the {D} elements of a cache row must lie side by side, strides are {c.stride()}")
@@ -1045,8 +1047,8 @@ def QKNormRoPE(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fr
     and values to their rows, in one launch (light_b200_qk_norm_rope): q (T, NH, D), k, v (T, KH, D) F32 / BF16 / F16, any token and head
     strides (views of one projection); positions (T,) I64; inv_freq F64 (rotary / 2) and factor from ops.RoPEFrequencies: the first
     rotary elements of a head turn, in pairs (i, i + rotary / 2), or (2 i, 2 i + 1) with `interleaved`.  Caches (pages, KH, page size, D)
-    of any order, slots (T,) I64 (ops.PagedAdvance): key and value of a token with a negative slot go nowhere; of two tokens with one slot
-    either may stay.  Returns (q, k), k None where it went to the cache.  No gradients."""
+    of any order, slots (T,) I64 (ops.PagedAdvance): key and value of a token with a negative slot go nowhere; tokens that share a
+    slot leave a mix of their elements.  Returns (q, k), k None where it went to the cache.  No gradients."""
     r = _host.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, factor, v, k_cache, v_cache, slots)
     if r is not None:
         return r
@@ -1057,6 +1059,8 @@ def QKNormRoPE(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fr
         raise ValueError(f"ops.QKNormRoPE: dtype {q.dtype} unsupported (F32 / BF16 / F16)")
     (T, NH, D), KH = q.shape, k.shape[1]
     dev = _dev(q, "QKNormRoPE")
+    if max(T, NH, KH, D) >= 1 << 31:
+        raise ValueError(f"ops.QKNormRoPE: q {tuple(q.shape)}, k {tuple(k.shape)}: want fewer than 2^31 of each")
     if positions.dtype != torch.int64 or tuple(positions.shape) != (T,) or positions.device != q.device:
         raise ValueError(f"ops.QKNormRoPE: positions must be I64 ({T},) on {q.device}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > D or inv_freq.device != q.device:
@@ -1098,7 +1102,7 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """Attention of one new token of each sequence over a paged cache (light_b200_paged_decode_attn; ops.DecodeAttention is its counterpart over
     contiguous caches of one position): q (B, NH, D) F32 / BF16 / F16, caches (pages, KH, page size, D) of q's type and any order of page,
     head and row, block_table (B, W) I32, lens (B,) I32 valid keys of each sequence, the new token's among them -> (B, NH, D).  window: the
-    last `window` keys only; softcap: scores softcap * tanh(scale q.k / softcap).  A sequence without keys (or whose scores are all -inf)
+    last `window` keys only; softcap (0, or 1e-20 to 1e20): scores softcap * tanh(scale q.k / softcap).  A sequence without keys (or whose scores are all -inf)
     gives zeros; lengths beyond the table and pages outside the cache are reported by ops.paged_status.  No gradients."""
     y = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap)
     if y is not None:
@@ -1117,9 +1121,11 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"ops.PagedDecodeAttention: block_table must be I32 ({B}, W) on {q.device}, got {block_table.dtype} {tuple(block_table.shape)} on {block_table.device}")
     if lens.dtype != torch.int32 or tuple(lens.shape) != (B,) or lens.device != q.device:
         raise ValueError(f"ops.PagedDecodeAttention: lens must be I32 ({B},) on {q.device}, got {lens.dtype} {tuple(lens.shape)} on {lens.device}")
-    if window < 0 or not softcap >= 0:
+    if window < 0 or not (softcap == 0 or 1e-20 <= softcap <= 1e20):
         raise ValueError(f"ops.PagedDecodeAttention: window {window}, softcap {softcap}")
     W = block_table.shape[1]
+    if max(B, NH, W) >= 1 << 31:
+        raise ValueError(f"ops.PagedDecodeAttention: q {tuple(q.shape)}, block_table {tuple(block_table.shape)}: want fewer than 2^31 of each")
     qh, lc = _head_rows(q), lens.contiguous()
     step = q.element_size()
     if (qh.data_ptr() | (qh.stride(0) * step if B > 1 else 0) | (qh.stride(1) * step if NH > 1 else 0)) & 15:  # the fast kernels read 16 bytes at a time
@@ -1139,5 +1145,6 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 
 def paged_status(device_index: int = 0) -> int:
     """What the paged operators met on this device so far (light_b200_paged_status; synchronises): 1 a length outside the table, 2 a page outside
-    the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of free pages."""
+    the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of free pages, a length beyond
+    the table at its release."""
     return _lib.lib().light_b200_paged_status(device_index)

@@ -85,6 +85,12 @@ def test_attention_entry_refuses(kw, code):
     assert _lib.lib().light_b200_paged_decode_attn(None, 0, None) == -3
 
 
+@pytest.mark.parametrize("softcap", [float("inf"), 3e38, 1.1e20, 9e-21, 1e-38])
+def test_attention_entry_refuses_caps_that_overflow(softcap):
+    """scale / cap and cap log2 e are f32: an infinite one would turn scores into NaN."""
+    assert _lib.lib().light_b200_paged_decode_attn(C.byref(_attn_args(softcap=softcap)), 0, None) == -2
+
+
 def _rope_args(**kw):
     a = dict(q=256, k=256, q_out=256, k_out=256, positions=256, inv_freq=256, q_stride=(256, 64), k_stride=(128, 64), T=3, dtype=1, NH=4, KH=2, D=64, rotary=64, page_size=1, eps=1e-6,
              factor=1.0)

@@ -233,6 +233,30 @@ def test_attention_refusals(cuda):
     assert call(q[:0], k, v, table[:0], lens[:0], 1.0).shape == (0, 8, 64)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [1e-20, 1e20])
+def test_attention_caps_at_their_ends(cuda, dtype, softcap):
+    _check(*_case(cuda, dtype, [1, 33, 700], 2, 4, 128, 16), softcap=softcap)
+
+
+def test_attention_refuses_caps_that_overflow_and_extents_beyond_31_bits(cuda):
+    q, k, v, table, lens = _case(cuda, torch.bfloat16, [40, 20], 2, 4, 64, 16)
+    call = ops.PagedDecodeAttention
+    for cap in (float("inf"), float("nan"), 3e38, 1e-38):
+        with pytest.raises(ValueError, match="softcap"):
+            call(q, k, v, table, lens, 1.0, softcap=cap)
+    wide = k[:1, :1, :1].expand(1, 1, (1 << 32) + 16, 64)
+    with pytest.raises(ValueError, match="2\\^31"):
+        call(q, wide, wide, table, lens, 1.0)
+    with pytest.raises(ValueError, match="2\\^31"):
+        call(q, k, v, table[:, :1].expand(2, (1 << 32) + 3), lens, 1.0)
+    with pytest.raises(ValueError, match="2\\^31"):
+        call(q[:, :1].expand(2, (1 << 32) + 8, 64), k, v, table, lens, 1.0)
+    pos, freq = torch.zeros(2, dtype=torch.int64, device=cuda), ops.RoPEFrequencies(64, 1e4)[0]
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.QKNormRoPE(q[:, :1].expand(2, (1 << 32) + 8, 64), q, pos, freq)
+
+
 # ---------------------------------------------------------------- norm, rotation, cache rows
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -343,6 +367,25 @@ def test_rotation_slots_outside_are_reported_and_not_written(cuda):
     assert torch.equal(kc, guard) and torch.equal(vc, guard) and ops.paged_status(0) & 4
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [7, 64, 128])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_of_nothing(cuda, dtype, D, interleaved):
+    """No frequencies: norm and the write of the rows alone.  No tokens: nothing."""
+    g = torch.Generator(cuda).manual_seed(D)
+    q, k, v = (torch.randn((19, n, D), generator=g, device=cuda).to(dtype) for n in (5, 2, 2))
+    w = (1 + 0.2 * torch.randn(D, generator=g, device=cuda)).to(dtype)
+    none, pos = torch.empty(0, dtype=torch.float64, device=cuda), torch.arange(19, device=cuda)
+    kc, vc = (torch.zeros((2, 2, 16, D), dtype=dtype, device=cuda) for _ in range(2))
+    got, _ = ops.QKNormRoPE(q, k, pos, none, q_weight=w, eps=1e-5, interleaved=interleaved, v=v, k_cache=kc, v_cache=vc, slots=pos)
+    want, bound = paged_plain.rotated(q, w, 1e-5, pos, none, interleaved, 1.0)
+    assert bool(((got.double() - want).abs() <= bound).all())
+    assert torch.equal(kc.transpose(1, 2).reshape(32, 2, D)[:19], k) and torch.equal(vc.transpose(1, 2).reshape(32, 2, D)[:19], v)
+    kb = kc.clone()
+    got, _ = ops.QKNormRoPE(q[:0], k[:0], pos[:0], none, v=v[:0], k_cache=kc, v_cache=vc, slots=pos[:0])
+    assert got.shape == (0, 5, D) and torch.equal(kc, kb)
+
+
 def test_rotation_refusals(cuda):
     q, k = torch.zeros((3, 4, 64), device=cuda), torch.zeros((3, 2, 64), device=cuda)
     p, f, kc = torch.zeros(3, dtype=torch.int64, device=cuda), torch.ones(32, dtype=torch.float64, device=cuda), torch.zeros((2, 2, 8, 64), device=cuda)
@@ -429,6 +472,39 @@ def test_pages_with_odd_counts_and_lengths(cuda):
     assert n.tolist() == [0, 0] and c.tolist() == [4] and F.tolist() == [4, 5, 6, 7]
     n, c = ops.PagedRelease(T, _t([4800, 17], cuda), _t([1, 0], cuda, torch.bool), _t([0] * 9, cuda), _t([1], cuda), 16)
     assert n.tolist() == [0, 17] and c.tolist() == [4]
+
+
+def test_release_reports_lengths_beyond_the_table(cuda):
+    """(The bit stays set on the device: a child process has it clear.)"""
+    import subprocess
+    import sys
+
+    from helpers import ROOT
+    code = """
+import torch
+from light_b200 import ops
+t = lambda x, d=torch.int32: torch.tensor(x, dtype=d, device="cuda")
+T = t([[4, 5], [7, 8]])
+for n, want in ((32, 0), (33, 8)):
+    lens, count = ops.PagedRelease(T, t([n, 33]), t([1, 0], torch.bool), t([0] * 9), t([1]), 16)
+    assert (lens.tolist(), count.tolist(), ops.paged_status(0)) == ([0, 33], [3], want), n
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)
+
+
+def test_advance_of_no_tokens_and_in_inference_mode(cuda):
+    T, F = _t([[4, -1], [5, -1]], cuda), _t([0, 1, 2], cuda)
+    s = ops.PagedAdvance(T, _t([16, 3], cuda), _t([0, 0], cuda), F, _t([3], cuda), 16, 0)
+    assert s.positions.shape == s.slots.shape == (0,) and s.starts.tolist() == [0, 0, 0] and s.lens.tolist() == [16, 3] and s.free_count.tolist() == [3]
+    with torch.inference_mode():
+        s = ops.PagedAdvance(T, _t([16, 3], cuda), _t([1, 1], cuda), F, _t([3], cuda), 16, 2)
+        s.slots.add_(0)
+        lens, count = ops.PagedRelease(T, s.lens, _t([1, 0], cuda, torch.bool), F, s.free_count, 16)
+    assert s.slots.is_inference() and s.slots.tolist() == [32, 5 * 16 + 3] and T.tolist() == [[4, 2], [5, -1]]
+    assert lens.tolist() == [0, 4] and count.tolist() == [3] and F.tolist() == [0, 1, 4]  # (a stack of three: page 2 has no room)
+    s = ops.PagedAdvance(T, lens, _t([0, 1], cuda), F, count, 16, 1)
+    s.lens.add_(1)
+    assert s.lens.tolist() == [1, 6] and s.granted.tolist() == [0, 1]
 
 
 def test_advance_writes_rows_of_a_wider_table_only(cuda):
