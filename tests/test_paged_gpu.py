@@ -234,6 +234,19 @@ def test_attention_refusals(cuda):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rise", [0.02, 0.4, -0.02, -0.4])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_attention_scores_that_rise_or_fall(cuda, dtype, rise, softcap):
+    """Every key's score a little above (below) the one before: a maximum that lags behind, never by more than it may."""
+    q, k, v, table, lens = _case(cuda, dtype, [1000, 37], 2, 4, 64, 16)
+    q.fill_(0.125)
+    for b, n in enumerate((1000, 37)):
+        for w in range(-(-n // 16)):
+            k[table[b, w]] = ((torch.arange(16 * w, 16 * w + 16, device=cuda) - n / 2) * rise).to(dtype)[None, :, None]
+    _check(q, k, v, table, lens, scale=0.125, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("softcap", [1e-20, 1e20])
 def test_attention_caps_at_their_ends(cuda, dtype, softcap):
     _check(*_case(cuda, dtype, [1, 33, 700], 2, 4, 128, 16), softcap=softcap)
