@@ -143,11 +143,12 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 //     without a key are filled with zeros: a weight of 0 times what lies there must not be NaN.
 //   * Pieces of a unit that was cut are joined in their order, first those of a CTA's warps at its end, in shared memory; what goes on
 //     over CTAs goes to scratch, at most two pieces a CTA, and a second launch joins those: no atomics, the same bits every time.
-// Bound by the memory where sequences are long: one of 131072 keys (537 MB, bf16) 89 us, 6.0 TB/s; eight of 8192 in f32 (537 MB) 90 us.  Of
+// Bound by the memory where sequences are long: one of 131072 keys (537 MB, bf16) 88 us, 6.1 TB/s; eight of 8192 in f32 (537 MB) 90 us.  Of
 // shorter ones by what a launch costs beside its stream: 64 ragged ones (232 MB) 45 us, of which about 6 are the chain of lengths,
 // schedule, pages and first rows (2000 + 1500 + 2000 + 2500 cycles) and 4 the join.
 //   * One wave of CTAs: two, three and four waves of finer runs take 98, 102 and 108 us for the one long sequence, each wave that chain again.
-//   * UNIT 3: 1, 2, 5, 8 give 49.7, 44.5, 45.1, 45.0 us for the 64, and 18.4, 17.6, 20.9, 24.3 for 200 of 300 keys at most (3: 45.2, 18.0).
+//   * UNIT 3: 1, 2, 5, 8 give 49.7, 44.5, 45.1, 45.0 us for the 64, and 18.4, 17.6, 20.9, 24.3 for 200 of 300 keys at most (3: 45.2, 18.0; all of it
+//     before the maximum's slack).
 //   * All four warps of a CTA on the blocks of one unit in turn, with barriers, took 75 us for the 64: two microseconds a unit.
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 4, CLUSTER_WIDE = 8;
 
@@ -203,7 +204,7 @@ __device__ __forceinline__ uint32_t pack(float &a, float &b, __nv_bfloat16) {
 // bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
 //   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
 //   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
-//   A block of 128 dims is about 400 instructions of a warp, 0.65 us by itself; eight warps of an SM fold 8 KB each in 1.4 us, which is the memory's rate.
+//   A block of 128 dims is about 340 instructions of a warp (of 400, with a maximum every block, it took 0.65 us by itself); eight warps of an SM fold 8 KB each in 1.4 us, which is the memory's rate.
 //   P is rounded to the cache's type, as the instruction wants it: 2^-8 (bf16) or 2^-11 of each weight, no more than the output's own rounding;
 //   the sum below the fraction adds the rounded weights, so that they sum to one.
 template <typename T_, int DP_, int NT>
