@@ -204,7 +204,8 @@ __device__ __forceinline__ uint32_t pack(float &a, float &b, __nv_bfloat16) {
 // bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
 //   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
 //   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
-//   A block of 128 dims is about 340 instructions of a warp (of 400, with a maximum every block, it took 0.65 us by itself); eight warps of an SM fold 8 KB each in 1.4 us, which is the memory's rate.
+//   A block of 128 dims is about 340 instructions of a warp (of 400, with a maximum every block, it took 0.65 us by itself); eight warps of an SM
+//   fold 8 KB each in 1.4 us, which is the memory's rate.
 //   P is rounded to the cache's type, as the instruction wants it: 2^-8 (bf16) or 2^-11 of each weight, no more than the output's own rounding;
 //   the sum below the fraction adds the rounded weights, so that they sum to one.
 template <typename T_, int DP_, int NT>
