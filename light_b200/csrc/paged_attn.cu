@@ -201,6 +201,11 @@ __device__ __forceinline__ uint32_t pack(float &a, float &b, __nv_bfloat16) {
   return v;
 }
 
+__device__ __forceinline__ float lds_f16(uint32_t addr) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(addr) : "memory");
+  return __half2float(__ushort_as_half(v));
+}
 // bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
 //   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
 //   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
@@ -208,10 +213,15 @@ __device__ __forceinline__ uint32_t pack(float &a, float &b, __nv_bfloat16) {
 //   fold 8 KB each in 1.4 us, which is the memory's rate.
 //   P is rounded to the cache's type, as the instruction wants it: 2^-8 (bf16) or 2^-11 of each weight, no more than the output's own rounding;
 //   the sum below the fraction adds the rounded weights, so that they sum to one.
+//   f16 has them 2^7 times larger (2^15 at most, with the slack; numerator and denominator share the factor, in all pieces), so that it keeps them down to
+//   2^-21 of the largest to 2^-11 of themselves.  A block with one below that has more products (fold_light): where a key holds nearly all the weight and its
+//   value little, the answer is the sum of many that are lighter than any f16.
 template <typename T_, int DP_, int NT>
 struct MmaBlock {
   using T = T_;
   static constexpr int DP = DP_, KB = 16, HEADS = 8 * NT, ROWB = DP * 2, PR = DP + 4, EXTRA = 0;
+  static constexpr bool HALF = std::is_same<T, __half>::value;
+  static constexpr float UP = HALF ? 7.f : 0.f;
   uint32_t q[DP / 16][NT][2];
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
 
@@ -292,9 +302,27 @@ struct MmaBlock {
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const float use = m[nt][e] == -INFINITY ? 0.f : m[nt][e];  // no key above -inf so far: all weights 0
+        const float use = (m[nt][e] == -INFINITY ? 0.f : m[nt][e]) - UP;  // no key above -inf so far: all weights 0
         s[nt][e] = ex2(s[nt][e] - use), s[nt][2 + e] = ex2(s[nt][2 + e] - use);
       }
+    }
+    if constexpr (HALF) {
+      bool any = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) any = any || light(s[nt][e]);
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) l[nt][e] += s[nt][e] + s[nt][2 + e];
+        fold_light(s, kbase + KB * ROWB, vrow);
+        return;
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
       const uint32_t lo = pack(s[nt][0], s[nt][1], T()), hi = pack(s[nt][2], s[nt][3], T());
       p[nt][0] = transposed(lo), p[nt][1] = transposed(hi);
 #pragma unroll
@@ -306,6 +334,76 @@ struct MmaBlock {
       ldm4_trans(f, vrow + (((2 * t + (lane >> 3 & 1)) ^ turn) << 4));
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) mma(o[t][nt], f, p[nt][0], p[nt][1], T());
+    }
+  }
+
+  // 0 < w < 2^-14: f16 has fewer than 11 bits for it; 0 < w < 2^-43: not 2^29 times larger either
+  __device__ __forceinline__ static bool light(float w) { return __float_as_uint(w) - 1u < 0x38800000u - 1u; }
+  __device__ __forceinline__ static bool faint(float w) { return __float_as_uint(w) - 1u < 0x2A000000u - 1u; }
+
+  // O^T += V^T P^T of a block with light weights: those go in 2^29 times larger, as products of their own.  A weight is 0 in one of the two, which an
+  // infinite value would make NaN of: where a result is NaN, and where weights are faint, fold_plain gives it.
+  __device__ __forceinline__ void fold_light(const float (&w)[NT][4], uint32_t vbase, uint32_t vrow) {
+    const int lane = threadIdx.x & 31, turn = spread(lane & 7);
+    bool any = false;
+    uint32_t p[NT][2], x[NT][2];  // keys 0 to 7, 8 to 15
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        float a[2], b[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float v = w[nt][2 * i + e];
+          any = any || faint(v), a[e] = light(v) ? 0.f : v, b[e] = light(v) ? v * 0x1p29f : 0.f;
+        }
+        p[nt][i] = transposed(pack(a[0], a[1], T())), x[nt][i] = transposed(pack(b[0], b[1], T()));
+      }
+    uint32_t left = __any_sync(0xffffffffu, any) ? ~0u : 0u;  // what fold_plain has to do, a bit for sixteen dims of eight heads
+    if (!left) {
+#pragma unroll
+      for (int t = 0; t < DP / 16; t++) {
+        uint32_t f[4];
+        ldm4_trans(f, vrow + (((2 * t + (lane >> 3 & 1)) ^ turn) << 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float u[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+          mma(u, f, p[nt][0], p[nt][1], T()), mma(y, f, x[nt][0], x[nt][1], T());
+          bool nan = false;
+#pragma unroll
+          for (int e = 0; e < 4; e++) u[e] = fmaf(y[e], 0x1p-29f, o[t][nt][e] + u[e]), nan = nan || u[e] != u[e];
+          nan = __any_sync(0xffffffffu, nan);
+          left |= (uint32_t)nan << (t * NT + nt);
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[t][nt][e] = nan ? o[t][nt][e] : u[e];
+        }
+      }
+    }
+    if (left) fold_plain(w, vbase, left);
+  }
+  // The same by f32 products: a key at a time, its weights from the lanes that have them.
+  __device__ __forceinline__ void fold_plain(const float (&p)[NT][4], uint32_t vbase, uint32_t which) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+#pragma unroll 1
+    for (int j = 0; j < KB; j++) {
+      float w[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) w[nt][e] = __shfl_sync(0xffffffffu, j < 8 ? p[nt][e] : p[nt][2 + e], (j & 7) * 4 + c);
+      const uint32_t row = vbase + j * ROWB + 2 * r;
+#pragma unroll
+      for (int t = 0; t < DP / 16; t++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+          if (which >> (t * NT + nt) & 1) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              const float v = lds_f16(row + (((2 * t + half) ^ spread(j)) << 4));
+#pragma unroll
+              for (int e = 0; e < 2; e++) o[t][nt][2 * half + e] = fmaf(w[nt][e], v, o[t][nt][2 * half + e]);
+            }
+          }
     }
   }
 

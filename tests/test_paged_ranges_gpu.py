@@ -1,0 +1,88 @@
+"""The paged operators where their ranges end: weights far below the largest, fewer query heads than key heads, angles next to a zero of the cosine,
+pools that hold what no pool should, the largest sizes."""
+import math
+
+import paged_plain
+import pytest
+import torch
+
+from light_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _dense(scores, v, KH, G, D, dtype, dev, page=16, width=0):
+    """One sequence per row of `scores` (B, n): key j's first element is its score, query heads look at nothing else, so scores are exact; v (B, n)
+    or (B, n, D) are the values of all heads."""
+    B, n = scores.shape
+    held = -(-n // page)
+    k_cache, v_cache = (torch.zeros((B * held, KH, page, D), dtype=dtype, device=dev) for _ in range(2))
+    table = torch.full((B, held + width), -1, dtype=torch.int32, device=dev)
+    table[:, :held] = torch.arange(B * held, device=dev).view(B, held)
+    pad = torch.zeros((B, held * page), dtype=dtype, device=dev)
+    pad[:, :n] = scores.to(dtype)
+    k_cache[..., 0] = pad.view(B * held, 1, page)
+    rows = torch.zeros((B, held * page, D), dtype=dtype, device=dev)
+    rows[:, :n] = v.to(dtype)[..., None] if v.dim() == 2 else v.to(dtype)
+    v_cache[:] = rows.view(B * held, 1, page, D)
+    q = torch.zeros((B, KH * G, D), dtype=dtype, device=dev)
+    q[..., 0] = 1
+    return q, k_cache, v_cache, table, torch.full((B,), n, dtype=torch.int32, device=dev)
+
+
+def _close(case, rounded_p=False, **kw):
+    """Within the arithmetic's bound, for weights that lose nothing to the cache's type, or (rounded_p) no more than one rounding each."""
+    got = ops.PagedDecodeAttention(*case, 1.0, **kw)
+    want, bound = paged_plain.attention(*case, 1.0, rounded_p=rounded_p, **kw)
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), (off / bound.clamp(min=1e-300)).max().item()
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("at", ["first", "last", "within"])
+@pytest.mark.parametrize("n,B,D", [(300, 1, 128), (8192, 3, 128), (8192, 40, 64), (131072, 1, 128), (1000, 2, 256), (500, 3, 37), (20000, 1, 80)])
+def test_light_keys_under_a_heavy_one(cuda, dtype, at, n, B, D):
+    """A key with nearly all of the weight and a value of zero: the answer is the sum of what the others weigh, however little each does."""
+    for binades in (10.0, 14.5, 20.0, 21.0, 22.0, 24.5, 26.0, 30.0, 40.0, 70.0):
+        s = torch.zeros((B, n), dtype=torch.float64, device=cuda)
+        s[:, 1::2] = -1.0
+        v = torch.full((B, n), 1.0, dtype=torch.float64, device=cuda)
+        v[:, ::3] = 3.0
+        if dtype != torch.bfloat16:
+            v *= 2.0 ** 12  # (so that the answer is no subnormal half)
+        j = {"first": 0, "last": n - 1, "within": min(n // 2 + 3, n - 1)}[at]
+        s[:, j], v[:, j] = binades * math.log(2), 0.0
+        _close(_dense(s, v, 1, 3, D, dtype, cuda), rounded_p=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G", [1, 9])
+def test_weights_of_every_size_side_by_side(cuda, dtype, G):
+    """Neighbouring keys 0 to 60 binades apart, each size with a value that makes it count; windows and caps among them."""
+    g = torch.Generator(cuda).manual_seed(G)
+    s = -torch.randint(0, 61, (6, 700), generator=g, device=cuda).double() * math.log(2)
+    v = torch.randn((6, 700, 64), generator=g, device=cuda).double() * torch.exp(-s).clamp(max=2.0 ** 13)[..., None]
+    for kw in ({}, {"window": 100}, {"softcap": 50.0}):
+        _close(_dense(s, v, 2, G, 64, dtype, cuda), rounded_p=True, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G,width", [(4, 0), (12, 0), (4, 3000)])
+@pytest.mark.parametrize("far", [0.0, 5.0, 17.0, 30.0, 40.0])
+def test_infinite_values_reach_their_heads_with_their_sign(cuda, dtype, G, width, far):
+    """A value of infinity under a weight that is not 0 is the result; opposite ones, or one under a weight of 0 (its score -inf), are NaN."""
+    s = torch.zeros((5, 200), dtype=torch.float64, device=cuda)
+    s[:, 7] = far
+    v = torch.ones((5, 200, 64), dtype=torch.float64, device=cuda)
+    v[0, 3, 0] = v[1, 7, 1] = v[3, 3, 2] = v[4, 3, 2] = math.inf
+    v[1, 150, 2] = v[3, 150, 2] = -math.inf
+    s[4, 3] = -math.inf
+    got = ops.PagedDecodeAttention(*_dense(s, v, 2, G, 64, dtype, cuda, width=width), 1.0).double()
+    odd = torch.zeros_like(got)
+    odd[0, :, 0] = odd[1, :, 1] = math.inf
+    odd[1, :, 2] = -math.inf
+    odd[3, :, 2] = odd[4, :, 2] = math.nan
+    assert torch.equal(got.isnan(), odd.isnan())
+    assert torch.equal(torch.where(got.isinf(), got, 0), torch.where(odd.isinf(), odd, 0))
