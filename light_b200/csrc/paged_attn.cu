@@ -206,13 +206,32 @@ __device__ __forceinline__ float lds_f16(uint32_t addr) {
   asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(addr) : "memory");
   return __half2float(__ushort_as_half(v));
 }
+
+// Two weights, 0 or above, as a high and a low 16-bit element each that sum to them: high is less than the weight by 2^-16 of it or more, so that the
+// low one has the same sign and is 0 only with it (a value of infinity keeps its sign under both), and by 2^-7 (f16: 2^-10) at most, of which the low one
+// keeps all but 2^-8 (2^-11).  (f16: elements lie 2^-24 apart at least.)
+__device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t &lo, __nv_bfloat16) {
+  const uint32_t x = __float_as_uint(a * (1.f - 0x1p-16f)), y = __float_as_uint(b * (1.f - 0x1p-16f));
+  hi = __byte_perm(x, y, 0x7632);  // (cut off)
+  a -= __uint_as_float(x & 0xFFFF0000u), b -= __uint_as_float(y & 0xFFFF0000u);
+  lo = pack(a, b, __nv_bfloat16());
+}
+__device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t &lo, __half) {
+  const float x = fmaf(a, 1.f - 0x1p-16f, -0x1p-24f), y = fmaf(b, 1.f - 0x1p-16f, -0x1p-24f);
+  asm("cvt.rz.relu.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(y), "f"(x));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+  a -= f.x, b -= f.y;
+  lo = pack(a, b, __half());
+}
+
 // bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
 //   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
 //   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
 //   A block of 128 dims is about 340 instructions of a warp (of 400, with a maximum every block, it took 0.65 us by itself); eight warps of an SM
 //   fold 8 KB each in 1.4 us, which is the memory's rate.
-//   P is rounded to the cache's type, as the instruction wants it: 2^-8 (bf16) or 2^-11 of each weight, no more than the output's own rounding;
-//   the sum below the fraction adds the rounded weights, so that they sum to one.
+//   A weight goes in as two elements of the cache's type, as the instruction wants it, right to 2^-15 (bf16; f16: 2^-21, or 2^-25 of 1) of itself: rounded to
+//   one, its 2^-8 (2^-11) stood out wherever values cancel, and two products instead of one cost little, the tensor pipe being idle for the most part.
+//   The sum below the fraction adds the f32 weights.
 //   f16 has them 2^7 times larger (2^15 at most, with the slack; numerator and denominator share the factor, in all pieces), so that it keeps them down to
 //   2^-21 of the largest to 2^-11 of themselves.  A block with one below that has more products (fold_light): where a key holds nearly all the weight and its
 //   value little, the answer is the sum of many that are lighter than any f16.
@@ -222,6 +241,7 @@ struct MmaBlock {
   static constexpr int DP = DP_, KB = 16, HEADS = 8 * NT, ROWB = DP * 2, PR = DP + 4, EXTRA = 0;
   static constexpr bool HALF = std::is_same<T, __half>::value;
   static constexpr float UP = HALF ? 7.f : 0.f;
+  static constexpr uint32_t LIGHT = 0x38800000u - 1u;  // bits of 2^-14, less one
   uint32_t q[DP / 16][NT][2];
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
 
@@ -297,48 +317,48 @@ struct MmaBlock {
           for (int e = 0; e < 4; e++) o[t][nt][e] *= corr[e & 1];
       }
     }
-    uint32_t p[NT][2];
+    uint32_t p[NT][2][2];  // high, low; keys 0 to 7, 8 to 15
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const float use = (m[nt][e] == -INFINITY ? 0.f : m[nt][e]) - UP;  // no key above -inf so far: all weights 0
         s[nt][e] = ex2(s[nt][e] - use), s[nt][2 + e] = ex2(s[nt][2 + e] - use);
+        l[nt][e] += s[nt][e] + s[nt][2 + e];
       }
     }
     if constexpr (HALF) {
-      bool any = false;
+      uint32_t least = ~0u;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) any = any || light(s[nt][e]);
-      if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) l[nt][e] += s[nt][e] + s[nt][2 + e];
+        for (int e = 0; e < 4; e++) least = min(least, __float_as_uint(s[nt][e]) - 1u);
+      if (__any_sync(0xffffffffu, least < LIGHT)) {
         fold_light(s, kbase + KB * ROWB, vrow);
         return;
       }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const uint32_t lo = pack(s[nt][0], s[nt][1], T()), hi = pack(s[nt][2], s[nt][3], T());
-      p[nt][0] = transposed(lo), p[nt][1] = transposed(hi);
 #pragma unroll
-      for (int e = 0; e < 2; e++) l[nt][e] += s[nt][e] + s[nt][2 + e];
+      for (int i = 0; i < 2; i++) {
+        halves(s[nt][2 * i], s[nt][2 * i + 1], p[nt][0][i], p[nt][1][i], T());
+        p[nt][0][i] = transposed(p[nt][0][i]), p[nt][1][i] = transposed(p[nt][1][i]);
+      }
     }
 #pragma unroll
     for (int t = 0; t < DP / 16; t++) {
       uint32_t f[4];
       ldm4_trans(f, vrow + (((2 * t + (lane >> 3 & 1)) ^ turn) << 4));
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) mma(o[t][nt], f, p[nt][0], p[nt][1], T());
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) mma(o[t][nt], f, p[nt][i][0], p[nt][i][1], T());
     }
   }
 
   // 0 < w < 2^-14: f16 has fewer than 11 bits for it; 0 < w < 2^-43: not 2^29 times larger either
-  __device__ __forceinline__ static bool light(float w) { return __float_as_uint(w) - 1u < 0x38800000u - 1u; }
+  __device__ __forceinline__ static bool light(float w) { return __float_as_uint(w) - 1u < LIGHT; }
   __device__ __forceinline__ static bool faint(float w) { return __float_as_uint(w) - 1u < 0x2A000000u - 1u; }
 
   // O^T += V^T P^T of a block with light weights: those go in 2^29 times larger, as products of their own.  A weight is 0 in one of the two, which an
@@ -346,7 +366,7 @@ struct MmaBlock {
   __device__ __forceinline__ void fold_light(const float (&w)[NT][4], uint32_t vbase, uint32_t vrow) {
     const int lane = threadIdx.x & 31, turn = spread(lane & 7);
     bool any = false;
-    uint32_t p[NT][2], x[NT][2];  // keys 0 to 7, 8 to 15
+    uint32_t p[NT][2][2], x[NT][2][2];  // high, low; keys 0 to 7, 8 to 15
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -357,7 +377,9 @@ struct MmaBlock {
           const float v = w[nt][2 * i + e];
           any = any || faint(v), a[e] = light(v) ? 0.f : v, b[e] = light(v) ? v * 0x1p29f : 0.f;
         }
-        p[nt][i] = transposed(pack(a[0], a[1], T())), x[nt][i] = transposed(pack(b[0], b[1], T()));
+        halves(a[0], a[1], p[nt][0][i], p[nt][1][i], T()), halves(b[0], b[1], x[nt][0][i], x[nt][1][i], T());
+#pragma unroll
+        for (int k = 0; k < 2; k++) p[nt][k][i] = transposed(p[nt][k][i]), x[nt][k][i] = transposed(x[nt][k][i]);
       }
     uint32_t left = __any_sync(0xffffffffu, any) ? ~0u : 0u;  // what fold_plain has to do, a bit for sixteen dims of eight heads
     if (!left) {
@@ -368,7 +390,8 @@ struct MmaBlock {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           float u[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-          mma(u, f, p[nt][0], p[nt][1], T()), mma(y, f, x[nt][0], x[nt][1], T());
+#pragma unroll
+          for (int k = 0; k < 2; k++) mma(u, f, p[nt][k][0], p[nt][k][1], T()), mma(y, f, x[nt][k][0], x[nt][k][1], T());
           bool nan = false;
 #pragma unroll
           for (int e = 0; e < 4; e++) u[e] = fmaf(y[e], 0x1p-29f, o[t][nt][e] + u[e]), nan = nan || u[e] != u[e];

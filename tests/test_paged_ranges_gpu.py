@@ -86,3 +86,31 @@ def test_infinite_values_reach_their_heads_with_their_sign(cuda, dtype, G, width
     odd[3, :, 2] = odd[4, :, 2] = math.nan
     assert torch.equal(got.isnan(), odd.isnan())
     assert torch.equal(torch.where(got.isinf(), got, 0), torch.where(odd.isinf(), odd, 0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G", [1, 12])
+@pytest.mark.parametrize("B,n", [(1, 2), (9, 64), (40, 1500)])
+def test_weights_are_as_exact_as_the_scores(cuda, dtype, G, B, n):
+    """Pairs of keys whose weighted values cancel: what a weight's rounding to the cache's type would leave over is far above the bound."""
+    g = torch.Generator(cuda).manual_seed(n)
+    s = (torch.rand((B, n), generator=g, device=cuda) * 3).to(dtype).double()
+    v = torch.ones((B, n), dtype=torch.float64, device=cuda)
+    v[:, 1::2] = -torch.exp(s[:, 0::2] - s[:, 1::2])
+    _close(_dense(s, v, 2, G, 64, dtype, cuda))
+    _close(_dense(s, v, 2, G, 64, dtype, cuda), softcap=20.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("down", [0.0, 9.0, 25.0])
+def test_weights_under_a_heavy_one_are_as_exact(cuda, dtype, down):
+    """The same under a key of value 0 that is `down` nats above the others; far below it halves have
+    products of their own."""
+    g = torch.Generator(cuda).manual_seed(5)
+    s = (-down - torch.rand((5, 400), generator=g, device=cuda) * 3).to(dtype).double()
+    v = torch.ones((5, 400), dtype=torch.float64, device=cuda)
+    v[:, 1::2] = -torch.exp(s[:, 0::2] - s[:, 1::2])
+    s[:, 0], v[:, :2] = 0.0, 0.0
+    v *= 2.0 ** 11
+    _close(_dense(s, v, 2, 4, 64, dtype, cuda))
+    _close(_dense(s, v, 2, 12, 64, dtype, cuda, width=3000))
