@@ -155,7 +155,6 @@ constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS
 // 16-bit: weights are 2^(score - m) for an m that follows the running maximum only when a score is above it by more than this: one vote a block
 // instead of the maximum's shuffles and the corrections (64 ragged sequences 45.1 -> 44.5 us, 33 with a window 19.6 -> 18.8; f32, whose heads'
 // maxima take three shuffles: 11.2 -> 11.6 for 4 x 1024).  Weights reach 2^8, and the largest is 1 or more, as with the maximum itself.
-constexpr float SLACK = 8.f;
 
 struct SplitArgs {
   PagedArgs p;
@@ -232,16 +231,15 @@ __device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t 
 //   A weight goes in as two elements of the cache's type, as the instruction wants it, right to 2^-15 (bf16; f16: 2^-21, or 2^-25 of 1) of itself: rounded to
 //   one, its 2^-8 (2^-11) stood out wherever values cancel, and two products instead of one cost little, the tensor pipe being idle for the most part.
 //   The sum below the fraction adds the f32 weights.
-//   f16 has them 2^7 times larger (2^15 at most, with the slack; numerator and denominator share the factor, in all pieces), so that it keeps them down to
-//   2^-21 of the largest to 2^-11 of themselves.  A block with one below that has more products (fold_light): where a key holds nearly all the weight and its
+//   f16 has them 2^11 times larger (2^15 at most, with a slack of 2^4; numerator and denominator share the factor, in all pieces), so that it keeps them down to
+//   2^-25 of the largest to 2^-11 of themselves.  A block with one below that has more products (fold_light): where a key holds nearly all the weight and its
 //   value little, the answer is the sum of many that are lighter than any f16.
 template <typename T_, int DP_, int NT>
 struct MmaBlock {
   using T = T_;
   static constexpr int DP = DP_, KB = 16, HEADS = 8 * NT, ROWB = DP * 2, PR = DP + 4, EXTRA = 0;
   static constexpr bool HALF = std::is_same<T, __half>::value;
-  static constexpr float UP = HALF ? 7.f : 0.f;
-  static constexpr uint32_t LIGHT = 0x38800000u - 1u;  // bits of 2^-14, less one
+  static constexpr float SLACK = HALF ? 4.f : 8.f, UP = HALF ? 15.f - SLACK : 0.f;
   uint32_t q[DP / 16][NT][2];
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
 
@@ -328,14 +326,21 @@ struct MmaBlock {
       }
     }
     if constexpr (HALF) {
-      uint32_t least = ~0u;
+      float least = 1.f;
+      bool any = false;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) least = min(least, __float_as_uint(s[nt][e]) - 1u);
-      if (__any_sync(0xffffffffu, least < LIGHT)) {
-        fold_light(s, kbase + KB * ROWB, vrow);
-        return;
+        for (int e = 0; e < 4; e++) least = fminf(least, s[nt][e]);
+      if (__any_sync(0xffffffffu, least < 0x1p-14f)) {  // (0 where there is no key)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) any = any || light(s[nt][e]);
+        if (__any_sync(0xffffffffu, any)) {
+          fold_light(s, kbase + KB * ROWB, vrow);
+          return;
+        }
       }
     }
 #pragma unroll
@@ -358,7 +363,7 @@ struct MmaBlock {
   }
 
   // 0 < w < 2^-14: f16 has fewer than 11 bits for it; 0 < w < 2^-43: not 2^29 times larger either
-  __device__ __forceinline__ static bool light(float w) { return __float_as_uint(w) - 1u < LIGHT; }
+  __device__ __forceinline__ static bool light(float w) { return __float_as_uint(w) - 1u < 0x38800000u - 1u; }
   __device__ __forceinline__ static bool faint(float w) { return __float_as_uint(w) - 1u < 0x2A000000u - 1u; }
 
   // O^T += V^T P^T of a block with light weights: those go in 2^29 times larger, as products of their own.  A weight is 0 in one of the two, which an
