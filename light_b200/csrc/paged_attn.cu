@@ -152,10 +152,6 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 //   * All four warps of a CTA on the blocks of one unit in turn, with barriers, took 75 us for the 64: two microseconds a unit.
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 4, CLUSTER_WIDE = 8;
 
-// 16-bit: weights are 2^(score - m) for an m that follows the running maximum only when a score is above it by more than this: one vote a block
-// instead of the maximum's shuffles and the corrections (64 ragged sequences 45.1 -> 44.5 us, 33 with a window 19.6 -> 18.8; f32, whose heads'
-// maxima take three shuffles: 11.2 -> 11.6 for 4 x 1024).  Weights reach 2^8, and the largest is 1 or more, as with the maximum itself.
-
 struct SplitArgs {
   PagedArgs p;
   int hpg, groups;    // query heads per unit, units per KV head
@@ -239,6 +235,9 @@ struct MmaBlock {
   using T = T_;
   static constexpr int DP = DP_, KB = 16, HEADS = 8 * NT, ROWB = DP * 2, PR = DP + 4, EXTRA = 0;
   static constexpr bool HALF = std::is_same<T, __half>::value;
+  // Weights are 2^(score - m) for an m that follows the running maximum only when a score is above it by more than SLACK: one vote a block instead of the
+  // maximum's shuffles and the corrections (64 ragged sequences 45.1 -> 44.5 us, 33 with a window 19.6 -> 18.8; f32, whose heads' maxima take three
+  // shuffles: 11.2 -> 11.6 for 4 x 1024).  Weights reach 2^SLACK, and the largest is 1 or more, as with the maximum itself.
   static constexpr float SLACK = HALF ? 4.f : 8.f, UP = HALF ? 15.f - SLACK : 0.f;
   uint32_t q[DP / 16][NT][2];
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
