@@ -495,6 +495,14 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
   int far_kind = kind0, slot_far = 0, slot_now = 0;
   long long far_t = t;
   Walk far = source(kind0, t);
+  // Past kinds of which this warp has no round (more): a slot of the ring is a round's.  With two warps per token and few query heads, its first kind may
+  // be one of those.
+  auto settle = [&]() {
+    while (far.left + hl <= 0 && far_t < a.T) {  // (the same for the whole warp)
+      if (++far_kind == kinds) far_kind = kind0, far_t += stride;
+      if (far_t < a.T) far = source(far_kind, far_t);
+    }
+  };
   auto fetch = [&]() {  // the next round, if there is one
     if (far_t < a.T) {
       if (far.left > 0) {
@@ -503,15 +511,13 @@ __global__ void __launch_bounds__(RC_WARPS * 32) qk_norm_rope_chunks_kernel(Rota
         if (c1 >= 0) cp_chunk<CB>(dst + 32 * CB, far.at + c1 * E);
       }
       far.at += far.step, far.left -= hop;
-      while (far.left + hl <= 0 && far_t < a.T) {  // (the same for the whole warp)
-        if (++far_kind == kinds) far_kind = kind0, far_t += stride;
-        if (far_t < a.T) far = source(far_kind, far_t);
-      }
+      settle();
     }
     cp_async_commit();
     slot_far = slot_far + 1 == RC_AHEAD ? 0 : slot_far + 1;
   };
   long long pos = a.positions[t], slot = a.slots ? a.slots[t] : 0;
+  settle();
 #pragma unroll
   for (int i = 0; i < RC_AHEAD; i++) fetch();  // on their way while the angles are worked out
   Walk to;

@@ -114,3 +114,25 @@ def test_weights_under_a_heavy_one_are_as_exact(cuda, dtype, down):
     v *= 2.0 ** 11
     _close(_dense(s, v, 2, 4, 64, dtype, cuda))
     _close(_dense(s, v, 2, 12, 64, dtype, cuda, width=3000))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [3, 500, 600, 1000, 1700, 2000])
+@pytest.mark.parametrize("NH,KH,D", [(4, 8, 128), (1, 8, 128), (4, 5, 128), (2, 16, 128), (8, 16, 64), (1, 40, 64), (3, 20, 80), (1, 3, 256)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_of_fewer_query_heads_than_key_heads(cuda, dtype, T, NH, KH, D, interleaved):
+    g = torch.Generator(cuda).manual_seed(T + NH)
+    q, k, v = (torch.randn((T, n, D), generator=g, device=cuda).to(dtype) for n in (NH, KH, KH))
+    w = (1 + 0.2 * torch.randn(D, generator=g, device=cuda)).to(dtype)
+    freq, _ = ops.RoPEFrequencies(D, 10000.0)
+    positions = torch.arange(T, device=cuda)
+    pages = T // 16 + 1
+    kc, vc = (torch.zeros((pages, KH, 16, D), dtype=dtype, device=cuda) for _ in range(2))
+    slots = torch.randperm(pages * 16, generator=g, device=cuda)[:T].contiguous()
+    got, _ = ops.QKNormRoPE(q, k, positions, freq, q_weight=w, k_weight=w, interleaved=interleaved, v=v, k_cache=kc, v_cache=vc, slots=slots)
+    again, dense = ops.QKNormRoPE(q, k, positions, freq, q_weight=w, k_weight=w, interleaved=interleaved)
+    want, bound = paged_plain.rotated(q, w, 1e-6, positions, freq, interleaved, 1.0)
+    assert bool(((got.double() - want).abs() <= bound).all()) and torch.equal(again, got)
+    want, bound = paged_plain.rotated(k, w, 1e-6, positions, freq, interleaved, 1.0)
+    assert bool(((dense.double() - want).abs() <= bound).all())
+    assert torch.equal(kc[slots // 16, :, slots % 16], dense) and torch.equal(vc[slots // 16, :, slots % 16], v)
