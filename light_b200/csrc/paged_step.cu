@@ -255,7 +255,7 @@ int launch_pages(void (*kern)(PagesArgs, bool), const PagesArgs &a, size_t smem,
 // y = x rsqrt(mean x^2 + eps) w over the D elements of a head (no weight: y = x), then the first R of them in pairs (a, b):
 //   (a cos t - b sin t, a sin t + b cos t) factor,   t = position * inv_freq[i],   pair i = (i, i + R / 2) or (2 i, 2 i + 1).
 // f32 from the operand to the one rounding at the end; t in f64 (200000 positions far, an f32 angle is off by 0.01), reduced there to
-// half a turn for the f32 functions.  The angles are the same for every head of a token, so each is computed once.
+// half a turn for the f32 functions, which get what that leaves over as a turn of their own.  The angles are the same for every head of a token, so each is computed once.
 struct RotateArgs {
   const void *q, *k, *v, *qw, *kw;
   void *q_out, *k_out, *v_out;            // k_out: dense, or the cache's keys with slots
@@ -271,9 +271,11 @@ struct RotateArgs {
 
 __device__ __forceinline__ float2 cos_sin(long long pos, double freq) {
   const double t = (double)pos * freq * 0.15915494309189533577;  // in turns: 10^6 radians keep 2^-35 of one
+  const double u = 2. * (t - rint(t));                           // in half turns, exact
+  const float x = (float)u, d = 3.14159265358979f * (float)(u - (double)x);
   float s, c;
-  sincospif(2.f * (float)(t - rint(t)), &s, &c);
-  return make_float2(c, s);
+  sincospif(x, &s, &c);
+  return make_float2(fmaf(-s, d, c), fmaf(c, d, s));  // what the f32 angle leaves over, d <= pi 2^-25: it is all of a sine or cosine next to a zero
 }
 
 constexpr int RT_THREADS = 256, RT_MAX_D = 256;

@@ -136,3 +136,26 @@ def test_rotation_of_fewer_query_heads_than_key_heads(cuda, dtype, T, NH, KH, D,
     want, bound = paged_plain.rotated(k, w, 1e-6, positions, freq, interleaved, 1.0)
     assert bool(((dense.double() - want).abs() <= bound).all())
     assert torch.equal(kc[slots // 16, :, slots % 16], dense) and torch.equal(vc[slots // 16, :, slots % 16], v)
+
+
+@pytest.mark.parametrize("D", [64, 7])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_keeps_sines_and_cosines_next_to_their_zeros(cuda, D, interleaved):
+    """Angles within 1e-6 of whole quarter turns, near and far from the start: the sine or cosine that is nearly zero has its own precision."""
+    R = D // 2 * 2
+    positions = torch.tensor([1, 3, 1001, 100003], device=cuda)
+    quarter = torch.arange(R // 2, dtype=torch.float64, device=cuda)
+    freq = (quarter % 7) * (math.pi / 2) + (0.1 + quarter) * 1e-11
+    q = torch.zeros((4, 3, D), device=cuda)
+    first = slice(0, R, 2) if interleaved else slice(0, R // 2)
+    q[:, :, first] = torch.tensor([1.0, -0.5, 3.0], device=cuda)[None, :, None]
+    got, _ = ops.QKNormRoPE(q, q, positions, freq, interleaved=interleaved)
+    t = positions.double()[:, None, None] * freq
+    a = q[:, :, first].double()
+    second = slice(1, R, 2) if interleaved else slice(R // 2, R)
+    # The angle in 64 bits has four roundings of 2^-53 (here one, there three); sine and cosine of an f32 angle at most pi 2^-25 away are right to two
+    # steps of 2^-23, as are the products and the sum that bring them there.
+    for part, want in ((first, a * torch.cos(t)), (second, a * torch.sin(t))):
+        bound = 4 * 2.0 ** -53 * t.abs() * a.abs() + 8 * 2.0 ** -23 * (want.abs() + 2.0 ** -23 * a.abs())
+        off = (got[:, :, part].double() - want).abs()
+        assert bool((off <= bound).all()), (off / bound.clamp(min=1e-300)).max().item()
