@@ -554,14 +554,18 @@ int light_b200_paged_decode_attn(const lb200_paged_attn_args *a, int device, voi
   return on.rc ? on.rc : paged_decode_attn(a, (cudaStream_t)stream);
 }
 
+// (its value is bits: an error has to be negative, whatever made it)
 int light_b200_paged_status(int device) {
+  auto failed = [](int rc) {
+    if (rc > 0) fail(-rc, "light_b200: paged_status: %s", cudaGetErrorString((cudaError_t)rc));
+    return rc > 0 ? -rc : rc;
+  };
   OnDevice on(device);
-  if (on.rc) return on.rc;
+  if (on.rc) return failed(on.rc);
   unsigned int x = 0, y = 0;
-  cudaError_t e = cudaDeviceSynchronize();
-  if (e != cudaSuccess) return fail((int)e, "light_b200: paged_status: %s", cudaGetErrorString(e));
-  if (int rc = paged_attn_status(&x)) return fail(rc, "light_b200: paged_status: %s", cudaGetErrorString((cudaError_t)rc));
-  if (int rc = paged_step_status(&y)) return fail(rc, "light_b200: paged_status: %s", cudaGetErrorString((cudaError_t)rc));
+  if (int rc = (int)cudaDeviceSynchronize()) return failed(rc);
+  if (int rc = paged_attn_status(&x)) return failed(rc);
+  if (int rc = paged_step_status(&y)) return failed(rc);
   return (int)(x | y);
 }
 

@@ -1147,4 +1147,7 @@ def paged_status(device_index: int = 0) -> int:
     """What the paged operators met on this device so far (light_b200_paged_status; synchronises): 1 a length outside the table, 2 a page outside
     the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of free pages, a length beyond
     the table at its release."""
-    return _lib.lib().light_b200_paged_status(device_index)
+    bits = _lib.lib().light_b200_paged_status(device_index)
+    if bits < 0:
+        _lib.check(bits)
+    return bits
