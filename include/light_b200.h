@@ -386,6 +386,8 @@ LB200_API int light_b200_decode_attn(const lb200_decode_attn_args *args, int dev
  * paged_release met a negative length or a count outside [0, capacity], or paged_release a length beyond the table (it pushed W pages).
  * Negative: the call itself failed (light_b200_last_error). */
 LB200_API int light_b200_paged_status(int device);
+/* The same, and the device's bits are 0 from then on: a server that ran out of pages once can see the next fault. */
+LB200_API int light_b200_paged_status_clear(int device);
 
 #define LB200_PAGED_MAX_REQUESTS 8192
 typedef struct lb200_paged_pages {

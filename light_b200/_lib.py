@@ -158,6 +158,7 @@ SYMBOLS = {
     "light_b200_paged_attn_scratch_bytes": (C.c_ulonglong, [C.POINTER(PagedAttnArgs), C.c_int]),
     "light_b200_paged_decode_attn": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_int, C.c_void_p]),
     "light_b200_paged_status": (C.c_int, [C.c_int]),
+    "light_b200_paged_status_clear": (C.c_int, [C.c_int]),
     "light_b200_inc_i64": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "light_b200_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_float,
                                      C.c_int, C.c_void_p]),

@@ -554,8 +554,8 @@ int light_b200_paged_decode_attn(const lb200_paged_attn_args *a, int device, voi
   return on.rc ? on.rc : paged_decode_attn(a, (cudaStream_t)stream);
 }
 
-// (its value is bits: an error has to be negative, whatever made it)
-int light_b200_paged_status(int device) {
+// (the value is bits: an error has to be negative, whatever made it)
+static int paged_status(int device, bool clear) {
   auto failed = [](int rc) {
     if (rc > 0) fail(-rc, "light_b200: paged_status: %s", cudaGetErrorString((cudaError_t)rc));
     return rc > 0 ? -rc : rc;
@@ -564,10 +564,12 @@ int light_b200_paged_status(int device) {
   if (on.rc) return failed(on.rc);
   unsigned int x = 0, y = 0;
   if (int rc = (int)cudaDeviceSynchronize()) return failed(rc);
-  if (int rc = paged_attn_status(&x)) return failed(rc);
-  if (int rc = paged_step_status(&y)) return failed(rc);
+  if (int rc = paged_attn_status(&x, clear)) return failed(rc);
+  if (int rc = paged_step_status(&y, clear)) return failed(rc);
   return (int)(x | y);
 }
+int light_b200_paged_status(int device) { return paged_status(device, false); }
+int light_b200_paged_status_clear(int device) { return paged_status(device, true); }
 
 int light_b200_embedding_q(int t, const void *table, const int64_t *ids, float *out, int64_t n_ids, int64_t V, int K, int device,
                            void *stream) {

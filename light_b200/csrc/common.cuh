@@ -143,8 +143,8 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *a, cudaStream_t st);
 int paged_attn_check(const lb200_paged_attn_args *a);
 unsigned long long paged_attn_scratch_bytes(const lb200_paged_attn_args *a);
 int paged_decode_attn(const lb200_paged_attn_args *a, cudaStream_t st);
-int paged_attn_status(unsigned int *bits);  // 0 or a CUDA error
-int paged_step_status(unsigned int *bits);
+int paged_attn_status(unsigned int *bits, bool clear);  // 0 or a CUDA error
+int paged_step_status(unsigned int *bits, bool clear);
 int argmax_rows(const float *x, int64_t *out, long long rows, int cols, cudaStream_t st);
 int moe_route_sigmoid(const float *logits, const float *bias, int64_t *ids, float *weights, int T, int E, int topk, int norm_topk,
                       cudaStream_t st);

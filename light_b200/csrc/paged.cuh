@@ -50,5 +50,20 @@ struct FastDiv {
   __device__ __forceinline__ int div(int n) const { return (int)(__umulhi((unsigned)n << 1, m) >> s); }
 };
 
+// The word as it was, and 0 in its place, in one: what a launch adds meanwhile is in this answer or the next.
+__device__ unsigned int g_taken;
+__global__ void take_status_kernel(unsigned int *word) { g_taken = atomicExch(word, 0u); }
+inline int taken_status(const unsigned int &symbol, unsigned int *bits) {
+  static std::mutex one;  // (g_taken is one word)
+  std::lock_guard<std::mutex> lk(one);
+  void *word = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&word, symbol);
+  if (e == cudaSuccess) {
+    take_status_kernel<<<1, 1>>>(static_cast<unsigned int *>(word));
+    e = cudaGetLastError();
+  }
+  return (int)(e != cudaSuccess ? e : cudaMemcpyFromSymbol(bits, g_taken, sizeof(*bits)));
+}
+
 }  // namespace
 }  // namespace lb

@@ -1427,6 +1427,8 @@ int paged_decode_attn(const lb200_paged_attn_args *p, cudaStream_t st) {
   return launched("paged_decode_attn");
 }
 
-int paged_attn_status(unsigned int *bits) { return (int)cudaMemcpyFromSymbol(bits, g_attn_status, sizeof(*bits)); }
+int paged_attn_status(unsigned int *bits, bool clear) {
+  return clear ? taken_status(g_attn_status, bits) : (int)cudaMemcpyFromSymbol(bits, g_attn_status, sizeof(*bits));
+}
 
 }  // namespace lb

@@ -773,8 +773,8 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
   return launched("qk_norm_rope");
 }
 
-int paged_step_status(unsigned int *bits) {
-  return (int)cudaMemcpyFromSymbol(bits, g_step_status, sizeof(*bits));
+int paged_step_status(unsigned int *bits, bool clear) {
+  return clear ? taken_status(g_step_status, bits) : (int)cudaMemcpyFromSymbol(bits, g_step_status, sizeof(*bits));
 }
 
 }  // namespace lb

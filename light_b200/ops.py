@@ -1143,11 +1143,12 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     return out
 
 
-def paged_status(device_index: int = 0) -> int:
-    """What the paged operators met on this device so far (light_b200_paged_status; synchronises): 1 a length outside the table, 2 a page outside
-    the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of free pages, a length beyond
-    the table at its release."""
-    bits = _lib.lib().light_b200_paged_status(device_index)
+def paged_status(device_index: int = 0, clear: bool = False) -> int:
+    """What the paged operators met on this device so far, or since it was last asked with `clear` (light_b200_paged_status, ..._clear; synchronises): 1 a
+    length outside the table, 2 a page outside the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of
+    free pages, a length beyond the table at its release."""
+    lib = _lib.lib()
+    bits = (lib.light_b200_paged_status_clear if clear else lib.light_b200_paged_status)(device_index)
     if bits < 0:
         _lib.check(bits)
     return bits

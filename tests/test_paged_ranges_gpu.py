@@ -159,3 +159,26 @@ def test_rotation_keeps_sines_and_cosines_next_to_their_zeros(cuda, D, interleav
         bound = 4 * 2.0 ** -53 * t.abs() * a.abs() + 8 * 2.0 ** -23 * (want.abs() + 2.0 ** -23 * a.abs())
         off = (got[:, :, part].double() - want).abs()
         assert bool((off <= bound).all()), (off / bound.clamp(min=1e-300)).max().item()
+
+
+def _i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def test_status_is_read_and_cleared(cuda):
+    """Each bit is met, read, read again and cleared; the next fault behind it shows."""
+    q, cache = torch.zeros((1, 2, 64), device=cuda), torch.zeros((2, 2, 8, 64), device=cuda)
+    table, one, none = _i32([[0, 1]], cuda), _i32([1], cuda), _i32([0], cuda)
+    pos, freq = torch.zeros(1, dtype=torch.int64, device=cuda), ops.RoPEFrequencies(64, 1e4)[0]
+    met = {1: lambda: ops.PagedDecodeAttention(q, cache, cache, table, _i32([17], cuda), 1.0),
+           2: lambda: ops.PagedDecodeAttention(q, cache, cache, _i32([[2, 0]], cuda), one, 1.0),
+           4: lambda: ops.QKNormRoPE(q, q, pos, freq, v=q, k_cache=cache.clone(), v_cache=cache.clone(), slots=pos + 16),
+           8: lambda: ops.PagedAdvance(table, none, one, one, none, 8, 1)}
+    ops.paged_status(0, clear=True)
+    for _ in range(2):
+        for bit, call in met.items():
+            call()
+            assert ops.paged_status(0) == bit and ops.paged_status(0, clear=True) == bit and ops.paged_status(0) == 0
+    for call in met.values():
+        call()
+    assert ops.paged_status(0, clear=True) == 15 and ops.paged_status(0, clear=True) == 0
