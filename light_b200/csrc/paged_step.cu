@@ -153,17 +153,19 @@ __global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, 
       if (i < a.tokens) a.positions[i] = pos[j], a.slots[i] = pg[j] >= 0 ? (long long)pg[j] * P + in[j] : -1;
     }
   }
-  for (int p0 = gid; p0 < taken; p0 += PG_AHEAD * threads) {  // (after the tokens: their first pages are not among these)
+  for (long long p0 = gid; p0 < taken; p0 += PG_AHEAD * (long long)threads) {  // (after the tokens: their first pages are not among these)
     int pg[PG_AHEAD];
 #pragma unroll
-    for (int j = 0; j < PG_AHEAD; j++)
-      if (p0 + j * threads < taken) pg[j] = a.free_pages[avail - 1 - (p0 + j * threads)];
+    for (int j = 0; j < PG_AHEAD; j++) {
+      const long long p = p0 + j * (long long)threads;
+      if (p < taken) pg[j] = a.free_pages[avail - 1 - p];
+    }
 #pragma unroll
     for (int j = 0; j < PG_AHEAD; j++) {
-      const int p = p0 + j * threads;
+      const long long p = p0 + j * (long long)threads;
       if (p < taken) {
-        const int b = owner_of(first, a.B, p), l = len[b];
-        a.table[(long long)b * a.table_stride + held_of(l < 0 ? -1 - l : l) + (p - first[b])] = pg[j];
+        const int b = owner_of(first, a.B, (int)p), l = len[b];
+        a.table[(long long)b * a.table_stride + held_of(l < 0 ? -1 - l : l) + ((int)p - first[b])] = pg[j];
       }
     }
   }

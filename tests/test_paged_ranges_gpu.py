@@ -182,3 +182,24 @@ def test_status_is_read_and_cleared(cuda):
     for call in met.values():
         call()
     assert ops.paged_status(0, clear=True) == 15 and ops.paged_status(0, clear=True) == 0
+
+
+def test_advance_of_nearly_two_to_the_31_pages(cuda):
+    """8192 prompts of 262143 tokens, a page each: what counts pages must not wrap around."""
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("not enough memory")
+    B, n = 8192, (1 << 18) - 1
+    total = B * n
+    table = torch.full((B, n + 1), -1, dtype=torch.int32, device=cuda)
+    free = torch.arange(total + 5, dtype=torch.int32, device=cuda)
+    new = torch.full((B,), n, dtype=torch.int32, device=cuda)
+    s = ops.PagedAdvance(table, torch.zeros_like(new), new, free, _i32([total + 5], cuda), 1, total)
+    assert s.free_count.tolist() == [5] and bool((s.granted == n).all()) and bool((s.lens == n).all()) and bool((table[:, n] == -1).all())
+    at = torch.arange(n, device=cuda)
+    for b in range(0, B, 256):
+        rows = (torch.arange(b, b + 256, device=cuda) * n)[:, None] + at
+        assert bool((s.positions[b * n:(b + 256) * n].view(256, n) == at).all())
+        assert bool((s.slots[b * n:(b + 256) * n].view(256, n) == total + 4 - rows).all())
+        assert bool((table[b:b + 256, :n] == total + 4 - rows).all())
+    del s, table, free
+    torch.cuda.empty_cache()
