@@ -383,7 +383,8 @@ LB200_API int light_b200_decode_attn(const lb200_decode_attn_args *args, int dev
 /* 0, or of the calls so far on this device (synchronises): bit 0: a length outside [0, W page_size] reached the attention (it used the
  * nearest inside); bit 1: a page outside [0, pages) did (its keys counted as absent); bit 2: a slot at or beyond pages * page_size
  * reached qk_norm_rope (nothing was written for it); bit 3: paged_advance left a request without its tokens, or it or
- * paged_release met a negative length or a count outside [0, capacity], or paged_release a length beyond the table (it pushed W pages).
+ * paged_release met a negative length, a count outside [0, capacity] or a page below 0 (the tokens on it have slot -1, although they count as
+ * granted; it stays in the table or on the stack), or paged_release a length beyond the table (it pushed W pages).
  * Negative: the call itself failed (light_b200_last_error). */
 LB200_API int light_b200_paged_status(int device);
 /* The same, and the device's bits are 0 from then on: a server that ran out of pages once can see the next fault. */

@@ -130,13 +130,14 @@ __global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, 
   }
   if (gid == 0) a.starts[a.B] = starts[a.B], a.count_out[0] = avail - taken;
   const int given_rows = starts[a.B];
+  bool hole = false;  // a page below 0 under a token that got its place, or on its way into the table
   for (long long i0 = gid; i0 < a.tokens; i0 += PG_AHEAD * (long long)threads) {
     int pg[PG_AHEAD], in[PG_AHEAD];
     long long pos[PG_AHEAD];
 #pragma unroll
     for (int j = 0; j < PG_AHEAD; j++) {
       const long long i = i0 + j * (long long)threads;
-      pg[j] = -1, pos[j] = 0, in[j] = 0;
+      pg[j] = -1, pos[j] = 0, in[j] = -1;
       if (i < given_rows && i < a.tokens) {
         const int b = owner_of(starts, a.B, (int)i), l = len[b], n = l < 0 ? -1 - l : l;
         pos[j] = (long long)n + ((int)i - starts[b]);
@@ -151,6 +152,7 @@ __global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, 
     for (int j = 0; j < PG_AHEAD; j++) {
       const long long i = i0 + j * (long long)threads;
       if (i < a.tokens) a.positions[i] = pos[j], a.slots[i] = pg[j] >= 0 ? (long long)pg[j] * P + in[j] : -1;
+      hole |= pg[j] < 0 && in[j] >= 0;
     }
   }
   for (long long p0 = gid; p0 < taken; p0 += PG_AHEAD * (long long)threads) {  // (after the tokens: their first pages are not among these)
@@ -166,9 +168,11 @@ __global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, 
       if (p < taken) {
         const int b = owner_of(first, a.B, (int)p), l = len[b];
         a.table[(long long)b * a.table_stride + held_of(l < 0 ? -1 - l : l) + ((int)p - first[b])] = pg[j];
+        hole |= pg[j] < 0;
       }
     }
   }
+  if (hole) atomicOr(&g_step_status, (unsigned)PAGED_REFUSED);
 }
 
 // The pages of the requests marked done, in order, on top of the stack.
@@ -206,6 +210,7 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, 
   const int gid = rank * blockDim.x + tid, threads = gridDim.x * blockDim.x;
   for (int b = gid; b < a.B; b += threads) a.lens_out[b] = keep[b];
   if (gid == 0) a.count_out[0] = avail + total;
+  bool hole = false;  // a page below 0
   for (long long p0 = gid; p0 < total; p0 += PG_AHEAD * (long long)threads) {
     int pg[PG_AHEAD];
 #pragma unroll
@@ -219,9 +224,10 @@ __global__ void __launch_bounds__(PG_THREADS) paged_release_kernel(PagesArgs a, 
 #pragma unroll
     for (int j = 0; j < PG_AHEAD; j++) {
       const long long p = p0 + j * (long long)threads;
-      if (p < total) a.free_pages[avail + p] = pg[j];
+      if (p < total) a.free_pages[avail + p] = pg[j], hole |= pg[j] < 0;
     }
   }
+  if (hole) atomicOr(&g_step_status, (unsigned)PAGED_REFUSED);
 }
 
 // `work`: entries at most, beside the requests

@@ -1145,8 +1145,8 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 
 def paged_status(device_index: int = 0, clear: bool = False) -> int:
     """What the paged operators met on this device so far, or since it was last asked with `clear` (light_b200_paged_status, ..._clear; synchronises): 1 a
-    length outside the table, 2 a page outside the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or a bad count of
-    free pages, a length beyond the table at its release."""
+    length outside the table, 2 a page outside the cache, 4 a slot outside it, 8 a request without its tokens, a negative length or page or a bad
+    count of free pages, a length beyond the table at its release."""
     lib = _lib.lib()
     bits = (lib.light_b200_paged_status_clear if clear else lib.light_b200_paged_status)(device_index)
     if bits < 0:

@@ -203,3 +203,24 @@ def test_advance_of_nearly_two_to_the_31_pages(cuda):
         assert bool((table[b:b + 256, :n] == total + 4 - rows).all())
     del s, table, free
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("B", [3, 3000])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_pages_below_zero_are_reported(cuda, B, inplace):
+    """A hole in a held page's place, on the stack, and on its way back to it: nothing of it goes by in silence."""
+    def step(held, free, done):
+        table = torch.full((B, 3), 7, dtype=torch.int32, device=cuda)
+        table[B - 1, 0] = held
+        lens, one = torch.zeros(B, dtype=torch.int32, device=cuda), torch.zeros(B, dtype=torch.int32, device=cuda)
+        lens[B - 1], one[B - 1], one[0] = 3, 1, 1
+        stack, count = _i32([1, free, 3], cuda), _i32([2], cuda)
+        s = ops.PagedAdvance(table, lens, one, stack, count, 4, 2, inplace=inplace)
+        given = (s.granted.tolist()[0], s.granted.tolist()[-1], s.slots.tolist(), ops.paged_status(0, clear=True))
+        ops.PagedRelease(table, s.lens, torch.arange(B, device=cuda) == (B - 1 if done else B), stack, s.free_count, 4, inplace=inplace)
+        return given, ops.paged_status(0, clear=True)
+    ops.paged_status(0, clear=True)
+    assert step(5, 2, True) == ((1, 1, [8, 23], 0), 0)
+    assert step(-1, 2, False) == ((1, 1, [8, -1], 8), 0)
+    assert step(-1, 2, True) == ((1, 1, [8, -1], 8), 8)
+    assert step(5, -4, False) == ((1, 1, [-1, 23], 8), 0)
