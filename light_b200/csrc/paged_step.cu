@@ -155,17 +155,17 @@ __global__ void __launch_bounds__(PG_THREADS) paged_advance_kernel(PagesArgs a, 
       hole |= pg[j] < 0 && in[j] >= 0;
     }
   }
-  for (long long p0 = gid; p0 < taken; p0 += PG_AHEAD * (long long)threads) {  // (after the tokens: their first pages are not among these)
+  for (unsigned p0 = gid; p0 < (unsigned)taken; p0 += PG_AHEAD * threads) {  // (after the tokens: their first pages are not among these; 2^31 and a step fit)
     int pg[PG_AHEAD];
 #pragma unroll
     for (int j = 0; j < PG_AHEAD; j++) {
-      const long long p = p0 + j * (long long)threads;
-      if (p < taken) pg[j] = a.free_pages[avail - 1 - p];
+      const unsigned p = p0 + j * threads;
+      if (p < (unsigned)taken) pg[j] = a.free_pages[avail - 1 - (int)p];
     }
 #pragma unroll
     for (int j = 0; j < PG_AHEAD; j++) {
-      const long long p = p0 + j * (long long)threads;
-      if (p < taken) {
+      const unsigned p = p0 + j * threads;
+      if (p < (unsigned)taken) {
         const int b = owner_of(first, a.B, (int)p), l = len[b];
         a.table[(long long)b * a.table_stride + held_of(l < 0 ? -1 - l : l) + ((int)p - first[b])] = pg[j];
         hole |= pg[j] < 0;
