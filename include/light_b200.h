@@ -439,7 +439,7 @@ typedef struct lb200_qk_norm_rope_args {
 LB200_API int light_b200_qk_norm_rope(const lb200_qk_norm_rope_args *args, int device, void *stream);
 
 /* out (B, NH, D) = softmax(s) V over the keys [max(0, lens[b] - window), lens[b]) of sequence b (window 0: all), s = scale q.k, with
- * softcap (1e-20 to 1e20, or 0 for none) softcap * tanh(scale q.k / softcap).  lens[b] counts the new token, whose key and value are in the cache already.  A
+ * softcap (1e-20 to 1e20, or 0 for none) softcap * tanh(scale q.k / softcap); |scale| and |scale| / softcap are 1e38 at most.  lens[b] counts the new token, whose key and value are in the cache already.  A
  * sequence without keys, or whose keys all score -inf, gives zeros.  scratch: device memory of light_b200_paged_attn_scratch_bytes or more, 256-byte aligned,
  * uninitialised, which nothing else uses until the call has run; 0 bytes where the call has no use for any. */
 typedef struct lb200_paged_attn_args {

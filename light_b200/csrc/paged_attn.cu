@@ -1385,6 +1385,9 @@ int paged_attn_check(const lb200_paged_attn_args *p) {
       p->table_stride < p->W || !(p->softcap == 0.f || (p->softcap >= 1e-20f && p->softcap <= 1e20f)))
     return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: B %d NH %d KH %d D %d (at most %d) page size %d table %d pages %lld window %d softcap %g", p->B, p->NH, p->KH,
                 p->D, PL_MAX_D, p->page_size, p->W, (long long)p->pages, p->window, (double)p->softcap);
+  // scale log2 e and scale / softcap are f32: infinite, they make NaN of a score of 0
+  if (!(fabsf(p->scale) <= 1e38f) || (p->softcap > 0.f && !(fabsf(p->scale) / p->softcap <= 1e38f)))
+    return fail(LB200_E_SHAPE, "light_b200: paged_decode_attn: scale %g, softcap %g: want a scale, and with a softcap its share of it, up to 1e38", (double)p->scale, (double)p->softcap);
   if ((long long)p->W * p->page_size > 0x7ffffc00ll || p->pages > 0x7fffffffll || (long long)p->B * p->NH > 0x7fffffffll)
     return fail(LB200_E_TOO_LARGE, "light_b200: paged_decode_attn: %d pages of %d rows per sequence, %lld pages, %d x %d heads: want fewer than 2^31 of each", p->W,
                 p->page_size, (long long)p->pages, p->B, p->NH);

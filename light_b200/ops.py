@@ -1102,7 +1102,7 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """Attention of one new token of each sequence over a paged cache (light_b200_paged_decode_attn; ops.DecodeAttention is its counterpart over
     contiguous caches of one position): q (B, NH, D) F32 / BF16 / F16, caches (pages, KH, page size, D) of q's type and any order of page,
     head and row, block_table (B, W) I32, lens (B,) I32 valid keys of each sequence, the new token's among them -> (B, NH, D).  window: the
-    last `window` keys only; softcap (0, or 1e-20 to 1e20): scores softcap * tanh(scale q.k / softcap).  A sequence without keys (or whose scores are all -inf)
+    last `window` keys only; softcap (0, or 1e-20 to 1e20): scores softcap * tanh(scale q.k / softcap); |scale| and |scale| / softcap are 1e38 at most.  A sequence without keys (or whose scores are all -inf)
     gives zeros; lengths beyond the table and pages outside the cache are reported by ops.paged_status.  No gradients."""
     y = _host.paged_attention(q, k_cache, v_cache, block_table, lens, scale, window, softcap)
     if y is not None:
@@ -1123,6 +1123,8 @@ def PagedDecodeAttention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"ops.PagedDecodeAttention: lens must be I32 ({B},) on {q.device}, got {lens.dtype} {tuple(lens.shape)} on {lens.device}")
     if window < 0 or not (softcap == 0 or 1e-20 <= softcap <= 1e20):
         raise ValueError(f"ops.PagedDecodeAttention: window {window}, softcap {softcap}")
+    if not abs(scale) <= 1e38 or (softcap and not abs(scale) / softcap <= 1e38):
+        raise ValueError(f"ops.PagedDecodeAttention: scale {scale}, softcap {softcap}: want a scale, and its share of the softcap, up to 1e38")
     W = block_table.shape[1]
     if max(B, NH, W) >= 1 << 31:
         raise ValueError(f"ops.PagedDecodeAttention: q {tuple(q.shape)}, block_table {tuple(block_table.shape)}: want fewer than 2^31 of each")

@@ -224,3 +224,13 @@ def test_pages_below_zero_are_reported(cuda, B, inplace):
     assert step(-1, 2, False) == ((1, 1, [8, -1], 8), 0)
     assert step(-1, 2, True) == ((1, 1, [8, -1], 8), 8)
     assert step(5, -4, False) == ((1, 1, [-1, 23], 8), 0)
+
+
+def test_attention_refuses_scales_that_overflow(cuda):
+    q, cache = torch.zeros((1, 2, 64), device=cuda), torch.ones((2, 2, 8, 64), device=cuda)
+    table, lens = _i32([[0, 1]], cuda), _i32([9], cuda)
+    for scale, cap in ((1e19, 1e-20), (3e38, 0.0), (math.inf, 0.0), (math.nan, 5.0)):
+        with pytest.raises(ValueError, match="scale"):
+            ops.PagedDecodeAttention(q, cache, cache, table, lens, scale, softcap=cap)
+    for scale, cap in ((1e18, 1e-20), (1e38, 0.0), (-1e38, 1e20), (1e-38, 1e20)):  # all scores 0: the mean of the values
+        assert bool((ops.PagedDecodeAttention(q, cache, cache, table, lens, scale, softcap=cap) == 1).all())
