@@ -362,7 +362,7 @@ PyObject *paged_advance(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
   const int dev = t.t->get_device();
   const int64_t B = t.t->size(0), W = t.t->size(1), cap = f.t->numel();
   NEED(i32_of(*l.t, dev, B) && i32_of(*n.t, dev, B) && i32_of(*c.t, dev, 1) && f.t->dim() == 1 && cap > 0 && cap < (1ll << 31) && i32_of(*f.t, dev, cap));
-  NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31) && tokens >= 0);
+  NEED(B <= LB200_PAGED_MAX_REQUESTS && W < (1ll << 31) && page > 0 && page < (1ll << 31) && tokens >= 0 && tokens < (1ll << 31));
   const at::Tensor whole = fresh({16 * tokens + 4 * (3 * B + 2)}, at::kByte, dev);
   const int64_t ints = 16 * tokens;
   at::Tensor pos = piece(whole, 0, {tokens}, at::kLong), slots = piece(whole, 8 * tokens, {tokens}, at::kLong);

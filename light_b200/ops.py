@@ -956,8 +956,8 @@ def PagedAdvance(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.
         return PagedStep(*r[:3], lens, r[4], free_count) if inplace else PagedStep(*r)
     dev, B, a = _pages_args("PagedAdvance", block_table, lens, free_pages, free_count, page_size)
     _i32("PagedAdvance", block_table.device, new_lens=new_lens)
-    if new_lens.numel() != B or tokens < 0:
-        raise ValueError(f"ops.PagedAdvance: new_lens {tuple(new_lens.shape)} for {B} requests, {tokens} tokens")
+    if new_lens.numel() != B or not 0 <= tokens < 1 << 31:
+        raise ValueError(f"ops.PagedAdvance: new_lens {tuple(new_lens.shape)} for {B} requests, {tokens} tokens (fewer than 2^31)")
     rows = torch.empty((2, tokens), dtype=torch.int64, device=lens.device)
     ints = torch.empty(3 * B + 2, dtype=torch.int32, device=lens.device)
     starts, granted = ints[:B + 1], ints[B + 1:2 * B + 1]

@@ -234,3 +234,11 @@ def test_attention_refuses_scales_that_overflow(cuda):
             ops.PagedDecodeAttention(q, cache, cache, table, lens, scale, softcap=cap)
     for scale, cap in ((1e18, 1e-20), (1e38, 0.0), (-1e38, 1e20), (1e-38, 1e20)):  # all scores 0: the mean of the values
         assert bool((ops.PagedDecodeAttention(q, cache, cache, table, lens, scale, softcap=cap) == 1).all())
+
+
+@pytest.mark.parametrize("tokens", [1 << 31, 1 << 40, 1 << 60, 1 << 63])
+def test_advance_refuses_more_tokens_than_it_counts_before_it_allocates(cuda, tokens):
+    held = torch.cuda.memory_reserved()
+    with pytest.raises(ValueError, match="PagedAdvance"):
+        ops.PagedAdvance(_i32([[0, 1]], cuda), _i32([0], cuda), _i32([1], cuda), _i32([2], cuda), _i32([1], cuda), 16, tokens)
+    assert torch.cuda.memory_reserved() - held < 1 << 30
