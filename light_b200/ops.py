@@ -1011,8 +1011,8 @@ def RoPEFrequencies(rotary: int, base: float, scaling: Optional[str] = None, fac
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         freq = freq * keep + freq / factor * (1 - keep)
     elif scaling == "yarn":
-        if not base > 1:
-            raise ValueError(f"ops.RoPEFrequencies: yarn scaling needs a base above 1, got {base}")
+        if not base > 1 or not beta_fast > beta_slow > 0:
+            raise ValueError(f"ops.RoPEFrequencies: yarn scaling needs a base above 1 and beta_fast above beta_slow above 0, got {base}, {beta_fast}, {beta_slow}")
         at = [rotary * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (beta_fast, beta_slow)]  # the pair that turns so often
         first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary - 1)
         keep = 1 - ((i / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)

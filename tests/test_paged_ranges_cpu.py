@@ -27,3 +27,9 @@ def test_attention_entry_refuses_scales_that_overflow(scale, softcap):
     assert _lib.lib().light_b200_paged_attn_scratch_bytes(C.byref(a), 0) == 0
     assert _lib.lib().light_b200_paged_decode_attn(C.byref(a), 0, None) == -2
     assert "scale" in _lib.last_error()
+
+
+@pytest.mark.parametrize("beta", [dict(beta_fast=0.0), dict(beta_slow=0.0), dict(beta_fast=1.0, beta_slow=32.0), dict(beta_fast=2.0, beta_slow=2.0), dict(beta_fast=float("nan"))])
+def test_yarn_refuses_turns_in_no_order(beta):
+    with pytest.raises(ValueError, match="RoPEFrequencies"):
+        ops.RoPEFrequencies(16, 10000.0, "yarn", 4.0, original=4096, device="cpu", **beta)
