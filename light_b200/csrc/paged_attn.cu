@@ -143,12 +143,12 @@ __global__ void __launch_bounds__(PL_WARPS * 32) paged_attn_any_kernel(PagedArgs
 //     without a key are filled with zeros: a weight of 0 times what lies there must not be NaN.
 //   * Pieces of a unit that was cut are joined in their order, first those of a CTA's warps at its end, in shared memory; what goes on
 //     over CTAs goes to scratch, at most two pieces a CTA, and a second launch joins those: no atomics, the same bits every time.
-// Bound by the memory where sequences are long: one of 131072 keys (537 MB, bf16) 88 us, 6.1 TB/s; eight of 8192 in f32 (537 MB) 90 us.  Of
+// Bound by the memory where sequences are long: one of 131072 keys (537 MB, bf16) 89 us, 6.1 TB/s; eight of 8192 in f32 (537 MB) 90 us.  Of
 // shorter ones by what a launch costs beside its stream: 64 ragged ones (232 MB) 45 us, of which about 6 are the chain of lengths,
 // schedule, pages and first rows (2000 + 1500 + 2000 + 2500 cycles) and 4 the join.
 //   * One wave of CTAs: two, three and four waves of finer runs take 98, 102 and 108 us for the one long sequence, each wave that chain again.
-//   * UNIT 3: 1, 2, 5, 8 give 49.7, 44.5, 45.1, 45.0 us for the 64, and 18.4, 17.6, 20.9, 24.3 for 200 of 300 keys at most (3: 45.2, 18.0; all of it
-//     before the maximum's slack).
+//   * UNIT 3.  1, 2, 3, 5, 8 give (us) 50.8, 44.2, 44.3, 44.9, 45.0 for the 64; 18.3, 17.2, 17.7, 20.5, 23.8 for 200 of 300 keys at most; 22.2, 21.3, 20.9,
+//     20.4, 20.3 for 33 in f16 with a window; the same for the long ones.  So 2 is the better by 3 % for short sequences, and worse by 2 % under a window.
 //   * All four warps of a CTA on the blocks of one unit in turn, with barriers, took 75 us for the 64: two microseconds a unit.
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, UNIT = 3, CLUSTER_BLOCKS = 4, CLUSTER_WIDE = 8;
 
@@ -222,14 +222,16 @@ __device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t 
 // bf16 / f16: a block of 16 keys on mma.sync (m16n8k16, f32 sums).  tcgen05 has no use here: its smallest tile has 128 rows, a unit 1 to 16.
 //   S^T = K Q^T: the keys are the rows, the query heads the 8 (or twice 8) columns; O^T += V^T P^T: the dims are the rows.  Both operands come
 //   from the ring by ldmatrix, plain and transposed; P^T is S^T with its 8 x 8 tiles turned by movmatrix, in registers.
-//   A block of 128 dims is about 340 instructions of a warp (of 400, with a maximum every block, it took 0.65 us by itself); eight warps of an SM
+//   A block of 128 dims is about 380 instructions of a warp (of 400, with a maximum every block, it took 0.65 us by itself); eight warps of an SM
 //   fold 8 KB each in 1.4 us, which is the memory's rate.
 //   A weight goes in as two elements of the cache's type, as the instruction wants it, right to 2^-15 (bf16; f16: 2^-21, or 2^-25 of 1) of itself: rounded to
-//   one, its 2^-8 (2^-11) stood out wherever values cancel, and two products instead of one cost little, the tensor pipe being idle for the most part.
+//   one, its 2^-8 (2^-11) stood out wherever values cancel, and two products instead of one cost little, the tensor pipe being idle for the most part (64 ragged
+//   sequences 44.5 -> 44.8 us; 33 in f16 with a window 20.4 -> 21.7, where the instructions count).
 //   The sum below the fraction adds the f32 weights.
 //   f16 has them 2^11 times larger (2^15 at most, with a slack of 2^4; numerator and denominator share the factor, in all pieces), so that it keeps them down to
 //   2^-25 of the largest to 2^-11 of themselves.  A block with one below that has more products (fold_light): where a key holds nearly all the weight and its
-//   value little, the answer is the sum of many that are lighter than any f16.
+//   value little, the answer is the sum of many that are lighter than any f16.  (16 sequences of 8192 keys: 90 us, with a heavy key in every block 96; by f32
+//   products, as fold_plain has them, 193.)
 template <typename T_, int DP_, int NT>
 struct MmaBlock {
   using T = T_;
@@ -237,7 +239,8 @@ struct MmaBlock {
   static constexpr bool HALF = std::is_same<T, __half>::value;
   // Weights are 2^(score - m) for an m that follows the running maximum only when a score is above it by more than SLACK: one vote a block instead of the
   // maximum's shuffles and the corrections (64 ragged sequences 45.1 -> 44.5 us, 33 with a window 19.6 -> 18.8; f32, whose heads' maxima take three
-  // shuffles: 11.2 -> 11.6 for 4 x 1024).  Weights reach 2^SLACK, and the largest is 1 or more, as with the maximum itself.
+  // shuffles: 11.2 -> 11.6 for 4 x 1024; all of it before weights had two halves).  Weights reach 2^SLACK, and the largest is 1 or more, as with the maximum
+  // itself.  2^4 for f16, which leaves its weights four binades more below the largest.
   static constexpr float SLACK = HALF ? 4.f : 8.f, UP = HALF ? 15.f - SLACK : 0.f;
   uint32_t q[DP / 16][NT][2];
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
@@ -1296,6 +1299,8 @@ Cut cut_of(const lb200_paged_attn_args *p) {
   // A cluster to a unit where all are resident at once and a warp has CLUSTER_BLOCKS blocks at most.  Up to there it is the faster one whatever
   // the lengths (bf16, 8 KV heads, us of the split kernel and of this one: 1 x 2048 keys 7.9, 6.2; 4 x 1024 9.2, 6.8; 16 x 512 12.1, 10.6);
   // with more blocks it gains less on sequences of one length (4 x 4096: 18.7, 16.9) than it loses on others (4 x 8192 ragged: 12.5, 21.2).
+  // The table's width stands for the lengths here, which the host does not know: under a table for 8192 tokens or more 1 x 1024 keys take 8.2 us instead of
+  // 5.1, 4 x 1024 9.2 instead of 6.4, 16 x 512 12.1 instead of 9.0.
   const long long n_units = (long long)p->B * p->KH * c.groups;
   for (c.ks = 1; c.ks < 8 && n_units * (c.ks + 1) <= slots && blocks > c.ks * PA_WARPS;) c.ks++;
   if (c.ks == 8 && n_units <= CLUSTER_WIDE && blocks > 8 * PA_WARPS) c.ks = 16;  // (1 x 2048: 7.2 -> 6.2, 1 x 4096: 10.7 -> 8.4)

@@ -14,8 +14,8 @@ __device__ unsigned int g_step_status = 0;
 // the stack does not hold gets none, and as first_b never falls, none after it that needs any.  Token i of the batch belongs to the
 // request with starts_b <= i < starts_{b + 1}: a binary search in shared memory.
 //
-// Two dependent reads (the lengths; then the stack or the table) and the stores bound it: latency.  A step of 256 requests 3.5 us, 43000 tokens of
-// 48 prompts 5.3, the return of 900 requests' 95000 pages 5.2.  Every CTA scans the lengths for itself and stores its share.  Where lengths and
+// Two dependent reads (the lengths; then the stack or the table) and the stores bound it: latency.  A step of 256 requests 3.6 us, 43000 tokens of
+// 48 prompts 5.4, the return of 900 requests' 95000 pages 5.2.  Every CTA scans the lengths for itself and stores its share.  Where lengths and
 // counter are updated in place the CTAs are one cluster, with its barrier between the scan and the stores; else any number of them.
 constexpr int PG_THREADS = 1024, PG_MAX_B = LB200_PAGED_MAX_REQUESTS, PG_AHEAD = 4;  // entries of a thread that are on their way together
 
@@ -757,8 +757,11 @@ int qk_norm_rope(const lb200_qk_norm_rope_args *p, cudaStream_t st) {
     const int lanes = p->interleaved ? ch.first : ch.first + (ch.count - 2 * ch.first + 1) / 2;
     for (ch.lg = 1; ch.lg < lanes;) ch.lg *= 2;
     if (ch.lg <= 32) {
-      // Warps per token: one that has its angles for all heads; two, of fewer than twelve tokens for every SM (1037 tokens of 48 F32 heads: 13.2 ->
-      // 9.7 us); of fewer than four, as many as have one to four rounds of one kind each, until there are eight for every SM.
+      // Warps per token: one that has its angles for all heads; two, of fewer than twelve tokens for every SM; of fewer than four, as many as have one to four
+      // rounds of one kind each, until there are eight for every SM.  Heads of 128, us with one warp and with two: bf16, 1000 tokens of 48 heads 9.9, 7.7, of
+      // 8 heads 6.3, 5.3; F32, 1400 of 48 15.7, 12.3, of 24 9.2, 7.3; beyond the rule (2500) bf16 17.0, 19.5, F32 22.4, 22.6.  It is the worse side for 1400 bf16
+      // tokens (48 heads 10.2, 12.7; 8 heads 6.6, 9.5: the second warps no longer fit on the SMs), for 600 F32 tokens of 8 heads (4.9, 5.4) and beyond it for
+      // 3500 F32 tokens of 48 (35.2, 31.9).
       const int per = 32 / ch.lg, rq = (p->NH + per - 1) / per, rk = (p->KH + per - 1) / per, kinds = p->slots ? 3 : 2;
       ch.split = p->T < 12ll * sm_count() ? 2 : 1, ch.q_parts = ch.k_parts = 0;
       if (p->T < 4ll * sm_count())
